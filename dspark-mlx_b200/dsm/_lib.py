@@ -25,7 +25,9 @@ STAGE_PITCH = 160
 DEVICE_ERRORS = {0x10: "expert id out of range", 0x11: "token id out of range",
                  0x12: "pipeline wait ran out of its time budget",
                  0x13: "an expert-parallel peer did not signal in time",
-                 0x14: "more expert-parallel rows than the exchange buffer holds"}
+                 0x14: "more expert-parallel rows than the exchange buffer holds",
+                 0x15: "a KV cache page or slot outside the pool, or a length past its block table",
+                 0x16: "the paged KV cache ran out of pages, block table or step rows"}
 
 EXPORTED = (
     "dsm_abi_version", "dsm_status_string", "dsm_last_error_message", "dsm_device_error",
@@ -42,6 +44,7 @@ EXPORTED = (
     "dsm_qkv_norm_rope", "dsm_gqa_attn_workspace_bytes", "dsm_gqa_attn", "dsm_set_attn_kernel",
     "dsm_linear_splitk_workspace_bytes", "dsm_linear_splitk", "dsm_add_rms_norm",
     "dsm_grouped_linear", "dsm_grouped_linear_splitk",
+    "dsm_paged_extend", "dsm_paged_trim", "dsm_kv8_append", "dsm_gqa_attn_kv8_workspace_bytes", "dsm_gqa_attn_kv8",
 )
 
 
@@ -86,6 +89,21 @@ class HeadDesc(ctypes.Structure):
         ("markov_w1", c_void_p), ("markov_w2", c_void_p),
         ("conf_w", c_void_p),
         ("conf_bias", c_float),
+    ]
+
+
+class KV8AttnDesc(ctypes.Structure):
+    """``dsm_kv8_attn_desc`` (field order and types follow the C struct)."""
+
+    _fields_ = [
+        ("q_batch_stride", c_int64), ("q_row_stride", c_int64), ("q_head_stride", c_int64),
+        ("bk_batch_stride", c_int64), ("bk_head_stride", c_int64), ("bk_row_stride", c_int64),
+        ("bv_batch_stride", c_int64), ("bv_head_stride", c_int64), ("bv_row_stride", c_int64),
+        ("table_stride", c_int64),
+        ("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("dtype", c_int), ("batch", c_int), ("block", c_int), ("n_heads", c_int), ("n_kv", c_int),
+        ("head_dim", c_int), ("page_size", c_int), ("n_pages", c_int), ("max_pages", c_int),
+        ("scale", c_float),
     ]
 
 
@@ -155,6 +173,11 @@ def _declare(lib):
         "dsm_add_rms_norm": (I, [V, V, I, I64, I, V, F, V, V, V]),
         "dsm_grouped_linear": (I, [V, V, I64, I, I, I, V, I, V, I, V, I, V, I64, V]),
         "dsm_grouped_linear_splitk": (I, [V, V, I64, I, I, I, V, I, V, I, V, I, V, I64, V, S, V]),
+        "dsm_paged_extend": (I, [V, V, I, I, V, I64, I, V, V, I, V, V, V, I64, V]),
+        "dsm_paged_trim": (I, [V, V, I, I, V, I64, I, V, V, I, V]),
+        "dsm_kv8_append": (I, [V, V, I, I64, I, I, I64, I64, I64, I64, V, I, I, V, V, V, V, V]),
+        "dsm_gqa_attn_kv8_workspace_bytes": (S, [I, I, I, I, I]),
+        "dsm_gqa_attn_kv8": (I, [POINTER(KV8AttnDesc), V, V, V, V, V, V, V, S, V]),
         "dsm_stage_rows_hilo": (I, [V, I64, I, V, I64, V, V]),
         "dsm_moe_workspace_bytes": (S, [POINTER(MoEDesc)]),
         "dsm_moe_forward": (I, [POINTER(MoEDesc), V, I, V, I, I64, V, V, V, V, S, V]),

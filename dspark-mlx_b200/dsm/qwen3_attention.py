@@ -12,7 +12,10 @@ Same constructor (``Qwen3DSparkAttention(args)``), parameter names (``q_proj``, 
   rows ``row0 ..`` of preallocated ``[b, n_kv, cap, head_dim]`` caches instead;
 * ``attend_cached(noise, ctx_k, ctx_v, cos, sin)``: the block over cached context K/V
   (``None`` for none; any view whose rows are ``head_dim`` contiguous values) and its own
-  rows (``qwen3.py:130-143``).
+  rows (``qwen3.py:130-143``);
+* ``append_paged(proj_ctx, cos, sin, cache, layer, rows)`` and ``attend_paged(noise, cache, layer,
+  cos, sin)``: the same two over a :class:`dsm.paged_cache.PagedKVCache`, whose sequences have
+  lengths of their own (no reference counterpart).
 
 The projections are ``Projection``s, dense or MLX affine after ``quantize`` as
 ``quantize_drafter`` leaves them, on ``dsm_linear`` (quantised ones on
@@ -33,6 +36,7 @@ from torch import nn
 
 from ._lib import check, dtype_code, lib, ptr, stream_ptr
 from .block import RMSNorm
+from .paged_cache import PagedKVCache, PagedRows
 from .qwen3 import Projection
 from .weights import pack
 
@@ -276,3 +280,44 @@ class Qwen3DSparkAttention(nn.Module):
         bv = torch.empty_like(bk)
         qh = self._heads(noise, dt, True, cos, sin, 0, bk, bv, q, 0)
         return self._out(self._attend(qh, ctx_k, ctx_v, bk, bv, dt), dt)
+
+    def _check_cache(self, cache: PagedKVCache, x: torch.Tensor) -> None:
+        if (cache.n_kv, cache.head_dim) != (self.nkv, self.hd):
+            raise ValueError(f"the cache holds {cache.n_kv} heads of {cache.head_dim}, the attention {self.nkv} of "
+                             f"{self.hd}")
+        if cache.lengths.device != x.device:
+            raise ValueError(f"the cache is on {cache.lengths.device}, the input on {x.device}")
+
+    def append_paged(self, proj_ctx: torch.Tensor, cos, sin, cache: PagedKVCache, layer: int, rows: PagedRows) -> None:
+        """Projected context rows ``[max_rows, hidden]`` of ``rows = cache.extend(...)`` into layer
+        ``layer`` of the cache, in 8 bits; ``cos`` / ``sin`` ``[max_rows, head_dim]`` are the RoPE table rows of
+        ``rows.positions``. Rows without a slot are projected and dropped."""
+        if proj_ctx.dim() != 2:
+            raise ValueError(f"proj_ctx must be [rows, {self.hidden}], got {tuple(proj_ctx.shape)}")
+        self._check_cache(cache, proj_ctx)
+        if rows.slot_map.shape[0] != proj_ctx.shape[0]:
+            raise ValueError(f"{proj_ctx.shape[0]} rows for a slot map of {rows.slot_map.shape[0]}")
+        with torch.cuda.device(cache.lengths.device):
+            k, v = self.context_kv(proj_ctx[None], cos, sin)
+            cache.append(layer, k[0].transpose(0, 1), v[0].transpose(0, 1), rows)
+
+    def attend_paged(self, noise: torch.Tensor, cache: PagedKVCache, layer: int, cos, sin) -> torch.Tensor:
+        """``attend_cached`` over the sequences' cached rows: ``noise`` ``[batch, q, hidden]``, ``cos`` /
+        ``sin`` ``[batch * q, head_dim]``, the table rows of each block token's position (they differ between
+        sequences)."""
+        self._check_cache(cache, noise)
+        with torch.cuda.device(cache.lengths.device):
+            noise, dt = self._prep(noise, "noise")
+            b, q, _ = noise.shape
+            if b != cache.lengths.shape[0]:
+                raise ValueError(f"{b} sequences over a cache of {cache.lengths.shape[0]}")
+            cos, sin = self._tables(cos, sin, noise.device)
+            if cos.shape[0] != b * q:
+                raise ValueError(f"cos/sin must have batch * q = {b * q} rows, got {cos.shape[0]}")
+            # every row has a position of its own: one sequence of b * q rows to the RoPE, [b, q] to the attention
+            bk = torch.empty(1, self.nkv, b * q, self.hd, dtype=dt, device=noise.device)
+            bv = torch.empty_like(bk)
+            qh = self._heads(noise.reshape(1, b * q, -1), dt, True, cos, sin, 0, bk, bv, b * q, 0)
+            blk_k, blk_v = (t.view(self.nkv, b, q, self.hd).transpose(0, 1) for t in (bk, bv))
+            o = cache.attend(layer, qh.view(b, q, self.nh, self.hd), blk_k, blk_v, scale=self.scale)
+            return self._out(o, dt)

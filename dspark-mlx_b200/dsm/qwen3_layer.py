@@ -10,7 +10,9 @@ Same constructor (``Qwen3DSparkLayer(args)``), parameter names (``self_attn``, `
 * ``context_kv(proj_ctx, cos, sin)``: the attention's cached context K/V, no norm
   (``qwen3.py:171-172``);
 * ``forward_cached(hidden, ctx_k, ctx_v, cos, sin)``: the same over cached context K/V
-  (``qwen3.py:174-176``).
+  (``qwen3.py:174-176``);
+* ``append_paged`` / ``forward_paged``: both over a :class:`dsm.paged_cache.PagedKVCache`, whose
+  sequences have lengths of their own (no reference counterpart).
 
 The attention is :class:`dsm.qwen3_attention.Qwen3DSparkAttention`, the MLP
 :class:`dsm.qwen3.Qwen3MLP` (``quantize`` quantises both as ``quantize_drafter`` does). The
@@ -33,6 +35,7 @@ from torch import nn
 
 from ._lib import check, dtype_code, lib, ptr, stream_ptr
 from .block import RMSNorm
+from .paged_cache import PagedKVCache, PagedRows
 from .qwen3 import Projection, Qwen3MLP
 from .qwen3_attention import Qwen3DSparkAttention, _get
 
@@ -100,6 +103,16 @@ class Qwen3DSparkLayer(nn.Module):
         hidden = self._check(hidden)
         _, x = self._norm(hidden, self.input_layernorm)
         return self._finish(hidden, self.self_attn.attend_cached(x, ctx_k, ctx_v, cos, sin))
+
+    def append_paged(self, proj_ctx: torch.Tensor, cos, sin, cache: PagedKVCache, layer: int, rows: PagedRows) -> None:
+        self.self_attn.append_paged(proj_ctx, cos, sin, cache, layer, rows)
+
+    def forward_paged(self, hidden: torch.Tensor, cache: PagedKVCache, layer: int, cos, sin) -> torch.Tensor:
+        """``forward_cached`` over the sequences' cached rows: ``cos`` / ``sin`` ``[batch * q, head_dim]``."""
+        hidden = self._check(hidden)
+        with torch.cuda.device(hidden.device):
+            _, x = self._norm(hidden, self.input_layernorm)
+            return self._finish(hidden, self.self_attn.attend_paged(x, cache, layer, cos, sin))
 
 
 class Qwen3Backbone(nn.Module):

@@ -42,6 +42,9 @@
  *                       attend_cached around dsm_linear (arch/qwen3.py:64-143)
  *   dsm_add_rms_norm    the residual adds and RMSNorms of Qwen3DSparkLayer (arch/qwen3.py:157-176)
  *   dsm_gather_rows     the draft block's embedding rows (block.py:97-101)
+ *   dsm_paged_extend, dsm_paged_trim, dsm_kv8_append, dsm_gqa_attn_kv8: the paged 8-bit form of the
+ *                       context caches that Qwen3DSparkDrafter.extend_context grows densely
+ *                       (arch/qwen3.py:122-143, 287-296); no counterpart of their own.
  *   dsm_ep_*            expert parallelism over peer stores; the reference runs on one device
  *                       (tests/reference_model.py:55-56 forces world_size 1) and has no
  *                       counterpart.
@@ -70,6 +73,8 @@ extern "C" {
 #define DSM_DEV_ERR_PIPELINE_TIMEOUT 0x12
 #define DSM_DEV_ERR_PEER_TIMEOUT 0x13   /* an expert-parallel peer did not signal within ~2 s */
 #define DSM_DEV_ERR_CAPACITY 0x14       /* more expert-parallel rows than the exchange buffer holds */
+#define DSM_DEV_ERR_PAGE_RANGE 0x15     /* a cache page or slot outside the pool, or a length past its block table */
+#define DSM_DEV_ERR_PAGES_SHORT 0x16    /* a step of the paged cache needs more pages, table or rows than there are */
 
 /* element types */
 #define DSM_DT_F32 0
@@ -365,6 +370,75 @@ int dsm_set_attn_kernel(int kernel);
  * not both NULL. dim <= 49152. */
 int dsm_add_rms_norm(const void* x, const void* delta, int dtype, int64_t n_rows, int dim, const float* weight,
                      float eps, void* sum_out, void* norm_out, void* stream);
+
+/* ---- the paged 8-bit KV cache ------------------------------------------------------------------
+ * A pool of n_pages pages of page_size tokens (a multiple of 64, at most 1024); sequence i of a
+ * batch (at most 8192) has its tokens [j * page_size, (j + 1) * page_size) in page
+ * block_table[i * table_stride + j], j < max_pages <= 2^20. Everything that depends on lengths is
+ * read on the GPU: no call synchronises, and a captured step replays as lengths change.
+ *
+ * paged_extend: sequence i grows from lengths[i] by new_len[i] tokens. The pages that it lacks come
+ *   off the top of the stack free_pages[0 .. *n_free) (capacity n_pages) in order of sequences:
+ *   with off_i the pages taken by sequences before i, its k-th new page is
+ *   free_pages[*n_free - 1 - off_i - k]. Writes the new block table entries, lengths, *n_free,
+ *   cu_rows [batch + 1] (first row of each sequence, in the order of the batch), and for each of
+ *   max_rows rows slot_map = page * page_size + offset and positions = index in the sequence;
+ *   rows behind the last sequence get slot -1, position 0. A sequence that cannot be served (a
+ *   negative length, more tokens than its table or int32 holds, no pages or rows left, or a
+ *   sequence before it ran out of either) keeps its length; its rows get slot -1, position 0, and
+ *   the error word is set (DSM_DEV_ERR_PAGES_SHORT).
+ * paged_trim: sequence i shrinks to min(lengths[i], max(keep_len[i], 0)) tokens. Surplus pages go
+ *   back on the stack in the mirrored order, so that a trim to the lengths before an extend
+ *   restores the stack. Table entries behind a sequence's pages are left as they are. If more
+ *   pages came back than the pool holds, nothing is changed and the error word is set.
+ *   Both: all buffers int32 but slot_map; the buffers of one call must not overlap.
+ *
+ * kv8_append: rows k, v (element r * row_stride + h * head_stride + d; F32 or BF16) into the slots
+ *   slot_map[r] of the cache, as e4m3 codes with one power-of-two scale per page and KV head:
+ *   2^e, the least e in [-120, 120] with max|x| <= 448 * 2^e over the page's rows. A page whose
+ *   token 0 is among the rows starts afresh; otherwise its scale never shrinks, and where it grows
+ *   the codes there are rounded again at the new scale. What is not finite takes no part in the
+ *   scale and is stored as NaN. Rows with slot -1 are skipped; slots outside the pool too, with the
+ *   error word set (DSM_DEV_ERR_PAGE_RANGE). Rows of one page must be neighbours in the slot map
+ *   (as paged_extend leaves them), each slot given once.
+ *   k_codes [n_pages, n_kv, page_size, head_dim]: from head_dim 128 on, 16-byte chunk c of token
+ *   t's row sits at chunk c ^ (t & 7). v_codes [n_pages, n_kv, page_size / 64, head_dim, 64].
+ *   k_scale, v_scale [n_pages, n_kv] fp32. head_dim 64, 128 or 256; codes 16-byte aligned.
+ *
+ * gqa_attn_kv8: out [batch, block, n_heads * head_dim] (dtype) = softmax(q k^T * scale) v per
+ *   query head h over KV head h / (n_heads / n_kv): the lengths[i] cached rows of sequence i and,
+ *   unless blk_k is NULL, the block's own rows, with no mask. A sequence without any row gives
+ *   zeros. Lengths below 0 count as 0; a length past the table is cut to it, and a page outside
+ *   the pool counts as absent, both with DSM_DEV_ERR_PAGE_RANGE. What the cache holds behind a
+ *   sequence's length is never read as a number. Strides are in elements; head_dim values of a
+ *   row are contiguous. workspace: dsm_gqa_attn_kv8_workspace_bytes, 16-byte aligned. */
+typedef struct dsm_kv8_attn_desc {
+  int64_t q_batch_stride, q_row_stride, q_head_stride;
+  int64_t bk_batch_stride, bk_head_stride, bk_row_stride;
+  int64_t bv_batch_stride, bv_head_stride, bv_row_stride;
+  int64_t table_stride;
+  const void* k_codes;
+  const void* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  int dtype, batch, block, n_heads, n_kv, head_dim;
+  int page_size, n_pages, max_pages;
+  float scale;
+} dsm_kv8_attn_desc;
+int dsm_paged_extend(int32_t* lengths, const int32_t* new_len, int batch, int page_size, int32_t* block_table,
+                     int64_t table_stride, int max_pages, const int32_t* free_pages, int32_t* n_free, int n_pages,
+                     int32_t* cu_rows, int64_t* slot_map, int32_t* positions, int64_t max_rows, void* stream);
+int dsm_paged_trim(int32_t* lengths, const int32_t* keep_len, int batch, int page_size, const int32_t* block_table,
+                   int64_t table_stride, int max_pages, int32_t* free_pages, int32_t* n_free, int n_pages,
+                   void* stream);
+int dsm_kv8_append(const void* k, const void* v, int dtype, int64_t n_rows, int n_kv, int head_dim,
+                   int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                   const int64_t* slot_map, int page_size, int n_pages, uint8_t* k_codes, uint8_t* v_codes,
+                   float* k_scale, float* v_scale, void* stream);
+size_t dsm_gqa_attn_kv8_workspace_bytes(int batch, int block, int n_heads, int n_kv, int head_dim);
+int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* desc, const void* q, const int32_t* block_table, const int32_t* lengths,
+                     const void* blk_k, const void* blk_v, void* out, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 /* Kernel regime of the grouped expert products: 0 (default) picks by rows per busy
  * expert -- the mma.sync weight-streaming kernel at decode sizes, the tcgen05/TMEM kernel

@@ -1,0 +1,675 @@
+"""The paged 8-bit KV cache on the GPU against its oracle (``oracle/paged_cache_oracle.py``).
+
+Page tables and stored codes have to be equal. The attention's bound is derived from its
+arithmetic. With u the type's half step (bf16 2^-8, fp32 2^-24), S = max sum_d |q_d k_d| * scale
+and V = max |v| of a sequence:
+
+* the result is rounded once: u |o|;
+* a score that is off by ds moves each weight by a factor of e^ds, numerator and denominator alike:
+  at most 2 ds V. bf16 calls split q and the weights into two e4m3 terms each. q: a term's half step
+  is 2^-4 of its value, so two leave 2^-8 |q_d|, and 2^-10 of e4m3's unit (its smallest step 2^-9,
+  halved) of a row scaled to at least 224: 2^-17 max |q|; the products are exact and their fp32 sums
+  add less than 2^-18 S. So ds <= (2^-8 + 2^-18) S in the worst case; but bf16's q has 8
+  significant bits, a first term takes 4, the residual at most 4 with its sign, and is exact where it
+  reaches e4m3's normals: 2^-17 max|q| sum|k| scale is what is left, held below 2^-17 * head_dim * S;
+* the weights' two terms leave 2^-8 of each, and 2^-18 of the largest of 64: at most
+  (2^-8 + 2^-12) V, and their sum is taken before the rounding;
+* fp32 calls split into two f16 terms (2^-22 each), or use fp32 products: ds <= (2^-21 + (hd + 8)
+  2^-24) S, weights 2^-21 + (n / 32 + 64) 2^-24 for n summed rows.
+"""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+import oracle
+from dsm import _lib
+from dsm import paged_cache as pc
+from oracle import paged_cache_oracle as po
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------- page tables
+def _tables_case(seed, b, page, longest, new_most, pool_extra, most=None, extra_cols=0):
+    r = random.Random(seed)
+    lengths = [r.choice([0, 1, page - 1, page, page + 1, r.randint(0, longest)]) for _ in range(b)]
+    new = [r.choice([0, 0, 1, 2, page, r.randint(0, new_most)]) for _ in range(b)]
+    need = [-(-n // page) for n in lengths]
+    n_pages = sum(need) + pool_extra
+    pool = list(range(n_pages))
+    r.shuffle(pool)
+    most = most or max(-(-(a + c) // page) for a, c in zip(lengths, new)) + 1
+    table = [[-7] * most for _ in range(b)]
+    for i, n in enumerate(need):
+        for j in range(n):
+            table[i][j] = pool.pop()
+    free = pool + [-3] * (n_pages - len(pool))
+    wide = torch.full((b, most + extra_cols), -9, dtype=torch.int32)
+    wide[:, :most] = torch.tensor(table)
+    return lengths, new, table, free, len(pool), wide.to(DEV)[:, :most]
+
+
+def _run_extend(lengths, new, table_gpu, free, n_free, page, max_rows):
+    L, F, N = i32(lengths), i32(free), i32([n_free])
+    rows = pc.paged_extend(L, i32(new), table_gpu, F, N, page, max_rows)
+    return L, F, N, rows
+
+
+@pytest.mark.parametrize("b,page,longest,new_most,tail,extra_cols", [
+    (1, 64, 300, 5, 0, 0), (1, 64, 0, 5000, 3, 0), (7, 128, 1000, 9, 5, 3), (61, 64, 700, 200, 40, 0),
+    (513, 64, 300, 4, 1, 0), (1025, 256, 900, 300, 7, 5), (8192, 64, 130, 2, 100, 0),
+])
+def test_extend_and_trim_match_the_oracle(b, page, longest, new_most, tail, extra_cols):
+    """One token to long prompts, one CTA and a cluster, one scan block and several, a strided table."""
+    lengths, new, table, free, n_free, tg = _tables_case(b, b, page, longest, new_most, 3 * b + 200 + b * new_most // page,
+                                                         extra_cols=extra_cols)
+    max_rows = sum(new) + tail
+    want = po.paged_extend(lengths, new, table, free, n_free, page, max_rows)
+    assert not want[6]
+    L, F, N, rows = _run_extend(lengths, new, tg, free, n_free, page, max_rows)
+    assert L.tolist() == want[0] and tg.tolist() == want[1] and N.tolist() == [want[2]]
+    assert rows.cu_rows.tolist() == want[3] and rows.slot_map.tolist() == want[4]
+    assert rows.positions.tolist() == want[5] and F.tolist() == free
+    # back to a mix of lengths: kept whole, cut, released, asked for more than there is
+    r = random.Random(5)
+    keep = [r.choice([n, n // 2, 0, n + 9, -4, max(0, n - 1)]) for n in want[0]]
+    back = po.paged_trim(want[0], keep, want[1], free, want[2], page)
+    pc.paged_trim(L, i32(keep), tg, F, N, page)
+    assert L.tolist() == back[0] and F.tolist() == back[1] and N.tolist() == [back[2]] and not back[3]
+    assert tg.tolist() == want[1]
+    assert _lib.device_error() == 0
+
+
+def test_extend_then_trim_to_the_old_lengths_restores_everything_but_the_table():
+    lengths, new, table, free, n_free, tg = _tables_case(3, 40, 64, 500, 100, 200)
+    L, F, N, _ = _run_extend(lengths, new, tg, free, n_free, 64, sum(new))
+    pc.paged_trim(L, i32(lengths), tg, F, N, 64)
+    assert (L.tolist(), F.tolist(), N.tolist()) == (lengths, free, [n_free])
+
+
+@pytest.mark.parametrize("short", ["pages", "rows", "table", "negative length", "negative rows", "int32"])
+def test_extend_leaves_out_what_does_not_fit(short):
+    """Who finds no pages, rows or table keeps its length and gets no slots; those before it, and
+    those after it that need nothing more, are served. The error word says so."""
+    page = 64
+    lengths, new, table, free, n_free, tg = _tables_case(11, 30, page, 300, 150, 60)
+    new = [max(1, n) for n in new]
+    lengths[4], new[4] = 10, 3  # fits its last page
+    table[4][0] = table[4][0] if table[4][0] >= 0 else 0
+    max_rows = sum(new)
+    if short == "pages":
+        n_free = 7
+    elif short == "rows":
+        max_rows = sum(new) // 2
+    elif short == "table":
+        most = 3
+        lengths = [min(n, most * page) for n in lengths]
+        table = [row[:most] for row in table]
+    elif short == "negative length":
+        lengths[2] = -5
+    elif short == "negative rows":
+        new[2] = -5
+    else:
+        new[2] = 2 ** 31 - 1
+    tg = i32(table)
+    want = po.paged_extend(lengths, new, table, free, n_free, page, max_rows)
+    assert want[6]
+    L, F, N, rows = _run_extend(lengths, new, tg, free, n_free, page, max_rows)
+    assert L.tolist() == want[0] and tg.tolist() == want[1] and N.tolist() == [want[2]]
+    assert rows.cu_rows.tolist() == want[3] and rows.slot_map.tolist() == want[4]
+    assert rows.positions.tolist() == want[5]
+    with pytest.raises(_lib.DsmError, match="ran out"):
+        _lib.raise_device_error()
+
+
+def test_trim_refuses_more_pages_than_the_pool_holds():
+    lengths, new, table, free, n_free, tg = _tables_case(2, 5, 64, 300, 1, 10)
+    lengths = [64 * 3] * 5
+    L, F, N = i32(lengths), i32(free), i32([len(free) - 2])
+    pc.paged_trim(L, i32([0] * 5), tg, F, N, 64)
+    assert L.tolist() == lengths and F.tolist() == free and N.tolist() == [len(free) - 2]
+    with pytest.raises(_lib.DsmError):
+        _lib.raise_device_error()
+
+
+def test_empty_batch_and_no_rows():
+    rows = pc.paged_extend(i32([]), i32([]), torch.empty(0, 4, dtype=torch.int32, device=DEV), i32([0, 1]), i32([2]), 64, 5)
+    assert rows.cu_rows.tolist() == [0] and rows.slot_map.tolist() == [-1] * 5
+    L, N = i32([3, 0]), i32([2])
+    rows = pc.paged_extend(L, i32([0, 0]), i32([[0], [0]]), i32([0, 1]), N, 64, 0)
+    assert L.tolist() == [3, 0] and rows.cu_rows.tolist() == [0, 0, 0] and rows.slot_map.numel() == 0
+    assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------- append
+def _pool(seed, n_pages, n_kv, page, hd, e_lo=-9, e_hi=3):
+    """A pool by token: code values (no NaN), scales; and its stored form on the GPU."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for _ in range(2):
+        codes = po.round_e4m3((torch.randn(n_pages, n_kv, page, hd, generator=g) * 100).clamp(-448, 448).double())
+        scale = torch.exp2(torch.randint(e_lo, e_hi, (n_pages, n_kv), generator=g).double())
+        out.append((codes, scale))
+    (k, ks), (v, vs) = out
+    layer = pc.KV8Layer(_codes(po.store_keys(k)), _codes(po.store_values(v)), ks.float().to(DEV), vs.float().to(DEV))
+    return k, ks, v, vs, layer
+
+
+def _codes(values):
+    """fp64 e4m3 values -> uint8 codes on the GPU."""
+    return values.float().to(torch.float8_e4m3fn).view(torch.uint8).contiguous().to(DEV)
+
+
+def _loaded(layer):
+    f = lambda t: t.view(torch.float8_e4m3fn).float().double().cpu()  # noqa: E731
+    return po.load_keys(f(layer.k_codes)), po.load_values(f(layer.v_codes)), layer.k_scale.double().cpu(), \
+        layer.v_scale.double().cpu()
+
+
+def _same(a, b):
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def _check_append(layer, pool, k, v, slots):
+    kc, ks, vc, vs = pool
+    pc.kv8_append(layer, k.to(DEV) if not k.is_cuda else k, v.to(DEV) if not v.is_cuda else v,
+                  torch.tensor(slots, dtype=torch.int64, device=DEV))
+    wk, wks = po.kv8_append(kc, ks, k.double().cpu(), slots)
+    wv, wvs = po.kv8_append(vc, vs, v.double().cpu(), slots)
+    gk, gv, gks, gvs = _loaded(layer)
+    assert torch.equal(gks, wks) and torch.equal(gvs, wvs)
+    assert _same(gk, wk) and _same(gv, wv)
+    return wk, wks, wv, wvs
+
+
+def _runs(r, n_pages, page, n_runs, most, skip=0.1):
+    """Slots of neighbouring rows page by page, as several sequences leave them, some rows without."""
+    slots = []
+    for pg in r.sample(range(n_pages), n_runs):
+        first = r.choice([0, 0, r.randrange(page)])
+        n = r.randint(1, min(most, page - first))
+        slots += [pg * page + first + j for j in range(n)]
+        if r.random() < skip:
+            slots.append(-1)
+    return slots
+
+
+@pytest.mark.parametrize("dtype,hd,page,n_kv,n_runs,most", [
+    (torch.bfloat16, 128, 64, 2, 1, 1), (torch.bfloat16, 128, 64, 8, 7, 64), (torch.bfloat16, 64, 128, 3, 6, 100),
+    (torch.bfloat16, 256, 64, 1, 5, 9), (torch.float32, 128, 256, 2, 4, 256), (torch.float32, 64, 64, 1, 6, 3),
+    (torch.float32, 256, 128, 2, 3, 128), (torch.bfloat16, 128, 1024, 1, 2, 700), (torch.bfloat16, 128, 64, 2, 40, 64),
+])
+def test_append_matches_the_oracle(dtype, hd, page, n_kv, n_runs, most):
+    r = random.Random(hd + page + n_runs)
+    n_pages = n_runs + 3
+    k, ks, v, vs, layer = _pool(hd, n_pages, n_kv, page, hd)
+    slots = _runs(r, n_pages, page, n_runs, most) + [-1, -1]
+    g = torch.Generator().manual_seed(page)
+    # rows from far below the pages' scales to far above them: kept, grown and fresh scales
+    mag = torch.exp2(torch.randint(-14, 14, (len(slots), n_kv, 1), generator=g).float())
+    rk = (torch.randn(len(slots), n_kv, hd, generator=g) * mag).to(dtype)
+    rv = (torch.randn(len(slots), n_kv, hd, generator=g) * mag.flip(0)).to(dtype)
+    pool = _check_append(layer, (k, ks, v, vs), rk, rv, slots)
+    # the same rows again: nothing moves but pages that start afresh with the same rows
+    _check_append(layer, (pool[0], pool[1], pool[2], pool[3]), rk, rv, slots)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("order", ["head first", "interleaved", "offset", "broadcast rows"])
+def test_append_takes_any_row_and_head_strides(order):
+    n, n_kv, hd, page = 70, 2, 128, 64
+    k, ks, v, vs, layer = _pool(4, 4, n_kv, page, hd)
+    slots = list(range(30, 64)) + list(range(128, 164))
+    g = torch.Generator().manual_seed(0)
+    base = torch.randn(2, 400, 400, generator=g).bfloat16().to(DEV)
+    if order == "head first":
+        rk, rv = (torch.randn(n_kv, n, hd, generator=g).bfloat16().to(DEV).transpose(0, 1) for _ in range(2))
+    elif order == "interleaved":  # q | k | v columns of one projection
+        rows = torch.randn(n, 3 * n_kv * hd, generator=g).bfloat16().to(DEV)
+        rk, rv = (rows[:, c * n_kv * hd:(c + 1) * n_kv * hd].unflatten(1, (n_kv, hd)) for c in (1, 2))
+    elif order == "offset":  # rows that start on two bytes
+        rk, rv = (base[c, :, 1:].as_strided((n, n_kv, hd), (400, 129, 1), base[c].storage_offset() + 1) for c in (0, 1))
+    else:
+        rk, rv = (base[c, 0, :hd].expand(n, n_kv, hd) for c in (0, 1))
+    _check_append(layer, (k, ks, v, vs), rk, rv, slots)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_borders_and_what_is_not_finite(dtype):
+    """Maxima at 448 * 2^e and a step to either side, all-zero rows, the type's largest and smallest values,
+    values halfway between codes, infinities and NaN."""
+    hd, page, n_kv = 64, 64, 1
+    tops = [448.0, 449.0, 450.0, 447.0, 3.5, 3.515625, 7 * 2.0 ** 100, 0.0, 1e-38, 2.0 ** -126, 2.0 ** -133,
+            torch.finfo(dtype).max, float("inf"), float("nan"), 1.0]
+    k, ks, v, vs, layer = _pool(9, len(tops), n_kv, page, hd)
+    vals = po.e4m3_values()[:127]
+    ties = (vals[:-1] + vals[1:]) / 2
+    rows, slots = [], []
+    for i, top in enumerate(tops):
+        x = torch.zeros(2, n_kv, hd, dtype=torch.float64)
+        x[0, 0, 0] = top
+        x[1, 0, 1:] = ties[2 * torch.arange(63)] * (1.0 if 440 <= top <= 450 or not abs(top) < 1e39 else 0.0)
+        x[1, 0, 3] = -top
+        rows.append(x)
+        slots += [i * page + (0 if i % 2 else 5), i * page + 6]
+    rows = torch.cat(rows).to(dtype)
+    _check_append(layer, (k, ks, v, vs), rows, rows.flip(2), slots)
+    assert _lib.device_error() == 0
+
+
+def test_append_skips_slots_outside_the_pool_and_says_so():
+    n_kv, hd, page = 2, 128, 64
+    k, ks, v, vs, layer = _pool(1, 2, n_kv, page, hd)
+    rk = torch.randn(5, n_kv, hd).bfloat16()
+    slots = [3, 2 * page, 2 ** 40, -5, page + 1]
+    _check_append(layer, (k, ks, v, vs), rk, rk * 2, slots)
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
+
+
+def test_append_slots_past_32_bits():
+    """A pool whose codes pass 2^32 bytes: the last page is written, the rest stays."""
+    n_pages, n_kv, page, hd = 2200, 8, 1024, 256
+    try:
+        codes = torch.zeros(2, n_pages, n_kv, page, hd, dtype=torch.uint8, device=DEV)
+    except torch.OutOfMemoryError:
+        pytest.skip("no room for the pool")
+    layer = pc.KV8Layer(codes[0], codes[1].view(n_pages, n_kv, page // 64, hd, 64),
+                        torch.ones(n_pages, n_kv, device=DEV), torch.ones(n_pages, n_kv, device=DEV))
+    rk = torch.randn(3, n_kv, hd, generator=torch.Generator().manual_seed(2)).bfloat16()
+    slots = [(n_pages - 1) * page + j for j in range(3)]
+    pc.kv8_append(layer, rk.to(DEV), rk.to(DEV), torch.tensor(slots, device=DEV))
+    last = pc.KV8Layer(*(t[-1:] for t in layer))
+    zero = torch.zeros(1, n_kv, page, hd, dtype=torch.float64)
+    wk, wks = po.kv8_append(zero, torch.ones(1, n_kv, dtype=torch.float64), rk.double(), [0, 1, 2])
+    gk, gv, gks, _ = _loaded(last)
+    assert _same(gk, wk) and _same(gv, wk) and torch.equal(gks, wks)
+    assert int(codes[:, :-1].max()) == 0
+
+
+# ------------------------------------------------------------------------------- attention
+def _attn_case(seed, lengths, s, n_kv, group, hd, page, dtype, with_block=True, q_mag=1.0, poison=True, cols=0, extra=2,
+               e_lo=-9, e_hi=-4):
+    """A pool of shuffled pages; whatever no sequence may read is NaN: codes behind the lengths, unused
+    pages and their scales."""
+    r = random.Random(seed)
+    need = [-(-n // page) for n in lengths]
+    n_pages = sum(need) + extra
+    k, ks, v, vs, layer = _pool(seed, n_pages, n_kv, page, hd, e_lo, e_hi)
+    pool = list(range(n_pages))
+    r.shuffle(pool)
+    most = max(1, max(need)) + 1
+    table = [[-1] * most for _ in need]
+    kept = torch.zeros(n_pages, page, dtype=torch.bool)
+    for i, n in enumerate(lengths):
+        for j in range(need[i]):
+            table[i][j] = pool.pop()
+            kept[table[i][j], :min(page, n - j * page)] = True
+    if poison:
+        nan = torch.full((), float("nan"), dtype=torch.float64)
+        m = kept[:, None, :, None]
+        k, v = torch.where(m, k, nan), torch.where(m, v, nan)
+        ks[pool], vs[pool] = float("nan"), float("nan")
+        layer = pc.KV8Layer(_codes(po.store_keys(k)), _codes(po.store_values(v)), ks.float().to(DEV),
+                            vs.float().to(DEV))
+    g = torch.Generator().manual_seed(seed + 1)
+    b = len(lengths)
+    q = (torch.randn(b, s, n_kv * group, hd, generator=g) * q_mag).to(dtype)
+    blk = [torch.randn(b, n_kv, s, hd, generator=g).to(dtype) if with_block else None for _ in range(2)]
+    wide = torch.full((b, most + cols), -1, dtype=torch.int32)
+    wide[:, :most] = torch.tensor(table)
+    return dict(q=q, layer=layer, table=table, tg=wide.to(DEV)[:, :most], lengths=lengths, blk=blk,
+                k=k * ks[..., None, None], v=v * vs[..., None, None], hd=hd)
+
+
+def _bound(dtype, ref, score, vmax, hd, n):
+    s, v = score[:, None, None], vmax[:, None, None]
+    if dtype == torch.bfloat16:
+        ds = (2.0 ** -17 * hd + 2.0 ** -18) * s
+        return 2.0 ** -8 * ref.abs() + (2 * ds + 2.0 ** -8 + 2.0 ** -12) * v
+    ds = (2.0 ** -21 + (hd + 8) * 2.0 ** -24) * s
+    return 2.0 ** -24 * ref.abs() + (2 * ds + 2.0 ** -21 + (n / 32 + 64) * 2.0 ** -24) * v
+
+
+def _check_attn(c, scale=None, out=None, lengths=None):
+    scale = c["hd"] ** -0.5 if scale is None else scale
+    lengths = c["lengths"] if lengths is None else lengths
+    blk = [None if t is None else t.to(DEV) for t in c["blk"]]
+    if out is None:
+        out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(lengths), *blk, scale=scale)
+    ref, score, vmax = po.kv8_attention(c["q"], c["k"], c["v"], c["table"], lengths, *c["blk"], scale)
+    got = out.double().cpu()
+    assert got.shape == ref.shape and out.dtype == c["q"].dtype
+    assert torch.isfinite(got).all()
+    err = (got - ref).abs()
+    tol = _bound(c["q"].dtype, ref, score, vmax, c["hd"], max(lengths) + c["q"].shape[1])
+    assert bool((err <= tol).all()), float((err / tol.clamp_min(1e-30)).max())
+    return out
+
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("dtype,lengths,s,n_kv,group,hd,page,with_block", [
+    (BF, [1], 1, 1, 1, 128, 64, False), (BF, [150], 1, 8, 4, 128, 64, True), (BF, [0], 7, 2, 4, 128, 64, True),
+    (BF, [0, 5, 0], 1, 2, 4, 128, 64, False), (BF, [64, 63, 65, 128, 1, 0], 7, 2, 4, 128, 64, True),
+    (BF, [700, 3, 1999, 0, 320], 7, 2, 4, 128, 64, True), (BF, [1000, 77], 7, 2, 8, 64, 64, True),
+    (BF, [513, 300], 5, 1, 3, 256, 128, True), (BF, [256, 255, 257], 2, 2, 1, 64, 256, True),
+    (BF, [2050], 16, 1, 8, 128, 128, True), (BF, [300, 90], 33, 1, 4, 128, 64, True),
+    (BF, [600, 1], 70, 1, 2, 64, 64, True), (BF, [3000], 1, 2, 16, 128, 1024, False), (BF, [129] * 40, 3, 4, 2, 128, 64, True),
+    (F32, [150, 0, 1], 1, 2, 4, 128, 64, True), (F32, [64, 63, 700], 5, 2, 4, 128, 64, True),
+    (F32, [333, 2], 7, 1, 8, 64, 128, False), (F32, [500, 40], 5, 1, 4, 256, 64, True),
+    (F32, [1300], 33, 1, 3, 128, 256, True),
+])
+def test_attention_matches_the_oracle(dtype, lengths, s, n_kv, group, hd, page, with_block):
+    c = _attn_case(sum(lengths) + s, lengths, s, n_kv, group, hd, page, dtype, with_block)
+    out = _check_attn(c)
+    if not with_block:
+        for i, n in enumerate(lengths):
+            assert n > 0 or int(out[i].count_nonzero()) == 0  # nothing to attend to: zeros
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,q_mag,e_lo,e_hi,scale", [
+    (BF, 30.0, -9, -4, None),   # peaked: a few keys carry everything
+    (BF, 1.0, -30, 20, 2.0 ** -26),  # page scales fifty octaves apart
+    (BF, 2.0 ** -100, -9, -4, 2.0 ** 95), (BF, 2.0 ** 100, -9, -4, 2.0 ** -105),
+    (F32, 30.0, -9, -4, None), (F32, 1.0, -30, 20, 2.0 ** -26), (F32, 2.0 ** -100, -9, -4, 2.0 ** 95),
+    (BF, 1.0, -9, -4, 0.0), (BF, 1.0, -9, -4, -0.7),
+])
+def test_attention_magnitudes(dtype, q_mag, e_lo, e_hi, scale):
+    c = _attn_case(3, [500, 64, 1], 5, 2, 4, 128, 64, dtype, with_block=e_hi < 0 and q_mag < 2.0 ** 90, q_mag=q_mag,
+                   e_lo=e_lo, e_hi=e_hi)
+    _check_attn(c, scale)
+
+
+def test_attention_rows_of_very_different_size():
+    """Query rows 2^60 apart in one call: each row has its own scale."""
+    c = _attn_case(5, [200, 90], 7, 2, 4, 128, 64, BF)
+    c["q"] = (c["q"].float() * torch.exp2(-torch.arange(7.0) * 10)[None, :, None, None]).bfloat16()
+    _check_attn(c)
+    c["q"][:, 3] = 0
+    _check_attn(c)
+
+
+def test_attention_sink_over_a_long_tail():
+    """One key 2^15 times heavier than each of 16384 others: the tail carries a third of the weight."""
+    hd, n = 64, 16384
+    c = _attn_case(8, [n], 1, 1, 2, hd, 64, BF, with_block=False, e_lo=-6, e_hi=-5)
+    kd = torch.zeros(hd, dtype=torch.float64)
+    kd[0] = 1.0
+    k = torch.zeros_like(c["k"])
+    sink = c["table"][0][0]
+    k[sink, 0, 0] = kd
+    c["k"] = k
+    codes = po.round_e4m3(k * 2.0 ** 6)
+    c["layer"].k_codes.copy_(_codes(po.store_keys(codes)))
+    c["layer"].k_scale.fill_(2.0 ** -6)
+    c["q"] = torch.zeros_like(c["q"])
+    c["q"][..., 0] = 10.375  # e^10.375 ~ 2^15
+    _check_attn(c, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_takes_strided_inputs(dtype):
+    c = _attn_case(12, [300, 65, 1], 5, 2, 4, 128, 64, dtype, cols=3)
+    b, s, nh, hd = c["q"].shape
+    ref = _check_attn(c)
+    rows = torch.zeros(b * s, nh * hd + 2 * 2 * hd + 1, dtype=dtype, device=DEV)  # q | k | v columns, odd row length
+    rows[:, :nh * hd] = c["q"].reshape(b * s, -1).to(DEV)
+    for j in (0, 1):
+        rows[:, nh * hd + j * 2 * hd:][:, :2 * hd] = c["blk"][j].transpose(1, 2).reshape(b * s, -1).to(DEV)
+    q = rows[:, :nh * hd].view(b, s, nh, hd)
+    bk, bv = (rows[:, nh * hd + j * 2 * hd:][:, :2 * hd].view(b, s, 2, hd).transpose(1, 2) for j in (0, 1))
+    out = pc.gqa_attention_kv8(q, c["layer"], c["tg"], i32(c["lengths"]), bk, bv)
+    assert torch.equal(out, ref)
+    one = c["q"][:1].to(DEV).expand(b, s, nh, hd)  # the same rows for every sequence
+    want = pc.gqa_attention_kv8(one.contiguous(), c["layer"], c["tg"], i32(c["lengths"]), bk, bv)
+    assert torch.equal(pc.gqa_attention_kv8(one, c["layer"], c["tg"], i32(c["lengths"]), bk, bv), want)
+
+
+def test_attention_is_the_same_twice_and_on_another_stream():
+    c = _attn_case(1, [1500, 3, 700, 0, 64], 7, 2, 4, 128, 64, BF)
+    a = _check_attn(c)
+    blk = [t.to(DEV) for t in c["blk"]]
+    q, n = c["q"].to(DEV), i32(c["lengths"])
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(4):
+        for s in (s1, s2):
+            with torch.cuda.stream(s):
+                outs.append(pc.gqa_attention_kv8(q, c["layer"], c["tg"], n, *blk))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, a) for o in outs)
+
+
+def test_attention_bad_tables_are_skipped_and_reported():
+    """Pages outside the pool count as absent; a length past the table is cut to it."""
+    c = _attn_case(7, [200, 130], 3, 1, 2, 128, 64, BF)
+    c["table"][0][1] = 10 ** 6
+    c["table"][1][0] = -2
+    c["tg"] = i32(c["table"])
+    _check_attn(c)
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
+    c = _attn_case(7, [200, 130], 3, 1, 2, 128, 64, BF)
+    most = len(c["table"][0])
+    for row in c["table"]:
+        row[:] = [p if p >= 0 else row[0] for p in row]
+    c["tg"] = i32(c["table"])
+    c["k"], c["v"] = torch.nan_to_num(c["k"]), torch.nan_to_num(c["v"])
+    for t in (c["layer"].k_codes, c["layer"].v_codes):
+        t[(t & 127) == 127] = 0
+    _check_attn(c, lengths=[most * 64 + 1000, 130])
+    assert _lib.device_error() == 0x15
+    _check_attn(c, lengths=[-3, 130])
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_passes_nan_of_its_own_rows_on(dtype):
+    """A NaN among the rows that a sequence does read reaches its outputs, and no other sequence's."""
+    c = _attn_case(2, [200, 90], 2, 1, 2, 128, 64, dtype)
+    c["layer"].v_codes[c["table"][0][1], 0, 0, 5, 7] = 0x7F
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]),
+                               *(t.to(DEV) for t in c["blk"])).view(2, 2, 2, 128)
+    assert bool(out[0, :, :, 5].isnan().all()) and bool(torch.isfinite(out[1]).all())
+    assert bool(torch.isfinite(out[0, :, :, :5]).all()) and bool(torch.isfinite(out[0, :, :, 6:]).all())
+    q = c["q"].clone()
+    q[1, 1, 0, 3] = float("inf")
+    out = pc.gqa_attention_kv8(q.to(DEV), c["layer"], c["tg"], i32(c["lengths"]),
+                               *(t.to(DEV) for t in c["blk"])).view(2, 2, 2, 128)
+    assert bool(out[1, 1, 0].isnan().all()) and bool(torch.isfinite(out[1, 0]).all())
+    assert bool(torch.isfinite(out[1, 1, 1]).all())
+
+
+def test_attention_offsets_past_32_bits():
+    """Pages behind 2^32 bytes of codes."""
+    n_pages, n_kv, page, hd = 2200, 8, 1024, 256
+    try:
+        codes = torch.zeros(2, n_pages, n_kv, page, hd, dtype=torch.uint8, device=DEV)
+    except torch.OutOfMemoryError:
+        pytest.skip("no room for the pool")
+    k, ks, v, vs, small = _pool(3, 2, n_kv, page, hd, -9, -4)
+    layer = pc.KV8Layer(codes[0], codes[1].view(n_pages, n_kv, page // 64, hd, 64),
+                        torch.full((n_pages, n_kv), float("nan"), device=DEV),
+                        torch.full((n_pages, n_kv), float("nan"), device=DEV))
+    for t, u in zip(layer, small):
+        t[-2:] = u
+    c = dict(q=torch.randn(1, 2, n_kv * 2, hd, generator=torch.Generator().manual_seed(0)).bfloat16(), layer=small,
+             table=[[1, 0]], tg=i32([[1, 0]]), lengths=[1500], blk=[None, None], k=k * ks[..., None, None],
+             v=v * vs[..., None, None], hd=hd)
+    want = _check_attn(c)
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), layer, i32([[n_pages - 1, n_pages - 2]]), i32([1500]))
+    assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------- together
+def test_a_run_of_steps_matches_the_oracle():
+    """Five steps of a batch on one cache: extend, append, attend, trim, with a sequence that is released and its
+    place taken by another, against a cache kept by the oracle."""
+    r = random.Random(0)
+    b, n_kv, group, hd, page, n_pages, most = 5, 2, 4, 128, 64, 24, 6
+    cache = pc.PagedKVCache(2, n_pages, n_kv, hd, b, most, page_size=page)
+    cache.k_codes.fill_(0xFF)
+    cache.v_codes.fill_(0xFF)
+    lengths, table = [0] * b, [[-1] * most for _ in range(b)]
+    free, n_free = list(range(n_pages - 1, -1, -1)), n_pages
+    state = {}
+    for kind in ("k", "v"):
+        state[kind] = (torch.full((n_pages, n_kv, page, hd), float("nan"), dtype=torch.float64),
+                       torch.full((n_pages, n_kv), 2.0 ** -120, dtype=torch.float64))
+    g = torch.Generator().manual_seed(1)
+    for step in range(5):
+        new = [r.choice([0, 1, 7, 70]) if step else r.randint(1, 130) for _ in range(b)]
+        max_rows = sum(new) + 2
+        rows = cache.extend(i32(new), max_rows)
+        lengths, table, n_free, cu, slots, pos, failed = po.paged_extend(lengths, new, table, free, n_free, page, max_rows)
+        assert not failed and rows.slot_map.tolist() == slots and cache.lengths.tolist() == lengths
+        x = [torch.randn(max_rows, n_kv, hd, generator=g).bfloat16() * 2.0 ** step for _ in range(2)]
+        cache.append(1, x[0].to(DEV), x[1].to(DEV), rows)
+        for kind, t in zip(("k", "v"), x):
+            state[kind] = po.kv8_append(*state[kind], t.double(), slots)
+        k, v = (state[n][0] * state[n][1][..., None, None] for n in ("k", "v"))
+        q = torch.randn(b, 3, n_kv * group, hd, generator=g).bfloat16() * 2.0 ** -step
+        blk = [torch.randn(b, n_kv, 3, hd, generator=g).bfloat16() for _ in range(2)]
+        out = cache.attend(1, q.to(DEV), *(t.to(DEV) for t in blk))
+        _check_attn(dict(q=q, k=k, v=v, table=table, lengths=lengths, blk=blk, hd=hd), out=out)
+        keep = [max(0, n - r.choice([0, 0, 3, 66])) for n in lengths]
+        if step == 2:
+            keep[1] = 0
+        cache.trim(i32(keep))
+        lengths, free, n_free, failed = po.paged_trim(lengths, keep, table, free, n_free, page)
+        assert not failed and cache.lengths.tolist() == lengths and cache.n_free.tolist() == [n_free]
+    assert _lib.device_error() == 0
+
+
+def test_a_captured_step_replays_as_the_lengths_change():
+    """extend, append, attend captured once; every replay grows the same cache, as eager calls grow another.
+    Two graphs replay on one cache in turn."""
+    b, n_kv, group, hd, page = 3, 2, 4, 128, 64
+    caches = [pc.PagedKVCache(1, 30, n_kv, hd, b, 8, page_size=page) for _ in range(2)]
+    g = torch.Generator(device=DEV).manual_seed(0)
+    mk = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    new, x, q, blk = i32([0] * b), [mk(60, n_kv, hd) for _ in range(2)], mk(b, 4, n_kv * group, hd), \
+        [mk(b, n_kv, 4, hd) for _ in range(2)]
+
+    def step(cache):
+        rows = cache.extend(new, 60)
+        cache.append(0, *x, rows)
+        return cache.attend(0, q, *blk)
+
+    step(caches[0])  # kernels loaded; nothing is added
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(caches[0])
+        graphs.append((gr, out))
+    r = random.Random(3)
+    for i in range(10):
+        new.copy_(i32([r.randint(0, 20) for _ in range(b)]))
+        for t in (*x, q, *blk):
+            t.copy_(torch.randn(t.shape, generator=g, device=DEV))
+        gr, out = graphs[i % 2]
+        gr.replay()
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        assert torch.equal(caches[0].lengths, caches[1].lengths) and torch.equal(caches[0].n_free, caches[1].n_free)
+        assert torch.equal(caches[0].block_table, caches[1].block_table)
+    assert int(caches[0].lengths.sum()) > 0 and _lib.device_error() == 0
+    del graphs, gr
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_qwen3_layer_over_the_paged_cache(dtype):
+    """``append_paged`` + ``forward_paged`` of a Qwen3 draft layer for sequences of different lengths against the
+    oracle's layer, one sequence at a time over the rows that the cache gives back: the 8-bit rounding of the context
+    is in both. Tolerances are those of the dense layer's tests (bf16 2e-2, fp32 5e-3 of the largest value)."""
+    from dsm.qwen3_attention import rope_tables
+    from dsm.qwen3_layer import Qwen3DSparkLayer
+    from helpers import max_rel_err
+
+    b, s, h, nh, nkv, hd, inter, page, theta, eps = 3, 5, 256, 8, 2, 128, 256, 64, 1e6, 1e-6
+    args = dict(hidden_size=h, num_attention_heads=nh, num_key_value_heads=nkv, head_dim=hd, rms_norm_eps=eps,
+                intermediate_size=inter)
+    g = torch.Generator().manual_seed(0)
+    rnd = lambda *sh, std=1.0: (torch.randn(*sh, generator=g) * std).to(dtype)  # noqa: E731
+    w = {"q_proj": rnd(nh * hd, h, std=h ** -0.5), "k_proj": rnd(nkv * hd, h, std=h ** -0.5),
+         "v_proj": rnd(nkv * hd, h, std=h ** -0.5), "o_proj": rnd(h, nh * hd, std=(nh * hd) ** -0.5),
+         "gate_proj": rnd(inter, h, std=h ** -0.5), "up_proj": rnd(inter, h, std=h ** -0.5),
+         "down_proj": rnd(h, inter, std=inter ** -0.5)}
+    layer = Qwen3DSparkLayer(args).to(DEV)
+    for n in ("q_proj", "k_proj", "v_proj", "o_proj"):
+        getattr(layer.self_attn, n).weight = torch.nn.Parameter(w[n].to(DEV), requires_grad=False)
+    for n in ("gate_proj", "up_proj", "down_proj"):
+        getattr(layer.mlp, n).weight = torch.nn.Parameter(w[n].to(DEV), requires_grad=False)
+    cache = pc.PagedKVCache(1, 20, nkv, hd, b, 5, page_size=page)
+    cos_t, sin_t = rope_tables(torch.arange(400), hd, theta)
+    cos_t, sin_t = cos_t.to(DEV), sin_t.to(DEV)
+    total = [0] * b
+    for new in ([130, 0, 64], [3, 1, 0], [0, 0, 70]):
+        max_rows = sum(new) + 1
+        rows = cache.extend(i32(new), max_rows)
+        pos = rows.positions.long()
+        layer.append_paged(rnd(max_rows, h).to(DEV), cos_t[pos], sin_t[pos], cache, 0, rows)
+        total = [a + c for a, c in zip(total, new)]
+    assert cache.lengths.tolist() == total
+    hidden = rnd(b, s, h)
+    at = torch.tensor([[n + j for j in range(s)] for n in total])
+    out = layer.forward_paged(hidden.to(DEV), cache, 0, cos_t[at.flatten().to(DEV)], sin_t[at.flatten().to(DEV)])
+    p = {"self_attn": {n: w[n] for n in ("q_proj", "k_proj", "v_proj", "o_proj")}}
+    p["self_attn"].update(q_norm=torch.ones(hd), k_norm=torch.ones(hd))
+    params = dict(w, q_norm=torch.ones(hd), k_norm=torch.ones(hd), input_layernorm=torch.ones(h),
+                  post_attention_layernorm=torch.ones(h))
+    gk, gv, gks, gvs = _loaded(cache.layer(0))
+    kd, vd = gk * gks[..., None, None], gv * gvs[..., None, None]
+    table = cache.block_table.tolist()
+    for i, n in enumerate(total):
+        ck, cv = (torch.cat([x[table[i][j]] for j in range(-(-n // page))], 1)[None, :, :n].to(dtype) if n else None
+                  for x in (kd, vd))
+        ref = oracle.qwen3_layer_cached(params, nh, nkv, hd, eps, hidden[i:i + 1], ck, cv, cos_t[at[i].to(DEV)].cpu(),
+                                        sin_t[at[i].to(DEV)].cpu())
+        assert max_rel_err(out[i:i + 1], ref) < (2e-2 if dtype == BF else 5e-3), i
+    assert _lib.device_error() == 0
+
+
+def test_modules_refuse_caches_that_do_not_fit():
+    from dsm.qwen3_attention import Qwen3DSparkAttention
+
+    a = Qwen3DSparkAttention(dict(hidden_size=64, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                                  rms_norm_eps=1e-6)).to(DEV)
+    cache = pc.PagedKVCache(1, 4, 2, 64, 2, 2)
+    cos = torch.zeros(6, 64)
+    x = torch.zeros(2, 3, 64, device=DEV)
+    rows = cache.extend(i32([1, 1]), 4)
+    for bad in (lambda: a.attend_paged(x, pc.PagedKVCache(1, 4, 1, 64, 2, 2), 0, cos, cos),
+                lambda: a.attend_paged(x, pc.PagedKVCache(1, 4, 2, 128, 2, 2), 0, cos, cos),
+                lambda: a.attend_paged(x[:1], cache, 0, cos[:3], cos[:3]),
+                lambda: a.attend_paged(x, cache, 0, cos[:3], cos[:3]),
+                lambda: a.attend_paged(x.cpu(), cache, 0, cos, cos),
+                lambda: a.append_paged(x[0], cos[:3], cos[:3], cache, 0, rows),
+                lambda: a.append_paged(x, cos, cos, cache, 0, rows),
+                lambda: cache.append(0, x[0].view(3, 1, 64), x[0].view(3, 1, 64), rows),
+                lambda: cache.append(0, torch.zeros(4, 2, 64, device=DEV).half(),
+                                     torch.zeros(4, 2, 64, device=DEV).half(), rows),
+                lambda: cache.append(0, torch.zeros(4, 64, 2, device=DEV).transpose(1, 2),
+                                     torch.zeros(4, 2, 64, device=DEV), rows),
+                lambda: cache.attend(0, torch.zeros(2, 1, 3, 64, device=DEV)),
+                lambda: cache.attend(0, torch.zeros(2, 1, 4, 64, device=DEV), torch.zeros(2, 2, 1, 64, device=DEV)),
+                lambda: cache.attend(0, torch.zeros(2, 1, 4, 64, device=DEV, dtype=torch.float16)),
+                lambda: cache.extend(i32([1]), 4), lambda: cache.extend(i32([1, 1]).long(), 4),
+                lambda: cache.extend(i32([1, 1]), -1), lambda: cache.trim(i32([1, 1])[::2])):
+        with pytest.raises(ValueError):
+            bad()
