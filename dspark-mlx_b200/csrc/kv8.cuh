@@ -60,4 +60,19 @@ __device__ __forceinline__ int kv8_scale_exp(float amax) {
   return amax > 0.f ? min(max(e, kKv8MinExp), kKv8MaxExp) : kKv8MinExp;
 }
 
+__device__ __forceinline__ float kv8_warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float kv8_warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+inline bool kv8_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool kv8_head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
+inline bool kv8_page_ok(int page) { return page > 0 && page % kKv8Group == 0 && page <= kKv8MaxPage; }
+
 }  // namespace dsm
