@@ -2,9 +2,9 @@
 // sequence's rows in the paged 8-bit cache (layout in kv8.cuh) and then the block's own rows, with no
 // mask: the paged form of Qwen3DSparkAttention.attend_cached (dspark_mlx/arch/qwen3.py:130-143).
 //
-//   kv8_attn_mma_kernel   bf16: e4m3 tensor-core products straight on the stored codes, split over
-//                         the keys; kv8_attn_combine_kernel joins what was split.
-//   kv8_attn_core_kernel  fp32 products on the CUDA cores, any type.
+//   kv8_attn_mma_kernel   tensor-core products, split over the keys; kv8_attn_combine_kernel joins what
+//                         was cut.
+//   kv8_attn_core_kernel  fp32 products on the CUDA cores.
 // dsm_set_attn_kernel picks between them (per host thread).
 #include <algorithm>
 
@@ -158,34 +158,39 @@ int launch_core(const AttnArgs& a, cudaStream_t s) {
 // ------------------------------------------------------------------------------------------
 // the tensor-core kernel
 // ------------------------------------------------------------------------------------------
-// Mathematics. The codes enter mma.m16n8k32 as they are stored. q, scaled per row by a power of two to
-// at most 448, is split into two e4m3 terms (hi = e4m3(x), lo = e4m3(x - hi)): exact for bf16's 8
-// significant bits wherever the residual reaches e4m3's normals, 2^-10 of a unit off elsewhere (row
-// maximum 224 to 448). Both terms add into one fp32 accumulator. The weights of a 64-key tile,
-// p = 2^(s - m_tile), are taken relative to the tile's own row maximum, so that a heavy key elsewhere
-// does not push them out of e4m3's range, scaled to at most 2^8 and split the same way (2^-8 of each
-// is lost, 2^-18 of the largest). The tile's product is then joined in fp32 with the running
-// (m, l, o) of the row: o = o * 2^(m - m') + (2^(m_tile - m') * v_scale) * (p v).
+// Mathematics. e4m3 codes are exact in f16, so keys and values enter mma.m16n8k16 as the codes'
+// values and the page's power-of-two scales stay outside. q, scaled per row by a power of two to at
+// most 448, is one f16 term for bf16 rows (their 8 bits fit f16's 11) and two for fp32 rows (hi + lo,
+// 2^-22). A row's weights are p = 2^(s - m) with a reference m that follows its running maximum only
+// when that has grown by more than 2^8, so that the sums are rescaled rarely; they enter f16
+// (in one or two terms as well) as p * 2^6 * 2^(ev - rv), ev the exponent of the page's value scale and
+// rv a reference that it moves when it leaves [rv - 10, rv]: the sums need no factor per page. Sums,
+// weights and maxima are fp32. The tensor cores' own additions cut off what they round: too coarse for
+// fp32 calls over long sums, whose products go into the fp32 sums a few steps at a time, by CUDA cores.
 //
 // What bounds it: reading 2 * head_dim bytes per key and KV head. At the copy peak an SM gets 64
-// keys of head_dim 128 per ~700 cycles; the e4m3 products take ~300 of them for 32 query rows (one
-// m16n8k32 per ~1.15 cycles; f16 products on converted codes would take ~560 and two conversions per
-// code pair), so codes are neither converted nor padded to 16 bits.
+// keys of head_dim 128 per ~700 cycles. mma.sync's e4m3 form runs as f16 products on this GPU, with the
+// conversions and fp32 additions around every one of them (measured: twice the tensor instructions for
+// q in two e4m3 terms, 4,000 instructions per tile and 32 rows, 3,400 cycles); converting each code once
+// per warp and keeping q and the weights in single f16 terms takes a quarter of that.
 //
 // Layout of the work. A unit is one sequence's KV head (and block of up to 128 query rows); its
-// tiles of 64 keys follow one another, and all units' tiles form one line that is cut into equal
-// ranges, one per CTA (one CTA per SM), whatever the lengths are. A cut near a unit's edge moves to
-// the edge. In a CTA, tile i of its range belongs to lane i % tl (tl = warps / mg lanes side by side,
-// of mg warps each; a warp holds all of the CTA's query rows, or 1 / mg of them where there are many).
-// Tiles come by one bulk copy of keys and one of values into stages that belong to the lane: it refills
-// the keys' half as soon as the scores are taken, the values' half after the sums, and waits for no
-// other lane in the main loop.
+// tiles of 64 keys follow one another, and all units' tiles form one line that is cut into ranges of
+// equal cost, one per CTA (one CTA per SM), whatever the lengths are; a unit costs kUnitCost tiles
+// beside its own. A cut near a unit's edge moves to the edge. In a CTA, tile i of its range belongs to
+// lane i % tl (tl = warps / mg lanes side by side, of mg warps each; a warp holds all of the CTA's query
+// rows, or 1 / mg of them where there are many). Tiles come by one bulk copy of keys and one of values
+// into stages that belong to the lane: it refills the keys' half as soon as the scores are taken, the
+// values' half after the sums, and waits for no other lane in the main loop. The block's own rows are
+// 16-key tiles of whichever CTA holds the unit's last tile, read straight from the caller's tensors.
 constexpr int kTile = kKv8Group;
 constexpr int kMaxDepth = 2;  // stages per lane, where they fit
+constexpr int kUnitCost = 6;  // a unit's q, join and output, in tiles
 // warps per CTA: a stage of head_dim 256 holds 32 KB, so four lanes fill shared memory
 constexpr int mma_warps(int hd) { return hd == 256 ? 4 : 8; }
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPScale = 8.f;  // weights enter e4m3 scaled by 2^8
+constexpr float kPScale = 6.f;  // weights at the reference enter f16 as 2^6,
+constexpr float kPGrow = 8.f;   // and grow to 2^14 before the reference follows
 constexpr float kLowest = -3.402823466e38f;
 
 struct MmaPlan {
@@ -194,9 +199,10 @@ struct MmaPlan {
   int rows;        // query rows of a KV head: group * block
   int depth;       // stages per lane
   int snap;        // a cut within this many tiles of a unit's edge moves there
-  int least;       // tiles a range should have at least
+  int least;       // cost that a range should have at least
+  bool vec_q, vec_blk;  // q's / the block's rows can be read 4 (8) values at a time
   float* part;     // [2 * grid][cta_rows][head_dim] partial sums
-  float* ml;       // [2 * grid][cta_rows][2] their maximum and weight
+  float4* ml;      // [2 * grid][cta_rows] their reference, weight and value exponent
 };
 
 // tiles before each sequence, for one KV head and row block (P [batch + 1]); a sequence without a
@@ -237,12 +243,12 @@ __device__ __forceinline__ void scan_tiles(const AttnArgs& p, int* P, int* warp_
 struct Place {
   int b, u, t, T;
 };
-__device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int x) {
-  const int q = x / hr;  // P[b] <= q < P[b + 1]
-  int lo = 0, hi = batch;
+// with `cost` > 0, x counts that many more tiles in front of each unit (t < 0 there)
+__device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int64_t x, int cost) {
+  int lo = 0, hi = batch;  // the last sequence that starts at or before x
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (P[mid] <= q)
+    if ((int64_t(P[mid]) + int64_t(mid) * cost) * hr <= x)
       lo = mid;
     else
       hi = mid;
@@ -250,24 +256,21 @@ __device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int x
   Place r;
   r.b = lo;
   r.T = P[lo + 1] - P[lo];
-  const int rem = x - P[lo] * hr;
-  r.u = rem / r.T;
-  r.t = rem - r.u * r.T;
+  const int64_t rem = x - (int64_t(P[lo]) + int64_t(lo) * cost) * hr;
+  r.u = int(rem / (r.T + cost));
+  r.t = int(rem - int64_t(r.u) * (r.T + cost)) - cost;
   return r;
 }
-// the start of CTA i's range; short lines go to fewer CTAs
+// the first tile of CTA i's range; short lines go to fewer CTAs
 __device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, int ctas, int snap, int least) {
-  const int total = P[batch] * hr;
-  ctas = min(ctas, (total + least - 1) / least);
+  const int64_t total = (int64_t(P[batch]) + int64_t(batch) * kUnitCost) * hr;
+  ctas = int(min(int64_t(ctas), (total + least - 1) / least));
   if (i <= 0) return 0;
-  if (i >= ctas) return total;
-  const int x = int(int64_t(total) * i / ctas);
-  if (x >= total) return total;
-  const Place a = place_of(P, batch, hr, x);
+  if (i >= ctas) return P[batch] * hr;
+  const Place a = place_of(P, batch, hr, total * i / ctas, kUnitCost);
   const int d = min(snap, a.T / 2);
-  if (a.t <= d) return x - a.t;
-  if (a.T - a.t <= d) return x + a.T - a.t;
-  return x;
+  const int t = a.t <= d ? 0 : a.T - a.t <= d ? a.T : a.t;
+  return P[a.b] * hr + a.u * a.T + t;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -275,48 +278,32 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// D += A (16 x 32 e4m3, row) * B (32 x 8 e4m3, col), fp32
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// (x0, x1) as one or two f16 terms, t[0] + t[1]
+template <int TERMS>
+__device__ __forceinline__ void f16_terms(float x0, float x1, uint32_t (&t)[TERMS]) {
+  t[0] = pack_f16(x0, x1);
+  if constexpr (TERMS == 2) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&t[0]));
+    t[1] = pack_f16(x0 - h.x, x1 - h.y);
+  }
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// four weights -> two e4m3 terms each, four bytes in order (x0 lowest): hi = e4m3(x), lo = e4m3(x - hi).
-// The weights pass through f16, whose 11 bits are more than the two terms keep.
-__device__ __forceinline__ void split_quad(float x0, float x1, float x2, float x3, uint32_t& hi, uint32_t& lo) {
-  asm("{\n .reg .b32 x, y, g, h;\n .reg .b16 a, b, c, d;\n"
-      " cvt.rn.f16x2.f32 x, %3, %2;\n"
-      " cvt.rn.f16x2.f32 y, %5, %4;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 a, x;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 b, y;\n"
-      " mov.b32 %0, {a, b};\n"
-      " cvt.rn.f16x2.e4m3x2 g, a;\n"
-      " cvt.rn.f16x2.e4m3x2 h, b;\n"
-      " sub.rn.f16x2 x, x, g;\n"
-      " sub.rn.f16x2 y, y, h;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 c, x;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 d, y;\n"
-      " mov.b32 %1, {c, d};\n}"
-      : "=&r"(hi), "=&r"(lo)
-      : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
-}
-// the same for four values of a query row, whose residual may need more than f16 holds: in fp32
-__device__ __forceinline__ void split_quad_f32(const float (&x)[4], uint32_t& hi, uint32_t& lo) {
-  asm("{\n .reg .b32 g, h;\n .reg .f32 s, t, u, v;\n .reg .b16 a, b, c, d, e, f;\n"
-      " cvt.rn.satfinite.e4m3x2.f32 a, %3, %2;\n"
-      " cvt.rn.satfinite.e4m3x2.f32 b, %5, %4;\n"
-      " mov.b32 %0, {a, b};\n"
-      " cvt.rn.f16x2.e4m3x2 g, a;\n"
-      " cvt.rn.f16x2.e4m3x2 h, b;\n"
-      " mov.b32 {c, d}, g;\n mov.b32 {e, f}, h;\n"
-      " cvt.f32.f16 s, c;\n cvt.f32.f16 t, d;\n cvt.f32.f16 u, e;\n cvt.f32.f16 v, f;\n"
-      " sub.rn.f32 s, %2, s;\n sub.rn.f32 t, %3, t;\n sub.rn.f32 u, %4, u;\n sub.rn.f32 v, %5, v;\n"
-      " cvt.rn.satfinite.e4m3x2.f32 c, t, s;\n"
-      " cvt.rn.satfinite.e4m3x2.f32 d, v, u;\n"
-      " mov.b32 %1, {c, d};\n}"
-      : "=&r"(hi), "=&r"(lo)
-      : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]));
+template <int A>
+__device__ __forceinline__ void zero(float (&x)[A][4]) {
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[a][e] = 0.f;
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -326,88 +313,51 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_vals(const T* p, int lane, float (&x)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = ld_f(p, lane * V + i);
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= -kLowest ? a : 0.f;
 }
-
-// The last step of a query row, by one warp: the cached rows' (m, l, o) (base-2 maximum, weight and
-// sum relative to it; m = -inf for none), then the block's own rows in fp32, then the division and the
-// one rounding to T. Lane i holds columns [i * V, (i + 1) * V).
-template <typename T, int HD>
-__device__ __forceinline__ void finish_row(const AttnArgs& p, int b, int g, int r, float m, float l,
-                                           float (&o)[HD / 32], int lane) {
-  constexpr int V = HD / 32;
-  const int group = p.n_heads / p.n_kv;
-  const int h = g * group + r / p.block, s = r % p.block;
-  if (p.blk_k) {
-    float q[V];
-    load_vals<T, V>(static_cast<const T*>(p.q) + b * p.q_batch + s * p.q_row + h * p.q_head, lane, q);
-    const T* bk = static_cast<const T*>(p.blk_k) + b * p.bk_batch + g * p.bk_head;
-    const T* bv = static_cast<const T*>(p.blk_v) + b * p.bv_batch + g * p.bv_head;
-    const float c = p.scale * kLog2e;
-    for (int base = 0; base < p.block; base += 8) {
-      float x[8];
-      float top = kLowest;
+__device__ __forceinline__ float scaled(float x, float f) {  // what is not finite becomes NaN
+  return fabsf(x) <= -kLowest ? x * f : __int_as_float(0x7fffffff);
+}
+// V (a multiple of 4) contiguous values
+template <typename T, int V>
+__device__ __forceinline__ void load_vals(const T* p, bool vec, float (&x)[V]) {
+  if (vec) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = 0.f;
-        if (base + j < p.block) {
-          float k[V];
-          load_vals<T, V>(bk + (base + j) * p.bk_row, lane, k);
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[j] = fmaf(q[i], k[i], x[j]);
-        }
+    for (int i = 0; i < V; i += 4) {
+      if constexpr (std::is_same<T, float>::value) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i);
+        x[i] = v.x;
+        x[i + 1] = v.y;
+        x[i + 2] = v.z;
+        x[i + 3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + i);
+        x[i] = __uint_as_float(v.x << 16);
+        x[i + 1] = __uint_as_float(v.x & 0xffff0000u);
+        x[i + 2] = __uint_as_float(v.y << 16);
+        x[i + 3] = __uint_as_float(v.y & 0xffff0000u);
       }
-#pragma unroll
-      for (int w = 16; w; w >>= 1) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += __shfl_xor_sync(0xffffffffu, x[j], w);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] *= c;
-        if (base + j < p.block) top = fmaxf(top, x[j]);
-      }
-      const float mn = fmaxf(m, top);
-      const float alpha = ex2(m - mn);
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] *= alpha;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (base + j < p.block) {
-          const float w = exp2f(x[j] - mn);
-          float v[V];
-          load_vals<T, V>(bv + (base + j) * p.bv_row, lane, v);
-          l += w;
-#pragma unroll
-          for (int i = 0; i < V; ++i) o[i] = fmaf(w, v[i], o[i]);
-        }
-      }
-      m = mn;
     }
-  }
-  T* out = static_cast<T*>(p.out) + ((int64_t(b) * p.block + s) * p.n_heads + h) * HD + lane * V;
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = st_f<T>(l == 0.f ? 0.f : o[i] / l);
+    for (int i = 0; i < V; ++i) x[i] = ld_f(p, i);
+  }
 }
 
 // shared memory of the kernel, in bytes from its start
 struct MmaSmem {
-  int buf, qf, rowf, ml, top, scales, full, empty, sums, P, bytes;
+  int buf, qf, rowf, ml, scales, full, empty, sums, P, bytes;
 };
-__host__ __device__ inline MmaSmem mma_smem(int hd, int mt, int mg, int depth, int batch) {
+__host__ __device__ inline MmaSmem mma_smem(int hd, int mt, int mg, int terms, int depth, int batch) {
   MmaSmem s;
   const int warps = mma_warps(hd), rows = 16 * mt * mg, tl = warps / mg, stages = depth * tl;
   s.buf = stages * 2 * kTile * hd;
-  const int halves = tl / 2 * mg;  // warps that hand their sums over in the first round
-  s.qf = s.buf + (halves * 16 * mt > rows ? halves * 16 * mt : rows) * hd * 4;
-  s.rowf = s.qf + rows * hd * 2;
+  s.qf = s.buf + tl / 2 * rows * hd * 4;  // the lanes that hand their sums over in the first round
+  s.rowf = s.qf + rows * hd * 2 * terms;
   s.ml = s.rowf + rows * 4;
-  s.top = s.ml + warps * 16 * mt * 8;
-  s.scales = s.top + rows * 8;
+  s.scales = s.ml + warps * 16 * mt * 16;
   s.full = s.scales + stages * 8;
   s.empty = s.full + stages * 16;
   s.sums = s.empty + stages * 8;
@@ -420,19 +370,18 @@ template <typename T, int HD, int MT>
 __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(const AttnArgs p, const MmaPlan pl) {
   constexpr int kWarps = mma_warps(HD);
   constexpr int kThreads = kWarps * 32;
-  constexpr int NT = HD / 8;      // column tiles of the output
-  constexpr int KS = HD / 32;     // k32 steps of q k
-  constexpr int CH = HD / 64;     // 16-byte chunks of a key row per thread
-  constexpr int V = HD / 32;
+  constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
+  constexpr int NT = HD / 8;   // column tiles of the output
+  constexpr int KS = HD / 16;  // k16 steps of q k
+  constexpr int CH = HD / 64;  // 16-byte chunks of a key row per thread
   constexpr int kKeyBytes = kTile * HD;
   constexpr int kWarpRows = 16 * MT;
   extern __shared__ __align__(128) uint8_t smem[];
-  const MmaSmem L = mma_smem(HD, MT, pl.mg, pl.depth, p.batch);
+  const MmaSmem L = mma_smem(HD, MT, pl.mg, TERMS, pl.depth, p.batch);
   float* buf = reinterpret_cast<float*>(smem + L.buf);
   uint32_t* qf = reinterpret_cast<uint32_t*>(smem + L.qf);
   float* rowf = reinterpret_cast<float*>(smem + L.rowf);
-  float2* ml = reinterpret_cast<float2*>(smem + L.ml);
-  float2* top = reinterpret_cast<float2*>(smem + L.top);
+  float4* ml = reinterpret_cast<float4*>(smem + L.ml);
   float2* scales = reinterpret_cast<float2*>(smem + L.scales);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.full);  // per stage: keys, values
   uint64_t* empty = reinterpret_cast<uint64_t*>(smem + L.empty);
@@ -460,7 +409,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
   if (n_tiles <= 0) return;
 
-  // ---- filling the stages: a cursor over the tiles that this lane fetches, one lane of warps my_mg == 0
+  // ---- filling the stages: a cursor over the tiles that this lane fetches, one thread of warps my_mg == 0
   auto page_at = [&](const Place& a) -> int {  // the page of a tile, -1: nothing to fetch
     if (a.t * kTile >= seq_len(p, a.b)) return -1;
     const int pg = __ldg(p.table + int64_t(a.b) * p.table_stride + a.t * kTile / p.page);
@@ -499,7 +448,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     }
   };
   if (my_mg == 0 && my_tl < n_tiles) {
-    cur = place_of(P, p.batch, hr, start + my_tl);
+    cur = place_of(P, p.batch, hr, start + my_tl, 0);
     for (int i = my_tl; i < min(S, n_tiles); i += tl) {
       const int pg = page_at(cur);
       if (lane == 0) {
@@ -513,17 +462,18 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
 
   // ---- the range, unit by unit
   for (int a0 = 0; a0 < n_tiles;) {
-    const Place un = place_of(P, p.batch, hr, start + a0);
+    const Place un = place_of(P, p.batch, hr, start + a0, 0);
     const int a1 = min(n_tiles, a0 + un.T - un.t);
+    const bool last = un.t + a1 - a0 == un.T, whole = last && un.t == 0;
     const int g = un.u / pl.row_blocks, r0 = (un.u % pl.row_blocks) * cta_rows;
     const int n_rows = min(cta_rows, pl.rows - r0);
     const int len = seq_len(p, un.b);
     const int group = p.n_heads / p.n_kv;
 
-    // q: a warp per row, split into two e4m3 terms in the A-fragment order of the products
+    // q: a warp per row, in f16 terms in the A-fragment order of the products
     __syncthreads();  // the previous unit's fragments and sums are used up
     for (int r = warp; r < cta_rows; r += kWarps) {
-      constexpr int QV = HD == 64 ? 4 : V;  // values per lane, whole words of codes
+      constexpr int QV = HD == 256 ? 8 : 4;  // values per thread
       const bool mine = lane * QV < HD;
       float x[QV];
       int e = kKv8MinExp;
@@ -533,37 +483,35 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         const int rr = r0 + r;
         if (mine)
           load_vals<T, QV>(static_cast<const T*>(p.q) + un.b * p.q_batch + (rr % p.block) * p.q_row +
-                               (g * group + rr / p.block) * p.q_head,
-                           lane, x);
+                               (g * group + rr / p.block) * p.q_head + lane * QV,
+                           pl.vec_q, x);
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < QV; ++i) mx = fmaxf(mx, fabsf(x[i]) <= -kLowest ? fabsf(x[i]) : 0.f);
+        for (int i = 0; i < QV; ++i) mx = fmaxf(mx, finite_abs(x[i]));
         e = kv8_scale_exp(kv8_warp_max(mx));
         // the sign of the factor goes into q: the row maximum is taken before the factor
         const float inv = p.scale < 0.f ? -kv8_exp2i(-e) : kv8_exp2i(-e);
 #pragma unroll
-        for (int i = 0; i < QV; ++i) x[i] = fabsf(x[i]) <= -kLowest ? x[i] * inv : __int_as_float(0x7fffffff);
+        for (int i = 0; i < QV; ++i) x[i] = scaled(x[i], inv);
       }
       if (lane == 0) rowf[r] = r < n_rows ? fabsf(p.scale) * kLog2e * kv8_exp2i(e) : 0.f;
+      if (mine) {
 #pragma unroll
-      for (int i = 0; i < QV; i += 4) {
-        uint32_t hi, lo;
-        const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
-        split_quad_f32(four, hi, lo);
-        const int d = lane * QV + i, chunk = d >> 4, w = (d & 15) >> 2;
-        int c, ks;  // the thread column and k32 step that multiply these columns
-        if constexpr (HD == 64) {
-          c = chunk;
-          ks = w >> 1;
-        } else {
-          c = (chunk & 7) >> 1;
-          ks = (chunk >> 3) * 4 + (chunk & 1) * 2 + (w >> 1);
-        }
-        const int reg = (w & 1) * 2 + ((r >> 3) & 1);
-        const int at = ((((r >> 4) * KS + ks) * 2) * 32 + (r & 7) * 4 + c) * 4 + reg;
-        if (mine) {
-          qf[at] = hi;
-          qf[at + 32 * 4] = lo;  // the lo fragment follows the hi one
+        for (int i = 0; i < QV; i += 4) {
+          // thread column c multiplies chunks 2 c and 2 c + 1 of each 128 columns (chunk c of 64), four
+          // columns per k16 step: its first two are k = 2 c, 2 c + 1, the others k + 8
+          const int d = lane * QV + i, chunk = d >> 4, w = (d & 15) >> 2;
+          const int c = HD == 64 ? chunk : (chunk & 7) >> 1;
+          const int ks = HD == 64 ? w : (chunk >> 3) * 8 + (chunk & 1) * 4 + w;
+          uint32_t lo2[TERMS], hi2[TERMS];
+          f16_terms<TERMS>(x[i], x[i + 1], lo2);
+          f16_terms<TERMS>(x[i + 2], x[i + 3], hi2);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) {
+            uint32_t* q4 = qf + ((((r >> 4) * KS + ks) * TERMS + t) * 32 + (r & 7) * 4 + c) * 4 + ((r >> 3) & 1);
+            q4[0] = lo2[t];
+            q4[2] = hi2[t];
+          }
         }
       }
     }
@@ -574,9 +522,10 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       cf[mt][0] = rowf[my_mg * kWarpRows + mt * 16 + gq];
       cf[mt][1] = rowf[my_mg * kWarpRows + mt * 16 + gq + 8];
     }
-    const uint4* my_q = reinterpret_cast<const uint4*>(qf) + my_mg * MT * KS * 2 * 32 + lane;
+    const uint4* my_q = reinterpret_cast<const uint4*>(qf) + my_mg * MT * KS * TERMS * 32 + lane;
 
     float o[MT][NT][4], m[MT][2], l[MT][2];
+    int rv = -200, top_rv = -200;  // the sums' value exponent, and the largest seen
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -585,6 +534,172 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.f;
       m[mt][0] = m[mt][1] = -INFINITY;
       l[mt][0] = l[mt][1] = 0.f;
+    }
+
+    // scores s of NJ 8-key tiles -> weights in place (f16-ready), sums and references brought up to date.
+    // bad(j, e): key column e of tile j is not to be attended; `some`: there are such.
+    auto weigh = [&](auto nj, auto& s, float k_scale, int ev, bool some, auto bad) {
+      constexpr int NJ = decltype(nj)::value;
+      if (some) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (bad(j, e)) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = s[mt][j][2 + e] = kLowest;
+            }
+      }
+      float top[MT][2];
+      bool grown = false;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = kLowest;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * h], s[mt][j][2 * h + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          top[mt][h] = mx * (cf[mt][h] * k_scale);
+          grown |= top[mt][h] > m[mt][h] + kPGrow;
+        }
+      top_rv = max(top_rv, ev);
+      const int want_rv = ev > rv || ev < rv - 10 ? max(ev, top_rv - 40) : rv;
+      if (__any_sync(0xffffffffu, grown) || want_rv != rv) {
+        const float fv = rv <= -200 ? 0.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
+        rv = want_rv;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float f[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mn = top[mt][h] > m[mt][h] + kPGrow ? top[mt][h] : m[mt][h];
+            const float a = m[mt][h] == mn ? 1.f : ex2(m[mt][h] - mn);
+            m[mt][h] = mn;
+            l[mt][h] *= a;
+            f[h] = a * fv;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][n][e] *= f[e >> 1];
+        }
+      }
+      const int dv = max(ev - rv, -60);  // <= 0
+      const float back = kv8_exp2i(-dv);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float c = cf[mt][h] * k_scale, off = kPScale + float(dv) - m[mt][h];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[mt][j][2 * h + e] = ex2(fmaf(s[mt][j][2 * h + e], c, off));
+        }
+      if (some) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (bad(j, e)) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = s[mt][j][2 + e] = 0.f;
+            }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) sum += s[mt][j][2 * h] + s[mt][j][2 * h + 1];
+          l[mt][h] = fmaf(sum, back, l[mt][h]);
+        }
+    };
+
+    // ---- the block's own rows: 16 keys at a time, by the lanes behind the unit's last tile
+    if (last && p.blk_k) {
+      const T* bk = static_cast<const T*>(p.blk_k) + un.b * p.bk_batch + g * p.bk_head;
+      const T* bv = static_cast<const T*>(p.blk_v) + un.b * p.bv_batch + g * p.bv_head;
+      for (int kb = ((my_tl - a1 % tl + tl) % tl) * 16; kb < p.block; kb += 16 * tl) {
+        // one power of two for the 16 keys' rows and one for the values', as a page would have
+        float mk = 0.f, mv = 0.f;
+        for (int r = kb + (lane >> 4); r < min(kb + 16, p.block); r += 2)
+#pragma unroll
+          for (int d = (lane & 15) * 4; d < HD; d += 64) {
+            float x[4], y[4];
+            load_vals<T, 4>(bk + r * p.bk_row + d, pl.vec_blk, x);
+            load_vals<T, 4>(bv + r * p.bv_row + d, pl.vec_blk, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              mk = fmaxf(mk, finite_abs(x[i]));
+              mv = fmaxf(mv, finite_abs(y[i]));
+            }
+          }
+        const int ek = kv8_scale_exp(kv8_warp_max(mk)), ev = kv8_scale_exp(kv8_warp_max(mv));
+        const float ik = kv8_exp2i(-ek), iv = kv8_exp2i(-ev);
+        // column n of key tile j is key kb + 4 * (n / 2) + 2 j + n % 2
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = kb + 4 * (gq >> 1) + 2 * j + (gq & 1);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const int d = HD == 64 ? cq * 16 + ks * 4 : (ks >> 3) * 128 + (2 * cq + ((ks >> 2) & 1)) * 16 + (ks & 3) * 4;
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (key < p.block) load_vals<T, 4>(bk + key * p.bk_row + d, pl.vec_blk, x);
+            uint32_t b0[TERMS], b1[TERMS];
+            f16_terms<TERMS>(scaled(x[0], ik), scaled(x[1], ik), b0);
+            f16_terms<TERMS>(scaled(x[2], ik), scaled(x[3], ik), b1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int tq = 0; tq < TERMS; ++tq) {
+                const uint4 q = my_q[((mt * KS + ks) * TERMS + tq) * 32];
+#pragma unroll
+                for (int tk = 0; tk < TERMS; ++tk) mma(s[mt][j], q, b0[tk], b1[tk]);
+              }
+          }
+        }
+        weigh(std::integral_constant<int, 2>(), s, kv8_exp2i(ek), ev, kb + 16 > p.block,
+                                     [&](int j, int e) { return kb + 4 * cq + 2 * j + e >= p.block; });
+        uint4 pf[MT][TERMS];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t f[4][TERMS];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f16_terms<TERMS>(s[mt][i >> 1][2 * (i & 1)], s[mt][i >> 1][2 * (i & 1) + 1], f[i]);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) pf[mt][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = kb + 4 * cq + i;
+            x[i] = key < p.block ? scaled(ld_f(bv, key * p.bv_row + 8 * n + gq), iv) : 0.f;
+          }
+          uint32_t b0[TERMS], b1[TERMS];
+          f16_terms<TERMS>(x[0], x[1], b0);
+          f16_terms<TERMS>(x[2], x[3], b1);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int tp = 0; tp < TERMS; ++tp)
+#pragma unroll
+              for (int tv = 0; tv < TERMS; ++tv) mma(o[mt][n], pf[mt][tp], b0[tv], b1[tv]);
+          }
+        }
+      }
     }
 
     for (int i = a0 + (my_tl - a0 % tl + tl) % tl; i < a1; i += tl) {
@@ -610,27 +725,37 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         const uint32_t krow = kb + (16 * (gq >> 1) + (gq & 1)) * HD;
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
-          uint4 q[MT][2][2];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int tq = 0; tq < TERMS; ++tq) {
+            uint4 q[MT][4];
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-              for (int x = 0; x < 2; ++x) q[mt][hf][x] = my_q[((mt * KS + ch * 2 + hf) * 2 + x) * 32];
+              for (int w = 0; w < 4; ++w) q[mt][w] = my_q[((mt * KS + ch * 4 + w) * TERMS + tq) * 32];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint32_t addr = krow + 2 * j * HD;
-            if constexpr (HD == 64)
-              addr += cq * 16;
-            else
-              addr += ((ch >> 1) * 8 + ((2 * cq + (ch & 1)) ^ (((2 * j) & 7) | (gq & 1)))) * 16;
-            const uint4 k = lds128(addr);
+            for (int j = 0; j < 8; ++j) {
+              uint32_t addr = krow + 2 * j * HD;
+              if constexpr (HD == 64)
+                addr += cq * 16;
+              else
+                addr += ((ch >> 1) * 8 + ((2 * cq + (ch & 1)) ^ (((2 * j) & 7) | (gq & 1)))) * 16;
+              const uint4 k = lds128(addr);
+              const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
+              float t[MT][4];
+              if constexpr (TERMS == 2) zero(t);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma_e4m3(s[mt][j], q[mt][0][0], k.x, k.y);
-              mma_e4m3(s[mt][j], q[mt][0][1], k.x, k.y);
-              mma_e4m3(s[mt][j], q[mt][1][0], k.z, k.w);
-              mma_e4m3(s[mt][j], q[mt][1][1], k.z, k.w);
+              for (int w = 0; w < 4; ++w) {
+                uint32_t b0, b1;
+                e4m3x4_to_f16(kw[w], b0, b1);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) mma(TERMS == 2 ? t[mt] : s[mt][j], q[mt][w], b0, b1);
+              }
+              if constexpr (TERMS == 2) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) s[mt][j][e] += t[mt][e];
+              }
             }
           }
         }
@@ -639,83 +764,50 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
           if (lane == 0) fetch(st, 0, cur, next_pg);
         }
         ok = mbar_wait(full + 2 * st + 1, (i / S) & 1);
-        const float v_scale = scales[st].y;
-        if (nv < kTile) {
+        weigh(std::integral_constant<int, 8>(), s, k_scale, kv8_exponent(scales[st].y), nv < kTile,
+                                     [&](int j, int e) { return 16 * cq + 2 * j + e >= nv; });
+        uint4 pf[MT][4][TERMS];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (16 * cq + 2 * j + e >= nv) {
+          for (int w = 0; w < 4; ++w) {
+            uint32_t f[4][TERMS];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = s[mt][j][2 + e] = kLowest;
-              }
-        }
-        uint4 ph[MT][2], pw[MT][2];  // the weights' two terms as A fragments of the two k32 steps
-        float alpha[MT][2], beta[MT][2];
+            for (int x = 0; x < 4; ++x)
+              f16_terms<TERMS>(s[mt][2 * w + (x >> 1)][2 * (x & 1)], s[mt][2 * w + (x >> 1)][2 * (x & 1) + 1], f[x]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx = kLowest;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * h], s[mt][j][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float c = cf[mt][h] * k_scale, mt_ = mx * c, off = kPScale - mt_;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float& x = s[mt][j][2 * h + e];
-                x = ex2(fmaf(x, c, off));
-                if (nv < kTile && 16 * cq + 2 * j + e >= nv) x = 0.f;
-                sum += x;
-              }
-            const float mn = fmaxf(m[mt][h], mt_);
-            alpha[mt][h] = ex2(m[mt][h] - mn);
-            const float bt = ex2(mt_ - mn);
-            l[mt][h] = fmaf(l[mt][h], alpha[mt][h], bt * sum);
-            beta[mt][h] = bt * v_scale;
-            m[mt][h] = mn;
+            for (int t = 0; t < TERMS; ++t) pf[mt][w][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
           }
-#pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            const float(&x)[8][4] = s[mt];
-            const int j = 4 * k2;
-            split_quad(x[j][0], x[j][1], x[j + 1][0], x[j + 1][1], ph[mt][k2].x, pw[mt][k2].x);
-            split_quad(x[j][2], x[j][3], x[j + 1][2], x[j + 1][3], ph[mt][k2].y, pw[mt][k2].y);
-            split_quad(x[j + 2][0], x[j + 2][1], x[j + 3][0], x[j + 3][1], ph[mt][k2].z, pw[mt][k2].z);
-            split_quad(x[j + 2][2], x[j + 2][3], x[j + 3][2], x[j + 3][3], ph[mt][k2].w, pw[mt][k2].w);
-          }
-        }
         // values: columns 8 n + gq, this thread's 16 keys. Codes behind the length are cleared: a weight of
         // zero would not take a NaN there out
-        uint32_t keep[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int k = nv - (16 * cq + 4 * w);
-          keep[w] = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
-        }
         const uint32_t vrow = vb + gq * kTile + cq * 16;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint4 v = lds128(vrow + n * 8 * kTile);
+          const uint4 v = lds128(vrow + n * 8 * kTile);
+          uint32_t vw[4] = {v.x, v.y, v.z, v.w};
           if (nv < kTile) {
-            v.x &= keep[0];
-            v.y &= keep[1];
-            v.z &= keep[2];
-            v.w &= keep[3];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int k = nv - (16 * cq + 4 * w);
+              vw[w] &= k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+            }
           }
+          float t4[MT][4];
+          if constexpr (TERMS == 2) zero(t4);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            float t[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_e4m3(t, ph[mt][0], v.x, v.y);
-            mma_e4m3(t, pw[mt][0], v.x, v.y);
-            mma_e4m3(t, ph[mt][1], v.z, v.w);
-            mma_e4m3(t, pw[mt][1], v.z, v.w);
+          for (int w = 0; w < 4; ++w) {
+            uint32_t b0, b1;
+            e4m3x4_to_f16(vw[w], b0, b1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][n][e] = fmaf(t[e], beta[mt][e >> 1], o[mt][n][e] * alpha[mt][e >> 1]);
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int t = 0; t < TERMS; ++t) mma(TERMS == 2 ? t4[mt] : o[mt][n], pf[mt][w][t], b0, b1);
+          }
+          if constexpr (TERMS == 2) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][n][e] += t4[mt][e];
           }
         }
       } else if (ok) {  // nothing to read; its values' half may still be on its way
@@ -735,7 +827,9 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       }
     }
 
-    // ---- the unit's sums of all lane groups into those of group 0
+    // ---- the unit's sums into those of the first lane that had a tile: lane number x from there
+    const int x_tl = (my_tl - a0 % tl + tl) % tl;
+    const int busy = min(tl, a1 - a0 + (last && p.blk_k ? (p.block + 15) / 16 : 0));
     const int wrow = warp * kWarpRows;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -744,23 +838,23 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         float x = l[mt][h];
         x += __shfl_xor_sync(0xffffffffu, x, 1);
         x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (cq == 0) ml[wrow + mt * 16 + h * 8 + gq] = make_float2(m[mt][h], x);
+        if (cq == 0) ml[wrow + mt * 16 + h * 8 + gq] = make_float4(m[mt][h], x, float(rv), 0.f);
       }
     __syncthreads();
+    float M[MT][2], W[MT][2], E = -200.f;
+    for (int t = 0; t < tl; ++t) E = fmaxf(E, ml[(my_mg * tl + t) * kWarpRows].z);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = mt * 16 + h * 8 + gq;
-        float M = -INFINITY, W = 0.f;
-        for (int t = 0; t < tl; ++t) M = fmaxf(M, ml[(my_mg * tl + t) * kWarpRows + r].x);
-        const float ref = M == -INFINITY ? 0.f : M;
-        for (int t = 0; t < tl; ++t) {
-          const float2 x = ml[(my_mg * tl + t) * kWarpRows + r];
-          W = fmaf(x.y, ex2(x.x - ref), W);
-        }
-        if (my_tl == 0 && cq == 0) top[my_mg * kWarpRows + r] = make_float2(M - kPScale, W);
-        const float f = ex2(m[mt][h] - ref);
+        const float4* row = ml + my_mg * tl * kWarpRows + mt * 16 + h * 8 + gq;
+        float a = -INFINITY, w = 0.f;
+        for (int t = 0; t < tl; ++t) a = fmaxf(a, row[t * kWarpRows].x);
+        const float ref = a == -INFINITY ? 0.f : a;
+        for (int t = 0; t < tl; ++t) w = fmaf(row[t * kWarpRows].y, ex2(row[t * kWarpRows].x - ref), w);
+        M[mt][h] = a;
+        W[mt][h] = w;
+        const float f = ex2(m[mt][h] - ref + fmaxf(float(rv) - E, -126.f));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           o[mt][n][2 * h] *= f;
@@ -768,8 +862,9 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         }
       }
     for (int half = tl / 2; half >= 1; half /= 2) {
-      float4* slot = reinterpret_cast<float4*>(buf) + (my_mg * half + my_tl % half) * (kWarpRows * HD / 4) + lane;
-      if (my_tl >= half && my_tl < 2 * half) {
+      if (half >= busy) continue;
+      float4* slot = reinterpret_cast<float4*>(buf) + (my_mg * half + x_tl % half) * (kWarpRows * HD / 4) + lane;
+      if (x_tl >= half && x_tl < min(2 * half, busy)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -777,7 +872,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
             slot[(mt * NT + n) * 32] = make_float4(o[mt][n][0], o[mt][n][1], o[mt][n][2], o[mt][n][3]);
       }
       __syncthreads();
-      if (my_tl < half) {
+      if (x_tl < half && x_tl + half < busy) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -791,31 +886,36 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       }
       __syncthreads();
     }
-    const bool whole = un.t == 0 && a1 - a0 == un.T;
-    const int slot = 2 * blockIdx.x + (a0 == 0 && un.t > 0 ? 0 : 1);
-    if (my_tl == 0) {  // rows as rows: to shared memory for the last step, or to the workspace
-      float* dst = whole ? buf : pl.part + int64_t(slot) * cta_rows * HD;
+    if (x_tl == 0) {
+      const int slot = 2 * blockIdx.x + (a0 == 0 && un.t > 0 ? 0 : 1);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = my_mg * kWarpRows + mt * 16 + h * 8 + gq;
+          if (whole) {
+            if (r >= n_rows) continue;
+            const int rr = r0 + r;
+            T* out = static_cast<T*>(p.out) +
+                     ((int64_t(un.b) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + 2 * cq;
+            const float inv = W[mt][h] == 0.f ? 0.f : 1.f / W[mt][h], fe = kv8_exp2i(max(int(E), -126));
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float2*>(dst + r * HD + 8 * n + 2 * cq) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+            for (int n = 0; n < NT; ++n) {
+              const float y0 = W[mt][h] == 0.f ? 0.f : o[mt][n][2 * h] * inv * fe;
+              const float y1 = W[mt][h] == 0.f ? 0.f : o[mt][n][2 * h + 1] * inv * fe;
+              if constexpr (std::is_same<T, float>::value)
+                *reinterpret_cast<float2*>(out + 8 * n) = make_float2(y0, y1);
+              else
+                *reinterpret_cast<__nv_bfloat162*>(out + 8 * n) = __floats2bfloat162_rn(y0, y1);
+            }
+          } else {
+            float* dst = pl.part + (int64_t(slot) * cta_rows + r) * HD + 2 * cq;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+            if (cq == 0) pl.ml[int64_t(slot) * cta_rows + r] = make_float4(M[mt][h], W[mt][h], E, 0.f);
+          }
         }
-    }
-    __syncthreads();
-    if (whole) {
-      for (int r = warp; r < n_rows; r += kWarps) {
-        float x[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = buf[r * HD + lane * V + i];
-        finish_row<T, HD>(p, un.b, g, r0 + r, top[r].x, top[r].y, x, lane);
-      }
-    } else {
-      float2* dst = reinterpret_cast<float2*>(pl.ml) + int64_t(slot) * cta_rows;
-      for (int r = tid; r < cta_rows; r += kThreads) dst[r] = top[r];
     }
     a0 = a1;
   }
@@ -825,10 +925,10 @@ constexpr int kCombineWarps = 8;
 
 // Joins the units that were cut: CTA (i, y) looks at the cut between ranges i and i + 1; if it is its unit's
 // first, it joins the unit's rows y * 8 .. y * 8 + 7, a warp each: the partial sums of its ranges in
-// order, then finish_row.
+// order, then the division and the one rounding to T.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(const AttnArgs p, const MmaPlan pl, int ctas,
-                                                                        int cta_rows) {
+__global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(const AttnArgs p, const MmaPlan pl,
+                                                                               int ctas, int cta_rows) {
   constexpr int V = HD / 32;
   extern __shared__ __align__(16) int P[];
   __shared__ int sums[kCombineWarps];
@@ -840,7 +940,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   const int total = P[p.batch] * hr;
   const int x = cut(P, p.batch, hr, i + 1, ctas, pl.snap, pl.least);
   if (x >= total || x == 0) return;
-  const Place un = place_of(P, p.batch, hr, x);
+  const Place un = place_of(P, p.batch, hr, x, 0);
   const int u0 = x - un.t, u1 = u0 + un.T;
   if (un.t == 0 || cut(P, p.batch, hr, i, ctas, pl.snap, pl.least) > u0) return;
   for (int k = i + tid; k <= ctas; k += kCombineWarps * 32) cuts[k] = cut(P, p.batch, hr, k, ctas, pl.snap, pl.least);
@@ -852,11 +952,15 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   if (r >= min(cta_rows, pl.rows - r0)) return;
   // range i's part is its last (slot 2 i + 1), the others' their first (slot 2 k); empty ranges have none
   auto slot_of = [&](int k) { return int64_t(k == i ? 2 * i + 1 : 2 * k) * cta_rows + r; };
-  const float2* ml = reinterpret_cast<const float2*>(pl.ml);
-  float M = -INFINITY;
+  float M = -INFINITY, E = -200.f;
   for (int k = i + lane; k <= last; k += 32)
-    if (cuts[k] < cuts[k + 1]) M = fmaxf(M, ml[slot_of(k)].x);
+    if (cuts[k] < cuts[k + 1]) {
+      const float4 w = pl.ml[slot_of(k)];
+      M = fmaxf(M, w.x);
+      E = fmaxf(E, w.z);
+    }
   M = kv8_warp_max(M);
+  E = kv8_warp_max(E);
   const float ref = M == -INFINITY ? 0.f : M;
   float l = 0.f, o[V];
 #pragma unroll
@@ -865,14 +969,19 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   for (int k = i; k <= last; ++k) {
     if (cuts[k] == cuts[k + 1]) continue;
     const int64_t s = slot_of(k);
-    const float2 w = ml[s];
-    const float f = ex2(w.x - ref);
+    const float4 w = pl.ml[s];
+    const float f = ex2(w.x - ref), fo = f * ex2(fmaxf(w.z - E, -126.f));
     const float* src = pl.part + s * HD + lane * V;
     l = fmaf(w.y, f, l);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = fmaf(src[j], f, o[j]);
+    for (int j = 0; j < V; ++j) o[j] = fmaf(src[j], fo, o[j]);
   }
-  finish_row<T, HD>(p, un.b, g, r0 + r, M, l, o, lane);
+  const int rr = r0 + r, group = p.n_heads / p.n_kv;
+  T* out = static_cast<T*>(p.out) +
+           ((int64_t(un.b) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + lane * V;
+  const float inv = 1.f / l, fe = kv8_exp2i(max(int(E), -126));
+#pragma unroll
+  for (int j = 0; j < V; ++j) out[j] = st_f<T>(l == 0.f ? 0.f : o[j] * inv * fe);
 }
 
 constexpr int kMmaSmemMax = 232448;  // 227 KB
@@ -881,11 +990,11 @@ struct MmaShape {
   int mt, mg, row_blocks, cta_rows;
 };
 // Query rows of a KV head -> rows per warp and warps per tile: 16 rows where that is all, else 32 (one
-// 16-row tile at head_dim 256, whose sums fill the registers), and more warps over the same tile
-// up to 128 rows (64 at head_dim 256).
-MmaShape mma_shape(int rows, int hd) {
+// 16-row tile at head_dim 256 and in two terms, whose sums or weights fill the registers), and more
+// warps over the same tile up to 128 rows (64 at head_dim 256).
+MmaShape mma_shape(int rows, int hd, int dtype) {
   MmaShape s;
-  s.mt = rows <= 16 || hd == 256 ? 1 : 2;
+  s.mt = rows <= 16 || hd == 256 || dtype == DSM_DT_F32 ? 1 : 2;
   const int most = hd == 256 ? 64 : 128;
   s.mg = 1;
   while (16 * s.mt * s.mg < std::min(rows, most)) s.mg *= 2;
@@ -896,9 +1005,10 @@ MmaShape mma_shape(int rows, int hd) {
 
 template <typename T, int HD, int MT>
 int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cudaStream_t s) {
+  constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
   int depth = std::max(kMaxDepth, sh.mg);
-  while (depth > 1 && mma_smem(HD, MT, sh.mg, depth, a.batch).bytes > kMmaSmemMax) --depth;
-  const int smem = mma_smem(HD, MT, sh.mg, depth, a.batch).bytes;
+  while (depth > 1 && mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes > kMmaSmemMax) --depth;
+  const int smem = mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes;
   if (smem > kMmaSmemMax) return fail(DSM_ERR_UNSUPPORTED, "dsm_gqa_attn_kv8: batch too large for shared memory");
   pl.depth = depth;
   auto k = kv8_attn_mma_kernel<T, HD, MT>;
@@ -908,32 +1018,40 @@ int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cuda
   const int st = check_launch("gqa_attn_kv8");
   if (st != DSM_OK || ctas == 1) return st;
   const dim3 grid(unsigned(ctas - 1), unsigned(ceil_div(std::min(sh.cta_rows, pl.rows), kCombineWarps)));
-  kv8_attn_combine_kernel<T, HD><<<grid, kCombineWarps * 32, size_t(a.batch + ctas + 2) * 4, s>>>(a, pl, ctas, sh.cta_rows);
+  kv8_attn_combine_kernel<T, HD><<<grid, kCombineWarps * 32, size_t(a.batch + ctas + 2) * 4, s>>>(a, pl, ctas,
+                                                                                                   sh.cta_rows);
   return check_launch("gqa_attn_kv8 combine");
 }
 
-size_t mma_ws_bytes(const MmaShape& sh, int hd) {
-  return size_t(2 * num_sms()) * sh.cta_rows * (size_t(hd) + 2) * 4;
+size_t mma_ws_bytes(int cta_rows, int hd) { return size_t(2 * num_sms()) * cta_rows * (size_t(hd) + 4) * 4; }
+
+bool vec_ok(const void* p, int64_t s0, int64_t s1, int64_t s2, size_t bytes) {
+  const size_t e = bytes / 4;  // one load takes four values
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && s0 * e % bytes == 0 && s1 * e % bytes == 0 && s2 * e % bytes == 0;
 }
 
 template <typename T>
 int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
-  const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd);
+  const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd, sizeof(T) == 4 ? DSM_DT_F32 : DSM_DT_BF16);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * sh.row_blocks;
   if (most > 0x7fffffff) return fail(DSM_ERR_UNSUPPORTED, "dsm_gqa_attn_kv8: block table too large");
-  const int ctas = int(std::min<int64_t>(num_sms(), std::max<int64_t>(most, 1)));
+  const int ctas = int(std::min<int64_t>(num_sms(), most));
   MmaPlan pl;
   pl.mg = sh.mg;
   pl.row_blocks = sh.row_blocks;
   pl.rows = a.n_heads / a.n_kv * a.block;
   pl.depth = 0;
   pl.snap = std::max(1, mma_warps(hd) / sh.mg / 2);
-  pl.least = pl.snap;
+  pl.least = kUnitCost;
+  pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 4 * sizeof(T));
+  pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 4 * sizeof(T)) &&
+               vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 4 * sizeof(T));
   pl.part = static_cast<float*>(ws);
-  pl.ml = pl.part + size_t(2 * num_sms()) * sh.cta_rows * hd;
+  pl.ml = reinterpret_cast<float4*>(pl.part + size_t(2 * num_sms()) * sh.cta_rows * hd);
+  constexpr int kWide = sizeof(T) == 4 ? 1 : 2;
   switch (hd) {
-    case 64: return sh.mt == 1 ? launch_mma<T, 64, 1>(a, sh, pl, ctas, s) : launch_mma<T, 64, 2>(a, sh, pl, ctas, s);
-    case 128: return sh.mt == 1 ? launch_mma<T, 128, 1>(a, sh, pl, ctas, s) : launch_mma<T, 128, 2>(a, sh, pl, ctas, s);
+    case 64: return sh.mt == 1 ? launch_mma<T, 64, 1>(a, sh, pl, ctas, s) : launch_mma<T, 64, kWide>(a, sh, pl, ctas, s);
+    case 128: return sh.mt == 1 ? launch_mma<T, 128, 1>(a, sh, pl, ctas, s) : launch_mma<T, 128, kWide>(a, sh, pl, ctas, s);
     default: return launch_mma<T, 256, 1>(a, sh, pl, ctas, s);
   }
 }
@@ -947,7 +1065,9 @@ extern "C" size_t dsm_gqa_attn_kv8_workspace_bytes(int batch, int block, int n_h
   if (batch <= 0 || batch > kKv8MaxBatch || block <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0 ||
       !kv8_head_dim_ok(head_dim))
     return 0;
-  return mma_ws_bytes(mma_shape(n_heads / n_kv * block, head_dim), head_dim);
+  const int rows = n_heads / n_kv * block;
+  return mma_ws_bytes(std::max(mma_shape(rows, head_dim, DSM_DT_F32).cta_rows, mma_shape(rows, head_dim, DSM_DT_BF16).cta_rows),
+                      head_dim);
 }
 
 extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const int32_t* block_table,
@@ -1003,7 +1123,8 @@ extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const
                       d->scale,
                       out};
   cudaStream_t s = as_stream(stream);
-  if (d->dtype == DSM_DT_BF16 && attn_kernel() == 0) return run_mma<__nv_bfloat16>(a, d->head_dim, ws, s);
+  if (attn_kernel() == 0)
+    return d->dtype == DSM_DT_BF16 ? run_mma<__nv_bfloat16>(a, d->head_dim, ws, s) : run_mma<float>(a, d->head_dim, ws, s);
   if (d->dtype == DSM_DT_BF16) {
     switch (d->head_dim) {
       case 64: return launch_core<__nv_bfloat16, 64>(a, s);

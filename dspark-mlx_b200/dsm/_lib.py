@@ -177,7 +177,7 @@ def _declare(lib):
         "dsm_paged_trim": (I, [V, V, I, I, V, I64, I, V, V, I, V]),
         "dsm_kv8_append": (I, [V, V, I, I64, I, I, I64, I64, I64, I64, V, I, I, V, V, V, V, V]),
         "dsm_gqa_attn_kv8_workspace_bytes": (S, [I, I, I, I, I]),
-        "dsm_gqa_attn_kv8": (I, [POINTER(KV8AttnDesc), V, V, V, V, V, V, V, S, V]),
+        "dsm_gqa_attn_kv8": (I, [V, V, V, V, V, V, V, V, S, V]),
         "dsm_stage_rows_hilo": (I, [V, I64, I, V, I64, V, V]),
         "dsm_moe_workspace_bytes": (S, [POINTER(MoEDesc)]),
         "dsm_moe_forward": (I, [POINTER(MoEDesc), V, I, V, I, I64, V, V, V, V, S, V]),

@@ -19,17 +19,18 @@ it) sets the device error word: ``dsm._lib.raise_device_error()`` reads it.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
-from ._lib import KV8AttnDesc, check, dtype_code, lib
+from ._lib import DT_BF16, DT_F32, check, lib
 
 HEAD_DIMS = (64, 128, 256)
 GROUP = 64  # tokens per value group: page sizes are multiples of it
 MAX_PAGE = 1024
 MAX_BATCH = 8192
+_ROW_DTYPES = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 
 
 class KV8Layer(NamedTuple):
@@ -53,56 +54,76 @@ class PagedRows(NamedTuple):
     positions: torch.Tensor
 
 
-def _need(cond: bool, msg: str) -> None:
-    if not cond:
-        raise ValueError(msg)
+# The calls below sit in the loop of a decode step, next to kernels of a few microseconds: their checks
+# are plain comparisons, and messages are put together only when one fails.
+_DESC = struct.Struct("@10q4Q9if")  # dsm_kv8_attn_desc
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _tensor(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device=None) -> None:
-    """``shape`` entries that are None are free; the tensor must be contiguous and on the GPU."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(t.dim() == len(shape) and all(w is None or w == h for w, h in zip(shape, t.shape)),
-          f"{name} must be {['any' if w is None else w for w in shape]}, got {list(t.shape)}")
-    _need(t.is_contiguous(), f"{name} must be contiguous")
-    _need(device is None or t.device == device, f"{name} is on {t.device}, the rest on {device}")
+def _tensor(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: int = -1) -> int:
+    """``t`` is a contiguous CUDA tensor of that dtype and shape (on device ``dev``); its device."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    at = t.get_device()
+    if dev >= 0 and at != dev:
+        raise ValueError(f"{name} is on cuda:{at}, the rest on cuda:{dev}")
+    return at
 
 
 def _page_size(page_size: int) -> int:
-    _need(isinstance(page_size, int) and 0 < page_size <= MAX_PAGE and page_size % GROUP == 0,
-          f"page_size must be a multiple of {GROUP}, at most {MAX_PAGE}, got {page_size}")
+    if not (isinstance(page_size, int) and 0 < page_size <= MAX_PAGE and page_size % GROUP == 0):
+        raise ValueError(f"page_size must be a multiple of {GROUP}, at most {MAX_PAGE}, got {page_size}")
     return page_size
 
 
-def _table(block_table: torch.Tensor, batch: int, device) -> None:
-    _need(isinstance(block_table, torch.Tensor) and block_table.is_cuda and block_table.device == device,
-          f"block_table must be a CUDA tensor on {device}")
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-          and block_table.shape[1] > 0, f"block_table must be int32 [{batch}, pages]")
-    _need(block_table.stride(1) == 1 and (batch < 2 or block_table.stride(0) >= block_table.shape[1]),
-          "block_table rows must be contiguous and must not overlap")
+def _table(table: torch.Tensor, batch: int, dev: int):
+    """The row stride and columns of a block table."""
+    if not (isinstance(table, torch.Tensor) and table.is_cuda and table.get_device() == dev
+            and table.dtype is torch.int32 and table.dim() == 2):
+        raise ValueError(f"block_table must be an int32 [{batch}, pages] tensor on cuda:{dev}")
+    rows, cols = table.shape
+    stride, inner = table.stride()
+    if rows != batch or cols < 1 or (inner != 1 and cols > 1) or (batch > 1 and stride < cols):
+        raise ValueError(f"block_table must be [{batch}, pages] with contiguous rows that do not overlap, got "
+                         f"{tuple(table.shape)} with strides {table.stride()}")
+    return max(stride, cols), cols
 
 
-def _table_stride(block_table: torch.Tensor) -> int:
-    return max(block_table.stride(0), block_table.shape[1])
+def _lengths(lengths: torch.Tensor):
+    if not (isinstance(lengths, torch.Tensor) and lengths.dim() == 1 and lengths.shape[0] <= MAX_BATCH):
+        raise ValueError(f"lengths must be int32 [batch], batch at most {MAX_BATCH}")
+    return lengths.shape[0], _tensor(lengths, "lengths", torch.int32, lengths.shape)
 
 
 def _layer(layer: KV8Layer):
     k, v, ks, vs = layer
-    _need(isinstance(k, torch.Tensor) and k.dim() == 4, "k_codes must be [n_pages, n_kv, page_size, head_dim]")
+    if not (isinstance(k, torch.Tensor) and k.dim() == 4):
+        raise ValueError("k_codes must be [n_pages, n_kv, page_size, head_dim]")
     n_pages, n_kv, page, hd = k.shape
     _page_size(page)
-    _need(hd in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {hd}")
-    _need(n_pages > 0 and n_kv > 0, "an empty cache")
-    _tensor(k, "k_codes", torch.uint8, (n_pages, n_kv, page, hd))
-    _tensor(v, "v_codes", torch.uint8, (n_pages, n_kv, page // GROUP, hd, GROUP), k.device)
-    _tensor(ks, "k_scale", torch.float32, (n_pages, n_kv), k.device)
-    _tensor(vs, "v_scale", torch.float32, (n_pages, n_kv), k.device)
-    return n_pages, n_kv, page, hd
+    if hd not in HEAD_DIMS or n_pages < 1 or n_kv < 1:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS} and the cache not empty, got {tuple(k.shape)}")
+    dev = _tensor(k, "k_codes", torch.uint8, k.shape)
+    _tensor(v, "v_codes", torch.uint8, (n_pages, n_kv, page // GROUP, hd, GROUP), dev)
+    _tensor(ks, "k_scale", torch.float32, (n_pages, n_kv), dev)
+    _tensor(vs, "v_scale", torch.float32, (n_pages, n_kv), dev)
+    return n_pages, n_kv, page, hd, dev
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _on_device(fn):
+    """Runs ``fn(dev, ...)`` with ``dev`` the current device (the library launches there)."""
+
+    def run(dev: int, *args):
+        if _current_device() == dev:
+            return fn(dev, *args)
+        with torch.cuda.device(dev):
+            return fn(dev, *args)
+
+    return run
 
 
 def paged_extend(lengths: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -111,68 +132,77 @@ def paged_extend(lengths: torch.Tensor, new_len: torch.Tensor, block_table: torc
     into ``block_table``, ``lengths`` and ``n_free`` are updated in place. Returns the step's rows;
     ``max_rows`` (known on the host) bounds them, rows behind the last sequence get slot -1. A
     sequence that finds no pages, table or rows keeps its length and sets the device error word."""
-    _need(isinstance(lengths, torch.Tensor) and lengths.dim() == 1, "lengths must be int32 [batch]")
-    b = lengths.shape[0]
-    _need(b <= MAX_BATCH, f"batch must be at most {MAX_BATCH}, got {b}")
-    _tensor(lengths, "lengths", torch.int32, (b,))
-    dev = lengths.device
+    b, dev = _lengths(lengths)
     _tensor(new_len, "new_len", torch.int32, (b,), dev)
-    _table(block_table, b, dev)
-    _tensor(free_pages, "free_pages", torch.int32, (None,), dev)
+    stride, cols = _table(block_table, b, dev)
+    _tensor(free_pages, "free_pages", torch.int32, (free_pages.numel(),), dev)
     _tensor(n_free, "n_free", torch.int32, (1,), dev)
     _page_size(page_size)
-    _need(0 <= max_rows <= 0x7FFFFFFF, f"max_rows out of range: {max_rows}")
-    with torch.cuda.device(dev):
-        rows = PagedRows(torch.empty(b + 1, dtype=torch.int32, device=dev),
-                         torch.empty(max_rows, dtype=torch.int64, device=dev),
-                         torch.empty(max_rows, dtype=torch.int32, device=dev))
-        check(lib().dsm_paged_extend(lengths.data_ptr(), new_len.data_ptr(), b, page_size, block_table.data_ptr(),
-                                     _table_stride(block_table), block_table.shape[1], free_pages.data_ptr(),
-                                     n_free.data_ptr(), free_pages.shape[0], rows.cu_rows.data_ptr(),
-                                     rows.slot_map.data_ptr(), rows.positions.data_ptr(), max_rows, _stream(dev)),
-              "dsm_paged_extend")
-    return rows
+    if not 0 <= max_rows <= 0x7FFFFFFF:
+        raise ValueError(f"max_rows out of range: {max_rows}")
+    return _extend(dev, lengths, new_len, block_table, free_pages, n_free, page_size, max_rows, b, stride, cols)
+
+
+@_on_device
+def _extend(dev, lengths, new_len, block_table, free_pages, n_free, page_size, max_rows, b, stride, cols) -> PagedRows:
+    at = lengths.device
+    cu_rows = torch.empty(b + 1, dtype=torch.int32, device=at)
+    slot_map = torch.empty(max_rows, dtype=torch.int64, device=at)
+    positions = torch.empty(max_rows, dtype=torch.int32, device=at)
+    rc = lib().dsm_paged_extend(lengths.data_ptr(), new_len.data_ptr(), b, page_size, block_table.data_ptr(), stride,
+                                cols, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0],
+                                cu_rows.data_ptr(), slot_map.data_ptr(), positions.data_ptr(), max_rows,
+                                _raw_stream(dev))
+    if rc:
+        check(rc, "dsm_paged_extend")
+    return PagedRows(cu_rows, slot_map, positions)
 
 
 def paged_trim(lengths: torch.Tensor, keep_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                n_free: torch.Tensor, page_size: int) -> None:
     """Every sequence shrinks to ``min(lengths[i], keep_len[i])`` tokens (0 releases it): its surplus
     pages go back on the stack, ``lengths`` and ``n_free`` are updated in place."""
-    _need(isinstance(lengths, torch.Tensor) and lengths.dim() == 1, "lengths must be int32 [batch]")
-    b = lengths.shape[0]
-    _need(b <= MAX_BATCH, f"batch must be at most {MAX_BATCH}, got {b}")
-    _tensor(lengths, "lengths", torch.int32, (b,))
-    dev = lengths.device
+    b, dev = _lengths(lengths)
     _tensor(keep_len, "keep_len", torch.int32, (b,), dev)
-    _table(block_table, b, dev)
-    _tensor(free_pages, "free_pages", torch.int32, (None,), dev)
+    stride, cols = _table(block_table, b, dev)
+    _tensor(free_pages, "free_pages", torch.int32, (free_pages.numel(),), dev)
     _tensor(n_free, "n_free", torch.int32, (1,), dev)
     _page_size(page_size)
-    with torch.cuda.device(dev):
-        check(lib().dsm_paged_trim(lengths.data_ptr(), keep_len.data_ptr(), b, page_size, block_table.data_ptr(),
-                                   _table_stride(block_table), block_table.shape[1], free_pages.data_ptr(),
-                                   n_free.data_ptr(), free_pages.shape[0], _stream(dev)), "dsm_paged_trim")
+    _trim(dev, lengths, keep_len, block_table, free_pages, n_free, page_size, b, stride, cols)
+
+
+@_on_device
+def _trim(dev, lengths, keep_len, block_table, free_pages, n_free, page_size, b, stride, cols) -> None:
+    rc = lib().dsm_paged_trim(lengths.data_ptr(), keep_len.data_ptr(), b, page_size, block_table.data_ptr(), stride,
+                              cols, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0], _raw_stream(dev))
+    if rc:
+        check(rc, "dsm_paged_trim")
 
 
 def kv8_append(layer: KV8Layer, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
     """Writes rows ``k``, ``v`` ``[rows, n_kv, head_dim]`` (bf16 or fp32, any row and head strides)
     into the cache slots ``slot_map`` int64 ``[rows]`` (-1: skipped). Rows of one page must be
     neighbours, as :func:`paged_extend` leaves them, each slot given once."""
-    n_pages, n_kv, page, hd = _layer(layer)
-    dev = layer.k_codes.device
-    _need(isinstance(k, torch.Tensor) and k.dim() == 3 and tuple(k.shape[1:]) == (n_kv, hd),
-          f"k must be [rows, {n_kv}, {hd}]")
-    _need(k.dtype in (torch.bfloat16, torch.float32), f"k dtype {k.dtype} unsupported (bf16 or fp32)")
-    _need(isinstance(v, torch.Tensor) and v.shape == k.shape and v.dtype == k.dtype,
-          "v must have the shape and dtype of k")
-    _need(k.device == dev and v.device == dev, f"k and v must be on {dev}")
-    _need(k.stride(2) == 1 and v.stride(2) == 1, f"rows of k and v must be {hd} contiguous values")
+    n_pages, n_kv, page, hd, dev = _layer(layer)
+    dt = _ROW_DTYPES.get(k.dtype)
+    if not (dt is not None and k.dim() == 3 and k.shape[1] == n_kv and k.shape[2] == hd and v.shape == k.shape
+            and v.dtype is k.dtype and k.get_device() == dev and v.get_device() == dev):
+        raise ValueError(f"k and v must be bf16 or fp32 [rows, {n_kv}, {hd}] tensors on cuda:{dev}, got {k.dtype} "
+                         f"{tuple(k.shape)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
+        raise ValueError(f"rows of k and v must be {hd} contiguous values")
     _tensor(slot_map, "slot_map", torch.int64, (k.shape[0],), dev)
-    with torch.cuda.device(dev):
-        check(lib().dsm_kv8_append(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), k.shape[0], n_kv, hd, k.stride(0),
-                                   k.stride(1), v.stride(0), v.stride(1), slot_map.data_ptr(), page, n_pages,
-                                   layer.k_codes.data_ptr(), layer.v_codes.data_ptr(), layer.k_scale.data_ptr(),
-                                   layer.v_scale.data_ptr(), _stream(dev)), "dsm_kv8_append")
+    _append(dev, layer, k, v, slot_map, dt, n_pages, n_kv, page, hd, ks, vs)
+
+
+@_on_device
+def _append(dev, layer, k, v, slot_map, dt, n_pages, n_kv, page, hd, ks, vs) -> None:
+    rc = lib().dsm_kv8_append(k.data_ptr(), v.data_ptr(), dt, k.shape[0], n_kv, hd, ks[0], ks[1], vs[0], vs[1],
+                              slot_map.data_ptr(), page, n_pages, layer[0].data_ptr(), layer[1].data_ptr(),
+                              layer[2].data_ptr(), layer[3].data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc, "dsm_kv8_append")
 
 
 def gqa_attention_kv8(q: torch.Tensor, layer: KV8Layer, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -182,42 +212,52 @@ def gqa_attention_kv8(q: torch.Tensor, layer: KV8Layer, block_table: torch.Tenso
     cached rows and then, unless ``blk_k`` is None, the block's own rows ``blk_k`` / ``blk_v``
     ``[batch, n_kv, block, head_dim]``, with no mask; ``scale`` defaults to ``head_dim ** -0.5``.
     Returns ``[batch, block, n_heads * head_dim]`` in q's dtype; a sequence without any row gives
-    zeros. Every tensor but the cache may have any strides with contiguous rows."""
-    n_pages, n_kv, page, hd = _layer(layer)
-    dev = layer.k_codes.device
-    _need(isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[3] == hd and q.shape[1] > 0
-          and q.shape[2] > 0 and q.shape[2] % n_kv == 0,
-          f"q must be [batch, block, a multiple of {n_kv} heads, {hd}]")
-    _need(q.dtype in (torch.bfloat16, torch.float32), f"q dtype {q.dtype} unsupported (bf16 or fp32)")
-    _need(q.device == dev, f"q must be on {dev}")
-    _need(q.stride(3) == 1, f"rows of q must be {hd} contiguous values")
+    zeros. q and the block's rows may have any strides with contiguous rows."""
+    n_pages, n_kv, page, hd, dev = _layer(layer)
+    dt = _ROW_DTYPES.get(q.dtype)
+    if not (dt is not None and q.dim() == 4 and q.shape[3] == hd and q.get_device() == dev):
+        raise ValueError(f"q must be a bf16 or fp32 [batch, block, heads, {hd}] tensor on cuda:{dev}, got {q.dtype} "
+                         f"{tuple(q.shape)} on {q.device}")
     b, s, nh, _ = q.shape
-    _need(b <= MAX_BATCH, f"batch must be at most {MAX_BATCH}, got {b}")
-    _need((blk_k is None) == (blk_v is None), "blk_k and blk_v must both be given or both be None")
-    for name, t in (("blk_k", blk_k), ("blk_v", blk_v)):
-        if t is not None:
-            _need(isinstance(t, torch.Tensor) and tuple(t.shape) == (b, n_kv, s, hd) and t.dtype == q.dtype
-                  and t.device == dev, f"{name} must be a {q.dtype} [{b}, {n_kv}, {s}, {hd}] tensor on {dev}")
-            _need(t.stride(3) == 1, f"rows of {name} must be {hd} contiguous values")
+    if s < 1 or nh < 1 or nh % n_kv or b > MAX_BATCH:
+        raise ValueError(f"q must be [batch <= {MAX_BATCH}, block, a multiple of {n_kv} heads, {hd}], got "
+                         f"{tuple(q.shape)}")
+    qs = q.stride()
+    if (blk_k is None) != (blk_v is None):
+        raise ValueError("blk_k and blk_v must both be given or both be None")
+    ks = vs = (0, 0, 0, 1)
+    if blk_k is not None:
+        want = (b, n_kv, s, hd)
+        if not (blk_k.shape == want and blk_v.shape == want and blk_k.dtype is q.dtype and blk_v.dtype is q.dtype
+                and blk_k.get_device() == dev and blk_v.get_device() == dev):
+            raise ValueError(f"blk_k and blk_v must be {q.dtype} {want} tensors on cuda:{dev}, got {blk_k.dtype} "
+                             f"{tuple(blk_k.shape)} on {blk_k.device} and {blk_v.dtype} {tuple(blk_v.shape)} on "
+                             f"{blk_v.device}")
+        ks, vs = blk_k.stride(), blk_v.stride()
+    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"rows of q, blk_k and blk_v must be {hd} contiguous values")
     _tensor(lengths, "lengths", torch.int32, (b,), dev)
-    _table(block_table, b, dev)
+    stride, cols = _table(block_table, b, dev)
+    desc = _DESC.pack(*qs[:3], *ks[:3], *vs[:3], stride, layer[0].data_ptr(), layer[1].data_ptr(), layer[2].data_ptr(),
+                      layer[3].data_ptr(), dt, b, s, nh, n_kv, hd, page, n_pages, cols,
+                      hd ** -0.5 if scale is None else scale)
+    return _attend(dev, desc, q, block_table, lengths, blk_k, blk_v, b, s, nh, n_kv, hd)
+
+
+@_on_device
+def _attend(dev, desc, q, block_table, lengths, blk_k, blk_v, b, s, nh, n_kv, hd) -> torch.Tensor:
     L = lib()
-    with torch.cuda.device(dev):
-        out = torch.empty(b, s, nh * hd, dtype=q.dtype, device=dev)
-        if b == 0:
-            return out
-        ws_bytes = L.dsm_gqa_attn_kv8_workspace_bytes(b, s, nh, n_kv, hd)
-        ws = torch.empty(max(1, ws_bytes), dtype=torch.uint8, device=dev)
-        bk = (blk_k.stride(0), blk_k.stride(1), blk_k.stride(2)) if blk_k is not None else (0, 0, 0)
-        bv = (blk_v.stride(0), blk_v.stride(1), blk_v.stride(2)) if blk_v is not None else (0, 0, 0)
-        d = KV8AttnDesc(q.stride(0), q.stride(1), q.stride(2), *bk, *bv, _table_stride(block_table),
-                        layer.k_codes.data_ptr(), layer.v_codes.data_ptr(), layer.k_scale.data_ptr(),
-                        layer.v_scale.data_ptr(), dtype_code(q.dtype), b, s, nh, n_kv, hd, page, n_pages,
-                        block_table.shape[1], float(hd ** -0.5 if scale is None else scale))
-        check(L.dsm_gqa_attn_kv8(ctypes.byref(d), q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-                                 None if blk_k is None else blk_k.data_ptr(),
-                                 None if blk_v is None else blk_v.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes,
-                                 _stream(dev)), "dsm_gqa_attn_kv8")
+    at = q.device
+    out = torch.empty(b, s, nh * hd, dtype=q.dtype, device=at)
+    if b == 0:
+        return out
+    ws_bytes = L.dsm_gqa_attn_kv8_workspace_bytes(b, s, nh, n_kv, hd)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=at)
+    rc = L.dsm_gqa_attn_kv8(desc, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+                            None if blk_k is None else blk_k.data_ptr(), None if blk_v is None else blk_v.data_ptr(),
+                            out.data_ptr(), ws.data_ptr(), ws_bytes, _raw_stream(dev))
+    if rc:
+        check(rc, "dsm_gqa_attn_kv8")
     return out
 
 
@@ -231,9 +271,10 @@ class PagedKVCache:
 
     def __init__(self, n_layers: int, n_pages: int, n_kv: int, head_dim: int, batch: int, max_pages: int, *,
                  page_size: int = 64, device="cuda"):
-        _need(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-        _need(min(n_layers, n_pages, n_kv, batch, max_pages) > 0, "sizes must be positive")
-        _need(batch <= MAX_BATCH, f"batch must be at most {MAX_BATCH}, got {batch}")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        if min(n_layers, n_pages, n_kv, batch, max_pages) < 1 or batch > MAX_BATCH:
+            raise ValueError(f"sizes must be positive and batch at most {MAX_BATCH}")
         self.page_size = _page_size(page_size)
         self.n_kv, self.head_dim, self.n_pages = n_kv, head_dim, n_pages
         u8 = dict(dtype=torch.uint8, device=device)

@@ -128,6 +128,9 @@ def test_desc_layout_matches_the_header():
     body = text[text.index("typedef struct dsm_kv8_attn_desc"):text.index("} dsm_kv8_attn_desc;")]
     c_fields = re.findall(r"\*?\s*([a-z_0-9]+)\s*[,;]", body)
     assert c_fields == [f for f, _ in _lib.KV8AttnDesc._fields_]
+    # what the calls pack is the same struct, byte for byte
+    values = list(range(1, 11)) + [1 << 40, 1 << 41, 1 << 42, 1 << 43] + list(range(20, 29)) + [0.25]
+    assert pc._DESC.pack(*values) == bytes(_lib.KV8AttnDesc(*values))
 
 
 def test_python_functions_refuse_cpu_tensors_and_bad_settings():
