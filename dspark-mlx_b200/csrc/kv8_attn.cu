@@ -293,7 +293,7 @@ __device__ __forceinline__ void f16_terms(float x0, float x1, uint32_t (&t)[TERM
   }
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
@@ -346,6 +346,10 @@ __device__ __forceinline__ void load_vals(const T* p, bool vec, float (&x)[V]) {
   }
 }
 
+// 16 of the block's own rows as B fragments of f16 terms, and their exponents, in words
+__host__ __device__ constexpr int mma_block_words(int hd, int terms) {
+  return 2 * (hd / 16) * terms * 64 + hd / 8 * terms * 64 + 32;
+}
 // shared memory of the kernel, in bytes from its start
 struct MmaSmem {
   int buf, qf, rowf, ml, scales, full, empty, sums, P, bytes;
@@ -354,7 +358,9 @@ __host__ __device__ inline MmaSmem mma_smem(int hd, int mt, int mg, int terms, i
   MmaSmem s;
   const int warps = mma_warps(hd), rows = 16 * mt * mg, tl = warps / mg, stages = depth * tl;
   s.buf = stages * 2 * kTile * hd;
-  s.qf = s.buf + tl / 2 * rows * hd * 4;  // the lanes that hand their sums over in the first round
+  // the lanes that hand their sums over in the first round; before that, 16 rows of the block per lane
+  const int sums = tl / 2 * rows * hd * 4, block = mma_block_words(hd, terms) * 4;
+  s.qf = s.buf + (sums > block ? sums : block);
   s.rowf = s.qf + rows * hd * 2 * terms;
   s.ml = s.rowf + rows * 4;
   s.scales = s.ml + warps * 16 * mt * 16;
@@ -376,6 +382,8 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   constexpr int CH = HD / 64;  // 16-byte chunks of a key row per thread
   constexpr int kKeyBytes = kTile * HD;
   constexpr int kWarpRows = 16 * MT;
+  constexpr int TPR = kThreads / 16, VB = HD / TPR;  // staging: 16 rows at a time, threads per row, values per thread
+  constexpr int kBlockWords = mma_block_words(HD, TERMS);
   extern __shared__ __align__(128) uint8_t smem[];
   const MmaSmem L = mma_smem(HD, MT, pl.mg, TERMS, pl.depth, p.batch);
   float* buf = reinterpret_cast<float*>(smem + L.buf);
@@ -393,6 +401,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   const int my_mg = warp / tl, my_tl = warp % tl;
   const int hr = p.n_kv * pl.row_blocks;
   const int cta_rows = kWarpRows * mg;
+  const int row_r = tid / TPR, row_d = tid % TPR * VB;  // this thread's row (of 16) and first column in staging
 
   if (tid < S) {
     mbar_init(full + 2 * tid, 2);  // the copy's expect_tx, and the scale's cp.async
@@ -470,49 +479,103 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     const int len = seq_len(p, un.b);
     const int group = p.n_heads / p.n_kv;
 
-    // q: a warp per row, in f16 terms in the A-fragment order of the products
+    // the power of two of a row whose VB values lie in each of its threads
+    auto row_exp = [&](const float(&x)[VB]) -> int {
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < VB; ++i) mx = fmaxf(mx, finite_abs(x[i]));
+#pragma unroll
+      for (int w = TPR / 2; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      return kv8_scale_exp(mx);
+    };
+    // thread column c multiplies chunks 2 c and 2 c + 1 of each 128 columns (chunk c of 64), four columns
+    // per k16 step: its first two are k = 2 c, 2 c + 1 (reg 0), the others k + 8 (reg 1)
+    auto k_place = [&](int d, int& c, int& ks, int& reg) {
+      const int chunk = d >> 4, w = (d & 15) >> 2;
+      c = HD == 64 ? chunk : (chunk & 7) >> 1;
+      ks = HD == 64 ? w : (chunk >> 3) * 8 + (chunk & 1) * 4 + w;
+      reg = (d & 3) >> 1;
+    };
+    // 16 rows of the block from row kb, as B fragments in the join buffer. Key r of them is column
+    // 2 * (r / 4) + r % 2 of key tile (r / 2) % 2, so that a thread's four keys are 4 c .. 4 c + 3.
+    auto load_block = [&](int kb, float(&x)[VB], float(&y)[VB]) {
+      if (kb + row_r < p.block) {
+        load_vals<T, VB>(static_cast<const T*>(p.blk_k) + un.b * p.bk_batch + g * p.bk_head +
+                             (kb + row_r) * p.bk_row + row_d, pl.vec_blk, x);
+        load_vals<T, VB>(static_cast<const T*>(p.blk_v) + un.b * p.bv_batch + g * p.bv_head +
+                             (kb + row_r) * p.bv_row + row_d, pl.vec_blk, y);
+      }
+    };
+    auto put_block = [&](int slot, float(&x)[VB], float(&y)[VB]) {
+      uint32_t* kf = reinterpret_cast<uint32_t*>(buf) + slot * kBlockWords;
+      uint32_t* vf = kf + 2 * KS * TERMS * 64;
+      const int ek = row_exp(x), ev = row_exp(y);
+      const float ik = kv8_exp2i(-ek), iv = kv8_exp2i(-ev);
+      if (row_d == 0) {
+        float* e = reinterpret_cast<float*>(vf + NT * TERMS * 64);
+        e[row_r] = kv8_exp2i(ek);
+        e[16 + row_r] = float(ev);
+      }
+      const int gk = 2 * (row_r >> 2) + (row_r & 1), jk = (row_r >> 1) & 1;
+#pragma unroll
+      for (int i = 0; i < VB; i += 2) {
+        const int d = row_d + i;
+        int c, ks, reg;
+        k_place(d, c, ks, reg);
+        uint32_t f[TERMS];
+        f16_terms<TERMS>(scaled(x[i], ik), scaled(x[i + 1], ik), f);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) kf[((jk * KS + ks) * TERMS + t) * 64 + (gk * 4 + c) * 2 + reg] = f[t];
+        f16_terms<TERMS>(scaled(y[i], iv), scaled(y[i + 1], iv), f);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          uint16_t* v16 = reinterpret_cast<uint16_t*>(
+              vf + ((d >> 3) * TERMS + t) * 64 + ((d & 7) * 4 + (row_r >> 2)) * 2 + ((row_r >> 1) & 1)) + (row_r & 1);
+          v16[0] = uint16_t(f[t]);
+          v16[16] = uint16_t(f[t] >> 16);  // the next column's thread, four on
+        }
+      }
+    };
+
+    // q and the block's own rows, TPR threads to a row: scaled per row by a power of two to at most 448, in
+    // f16 terms, in the fragment order of the products
     __syncthreads();  // the previous unit's fragments and sums are used up
-    for (int r = warp; r < cta_rows; r += kWarps) {
-      constexpr int QV = HD == 256 ? 8 : 4;  // values per thread
-      const bool mine = lane * QV < HD;
-      float x[QV];
-      int e = kKv8MinExp;
-#pragma unroll
-      for (int i = 0; i < QV; ++i) x[i] = 0.f;
-      if (r < n_rows) {
+    {
+      const T* qg = static_cast<const T*>(p.q) + un.b * p.q_batch;
+      auto load_q = [&](int r, float(&x)[VB]) {
         const int rr = r0 + r;
-        if (mine)
-          load_vals<T, QV>(static_cast<const T*>(p.q) + un.b * p.q_batch + (rr % p.block) * p.q_row +
-                               (g * group + rr / p.block) * p.q_head + lane * QV,
-                           pl.vec_q, x);
-        float mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < QV; ++i) mx = fmaxf(mx, finite_abs(x[i]));
-        e = kv8_scale_exp(kv8_warp_max(mx));
+        if (r < n_rows)
+          load_vals<T, VB>(qg + (rr % p.block) * p.q_row + (g * group + rr / p.block) * p.q_head + row_d, pl.vec_q, x);
+      };
+      auto put_q = [&](int r, float(&x)[VB]) {
+        const int e = row_exp(x);
         // the sign of the factor goes into q: the row maximum is taken before the factor
         const float inv = p.scale < 0.f ? -kv8_exp2i(-e) : kv8_exp2i(-e);
+        if (row_d == 0) rowf[r] = r < n_rows ? fabsf(p.scale) * kLog2e * kv8_exp2i(e) : 0.f;
 #pragma unroll
-        for (int i = 0; i < QV; ++i) x[i] = scaled(x[i], inv);
-      }
-      if (lane == 0) rowf[r] = r < n_rows ? fabsf(p.scale) * kLog2e * kv8_exp2i(e) : 0.f;
-      if (mine) {
+        for (int i = 0; i < VB; i += 2) {
+          int c, ks, reg;
+          k_place(row_d + i, c, ks, reg);
+          uint32_t f[TERMS];
+          f16_terms<TERMS>(scaled(x[i], inv), scaled(x[i + 1], inv), f);
 #pragma unroll
-        for (int i = 0; i < QV; i += 4) {
-          // thread column c multiplies chunks 2 c and 2 c + 1 of each 128 columns (chunk c of 64), four
-          // columns per k16 step: its first two are k = 2 c, 2 c + 1, the others k + 8
-          const int d = lane * QV + i, chunk = d >> 4, w = (d & 15) >> 2;
-          const int c = HD == 64 ? chunk : (chunk & 7) >> 1;
-          const int ks = HD == 64 ? w : (chunk >> 3) * 8 + (chunk & 1) * 4 + w;
-          uint32_t lo2[TERMS], hi2[TERMS];
-          f16_terms<TERMS>(x[i], x[i + 1], lo2);
-          f16_terms<TERMS>(x[i + 2], x[i + 3], hi2);
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t) {
-            uint32_t* q4 = qf + ((((r >> 4) * KS + ks) * TERMS + t) * 32 + (r & 7) * 4 + c) * 4 + ((r >> 3) & 1);
-            q4[0] = lo2[t];
-            q4[2] = hi2[t];
-          }
+          for (int t = 0; t < TERMS; ++t)
+            qf[((((r >> 4) * KS + ks) * TERMS + t) * 32 + (r & 7) * 4 + c) * 4 + 2 * reg + ((r >> 3) & 1)] = f[t];
         }
+      };
+      float x[2][VB] = {}, y[2][VB] = {};
+      if (last && p.blk_k) load_block(0, x[0], x[1]);
+      load_q(row_r, y[0]);
+      if (MT * mg > 1) load_q(row_r + 16, y[1]);
+      if (last && p.blk_k) put_block(0, x[0], x[1]);
+      put_q(row_r, y[0]);
+      if (MT * mg > 1) put_q(row_r + 16, y[1]);
+      for (int r = row_r + 32; r < cta_rows; r += 32) {
+        float z[2][VB] = {};
+        load_q(r, z[0]);
+        load_q(r + 16, z[1]);
+        put_q(r, z[0]);
+        put_q(r + 16, z[1]);
       }
     }
     __syncthreads();
@@ -619,86 +682,81 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         }
     };
 
-    // ---- the block's own rows: 16 keys at a time, by the lanes behind the unit's last tile
+    // ---- the block's own rows, 16 at a time: the first by the lane behind the unit's last tile, while the
+    // others begin with the cached rows
     if (last && p.blk_k) {
-      const T* bk = static_cast<const T*>(p.blk_k) + un.b * p.bk_batch + g * p.bk_head;
-      const T* bv = static_cast<const T*>(p.blk_v) + un.b * p.bv_batch + g * p.bv_head;
-      for (int kb = ((my_tl - a1 % tl + tl) % tl) * 16; kb < p.block; kb += 16 * tl) {
-        // one power of two for the 16 keys' rows and one for the values', as a page would have
-        float mk = 0.f, mv = 0.f;
-        for (int r = kb + (lane >> 4); r < min(kb + 16, p.block); r += 2)
-#pragma unroll
-          for (int d = (lane & 15) * 4; d < HD; d += 64) {
-            float x[4], y[4];
-            load_vals<T, 4>(bk + r * p.bk_row + d, pl.vec_blk, x);
-            load_vals<T, 4>(bv + r * p.bv_row + d, pl.vec_blk, y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              mk = fmaxf(mk, finite_abs(x[i]));
-              mv = fmaxf(mv, finite_abs(y[i]));
-            }
-          }
-        const int ek = kv8_scale_exp(kv8_warp_max(mk)), ev = kv8_scale_exp(kv8_warp_max(mv));
-        const float ik = kv8_exp2i(-ek), iv = kv8_exp2i(-ev);
-        // column n of key tile j is key kb + 4 * (n / 2) + 2 j + n % 2
+      auto block_tile = [&](int kb) {
+        const uint2* kf = reinterpret_cast<const uint2*>(buf) + lane;
+        const uint2* vf = kf + 2 * KS * TERMS * 32;
+        const float* ex = reinterpret_cast<const float*>(reinterpret_cast<uint32_t*>(buf) + kBlockWords - 32);
         float s[MT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) zero(s[mt]);
+#pragma unroll 4
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int tq = 0; tq < TERMS; ++tq) {
+            uint4 q[MT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+            for (int mt = 0; mt < MT; ++mt) q[mt] = my_q[((mt * KS + ks) * TERMS + tq) * 32];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = kb + 4 * (gq >> 1) + 2 * j + (gq & 1);
+            for (int tk = 0; tk < TERMS; ++tk)
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const int d = HD == 64 ? cq * 16 + ks * 4 : (ks >> 3) * 128 + (2 * cq + ((ks >> 2) & 1)) * 16 + (ks & 3) * 4;
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (key < p.block) load_vals<T, 4>(bk + key * p.bk_row + d, pl.vec_blk, x);
-            uint32_t b0[TERMS], b1[TERMS];
-            f16_terms<TERMS>(scaled(x[0], ik), scaled(x[1], ik), b0);
-            f16_terms<TERMS>(scaled(x[2], ik), scaled(x[3], ik), b1);
+              for (int j = 0; j < 2; ++j) {
+                const uint2 k = kf[((j * KS + ks) * TERMS + tk) * 32];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int tq = 0; tq < TERMS; ++tq) {
-                const uint4 q = my_q[((mt * KS + ks) * TERMS + tq) * 32];
-#pragma unroll
-                for (int tk = 0; tk < TERMS; ++tk) mma(s[mt][j], q, b0[tk], b1[tk]);
+                for (int mt = 0; mt < MT; ++mt) mma(s[mt][j], q[mt], k.x, k.y);
               }
           }
-        }
-        weigh(std::integral_constant<int, 2>(), s, kv8_exp2i(ek), ev, kb + 16 > p.block,
-                                     [&](int j, int e) { return kb + 4 * cq + 2 * j + e >= p.block; });
+        float ev = -200.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ev = kb + r < p.block ? fmaxf(ev, ex[16 + r]) : ev;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = ex[4 * cq + 2 * j + e];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              s[mt][j][e] *= f;
+              s[mt][j][2 + e] *= f;
+            }
+          }
+        weigh(std::integral_constant<int, 2>(), s, 1.f, int(ev), kb + 16 > p.block,
+              [&](int j, int e) { return kb + 4 * cq + 2 * j + e >= p.block; });
         uint4 pf[MT][TERMS];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t f[4][TERMS];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f16_terms<TERMS>(s[mt][i >> 1][2 * (i & 1)], s[mt][i >> 1][2 * (i & 1) + 1], f[i]);
+          for (int i = 0; i < 4; ++i) {
+            const int j = i >> 1;
+            const float f0 = ex2(ex[16 + 4 * cq + 2 * j] - ev), f1 = ex2(ex[16 + 4 * cq + 2 * j + 1] - ev);
+            f16_terms<TERMS>(s[mt][j][2 * (i & 1)] * f0, s[mt][j][2 * (i & 1) + 1] * f1, f[i]);
+          }
 #pragma unroll
           for (int t = 0; t < TERMS; ++t) pf[mt][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float x[4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = kb + 4 * cq + i;
-            x[i] = key < p.block ? scaled(ld_f(bv, key * p.bv_row + 8 * n + gq), iv) : 0.f;
+          for (int tv = 0; tv < TERMS; ++tv) {
+            const uint2 v = vf[(n * TERMS + tv) * 32];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int tp = 0; tp < TERMS; ++tp) mma(o[mt][n], pf[mt][tp], v.x, v.y);
           }
-          uint32_t b0[TERMS], b1[TERMS];
-          f16_terms<TERMS>(x[0], x[1], b0);
-          f16_terms<TERMS>(x[2], x[3], b1);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int tp = 0; tp < TERMS; ++tp)
-#pragma unroll
-              for (int tv = 0; tv < TERMS; ++tv) mma(o[mt][n], pf[mt][tp], b0[tv], b1[tv]);
-          }
+      };
+      for (int kb = 0; kb < p.block; kb += 16) {
+        if (kb > 0) {
+          __syncthreads();
+          float x[2][VB] = {};
+          load_block(kb, x[0], x[1]);
+          put_block(0, x[0], x[1]);
+          __syncthreads();
         }
+        if (my_tl == (a1 + kb / 16) % tl) block_tile(kb);
       }
     }
 
@@ -711,7 +769,8 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       const float k_scale = scales[st].x;
       const int nv = min(kTile, len - (un.t + i - a0) * kTile);
       const bool any = ok && nv > 0 && k_scale == k_scale;
-      const uint32_t kb = smem_u32(smem + st * 2 * kKeyBytes), vb = kb + kKeyBytes;
+      const uint8_t* kt = smem + st * 2 * kKeyBytes;
+      const uint8_t* vt = kt + kKeyBytes;
       if (any) {
         float s[MT][8][4];
 #pragma unroll
@@ -722,39 +781,42 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
             for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
         // scores: column n of key tile j is key 16 * (n / 2) + 2 j + n % 2, so that a thread ends up with
         // the 16 keys whose codes of one value column lie together
-        const uint32_t krow = kb + (16 * (gq >> 1) + (gq & 1)) * HD;
-#pragma unroll
+        const uint8_t* krow = kt + (16 * (gq >> 1) + (gq & 1)) * HD;
+        // four key tiles at a time: their products are independent, a chain's steps are 4 MT products apart
+#pragma unroll 1
         for (int ch = 0; ch < CH; ++ch) {
+          const uint32_t chunk = HD == 64 ? cq : 2 * cq + (ch & 1);
 #pragma unroll
-          for (int tq = 0; tq < TERMS; ++tq) {
-            uint4 q[MT][4];
+          for (int j4 = 0; j4 < 8; j4 += 4) {
+            uint4 k[4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int j = 0; j < 4; ++j) {
+              const int t = 2 * (j4 + j);  // its token is 16 * (gq / 2) + t + gq % 2
+              const uint32_t at = HD == 64 ? chunk : (chunk ^ ((t & 7) | (gq & 1))) + (ch >> 1) * 8;
+              k[j] = *reinterpret_cast<const uint4*>(krow + t * HD + at * 16);
+            }
 #pragma unroll
-              for (int w = 0; w < 4; ++w) q[mt][w] = my_q[((mt * KS + ch * 4 + w) * TERMS + tq) * 32];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint32_t addr = krow + 2 * j * HD;
-              if constexpr (HD == 64)
-                addr += cq * 16;
-              else
-                addr += ((ch >> 1) * 8 + ((2 * cq + (ch & 1)) ^ (((2 * j) & 7) | (gq & 1)))) * 16;
-              const uint4 k = lds128(addr);
-              const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
-              float t[MT][4];
-              if constexpr (TERMS == 2) zero(t);
+            for (int tq = 0; tq < TERMS; ++tq) {
+              float t4[4][4];
+              if constexpr (TERMS == 2) zero(t4);
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
-                uint32_t b0, b1;
-                e4m3x4_to_f16(kw[w], b0, b1);
+                uint4 q[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) mma(TERMS == 2 ? t[mt] : s[mt][j], q[mt][w], b0, b1);
+                for (int mt = 0; mt < MT; ++mt) q[mt] = my_q[((mt * KS + ch * 4 + w) * TERMS + tq) * 32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t b0, b1;
+                  e4m3x4_to_f16(w == 0 ? k[j].x : w == 1 ? k[j].y : w == 2 ? k[j].z : k[j].w, b0, b1);
+#pragma unroll
+                  for (int mt = 0; mt < MT; ++mt) mma(TERMS == 2 ? t4[j] : s[mt][j4 + j], q[mt], b0, b1);
+                }
               }
-              if constexpr (TERMS == 2) {
+              if constexpr (TERMS == 2) {  // MT is 1
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) s[mt][j][e] += t[mt][e];
+                  for (int e = 0; e < 4; ++e) s[0][j4 + j][e] += t4[j][e];
               }
             }
           }
@@ -780,34 +842,45 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
           }
         // values: columns 8 n + gq, this thread's 16 keys. Codes behind the length are cleared: a weight of
         // zero would not take a NaN there out
-        const uint32_t vrow = vb + gq * kTile + cq * 16;
+        const uint8_t* vrow = vt + gq * kTile + cq * 16;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4 v = lds128(vrow + n * 8 * kTile);
-          uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+        for (int n4 = 0; n4 < NT; n4 += 4) {
+          uint4 v[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v[n] = *reinterpret_cast<const uint4*>(vrow + (n4 + n) * 8 * kTile);
           if (nv < kTile) {
+            uint32_t keep[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const int k = nv - (16 * cq + 4 * w);
-              vw[w] &= k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+              keep[w] = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              v[n].x &= keep[0];
+              v[n].y &= keep[1];
+              v[n].z &= keep[2];
+              v[n].w &= keep[3];
             }
           }
-          float t4[MT][4];
+          float t4[4][4];
           if constexpr (TERMS == 2) zero(t4);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t b0, b1;
-            e4m3x4_to_f16(vw[w], b0, b1);
+          for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < 4; ++n) {
+              uint32_t b0, b1;
+              e4m3x4_to_f16(w == 0 ? v[n].x : w == 1 ? v[n].y : w == 2 ? v[n].z : v[n].w, b0, b1);
 #pragma unroll
-              for (int t = 0; t < TERMS; ++t) mma(TERMS == 2 ? t4[mt] : o[mt][n], pf[mt][w][t], b0, b1);
-          }
+              for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) mma(TERMS == 2 ? t4[n] : o[mt][n4 + n], pf[mt][w][t], b0, b1);
+            }
           if constexpr (TERMS == 2) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[mt][n][e] += t4[mt][e];
+              for (int e = 0; e < 4; ++e) o[0][n4 + n][e] += t4[n][e];
           }
         }
       } else if (ok) {  // nothing to read; its values' half may still be on its way
