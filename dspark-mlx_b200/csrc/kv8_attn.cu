@@ -8,27 +8,10 @@
 // dsm_set_attn_kernel picks between them (per host thread).
 #include <algorithm>
 
-#include "kv8.cuh"
+#include "kv8_attn.cuh"
 
 namespace dsm {
 namespace {
-
-struct AttnArgs {
-  const void* q;
-  int64_t q_batch, q_row, q_head;  // strides in elements
-  const uint8_t *k_codes, *v_codes;
-  const float *k_scale, *v_scale;
-  int page, n_pages;
-  const int32_t* table;
-  int64_t table_stride;
-  int max_pages;
-  const int32_t* lengths;
-  const void *blk_k, *blk_v;  // NULL: the cached rows alone
-  int64_t bk_batch, bk_head, bk_row, bv_batch, bv_head, bv_row;
-  int batch, block, n_heads, n_kv;
-  float scale;
-  void* out;
-};
 
 // The CUDA-core kernel: one warp per query row, 32 keys at a time with an online softmax, all in
 // fp32. Lanes take a key each for the scores, then head_dim / 32 columns each for the sum. Runs
@@ -183,101 +166,20 @@ int launch_core(const AttnArgs& a, cudaStream_t s) {
 // into stages that belong to the lane: it refills the keys' half as soon as the scores are taken, the
 // values' half after the sums, and waits for no other lane in the main loop. The block's own rows are
 // 16-key tiles of whichever CTA holds the unit's last tile, read straight from the caller's tensors.
-constexpr int kTile = kKv8Group;
 constexpr int kMaxDepth = 2;  // stages per lane, where they fit
 constexpr int kUnitCost = 6;  // a unit's q, join and output, in tiles
 // warps per CTA: a stage of head_dim 256 holds 32 KB, so four lanes fill shared memory
 constexpr int mma_warps(int hd) { return hd == 256 ? 4 : 8; }
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScale = 6.f;  // weights at the reference enter f16 as 2^6,
 constexpr float kPGrow = 8.f;   // and grow to 2^14 before the reference follows
-constexpr float kLowest = -3.402823466e38f;
 
 struct MmaPlan {
-  int mg;          // warps that share a tile, each with its own query rows
-  int row_blocks;  // CTAs' row blocks per KV head
-  int rows;        // query rows of a KV head: group * block
-  int depth;       // stages per lane
-  int snap;        // a cut within this many tiles of a unit's edge moves there
-  int least;       // cost that a range should have at least
-  bool vec_q, vec_blk;  // q's / the block's rows can be read 4 (8) values at a time
-  float* part;     // [2 * grid][cta_rows][head_dim] partial sums
-  float4* ml;      // [2 * grid][cta_rows] their reference, weight and value exponent
+  KvSplit sp;
+  int mg;     // warps that share a tile, each with its own query rows
+  int depth;  // stages per lane
+  bool vec_q, vec_blk;  // q's / the block's rows can be read 4 values at a time
 };
 
-// tiles before each sequence, for one KV head and row block (P [batch + 1]); a sequence without a
-// cached row counts as one tile: its block's own rows still have to be attended
-__device__ __forceinline__ int seq_len(const AttnArgs& p, int b) {
-  return int(min(int64_t(max(__ldg(p.lengths + b), 0)), int64_t(p.max_pages) * p.page));
-}
-
-template <int kThreads>
-__device__ __forceinline__ void scan_tiles(const AttnArgs& p, int* P, int* warp_sums) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int before = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int b = base + tid;
-    const int mine = b < p.batch ? max(1, (seq_len(p, b) + kTile - 1) / kTile) : 0;
-    int x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int pre = before;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) pre += warp_sums[w];
-      before += warp_sums[w];
-    }
-    if (b < p.batch) P[b] = pre + x - mine;
-    __syncthreads();
-  }
-  if (tid == 0) P[p.batch] = before;
-  __syncthreads();
-}
-
-// where tile x of the line lies: sequence b, unit u of it (KV head * row_blocks + row block), tile t of T
-struct Place {
-  int b, u, t, T;
-};
-// with `cost` > 0, x counts that many more tiles in front of each unit (t < 0 there)
-__device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int64_t x, int cost) {
-  int lo = 0, hi = batch;  // the last sequence that starts at or before x
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((int64_t(P[mid]) + int64_t(mid) * cost) * hr <= x)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  Place r;
-  r.b = lo;
-  r.T = P[lo + 1] - P[lo];
-  const int64_t rem = x - (int64_t(P[lo]) + int64_t(lo) * cost) * hr;
-  r.u = int(rem / (r.T + cost));
-  r.t = int(rem - int64_t(r.u) * (r.T + cost)) - cost;
-  return r;
-}
-// the first tile of CTA i's range; short lines go to fewer CTAs
-__device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, int ctas, int snap, int least) {
-  const int64_t total = (int64_t(P[batch]) + int64_t(batch) * kUnitCost) * hr;
-  ctas = int(min(int64_t(ctas), (total + least - 1) / least));
-  if (i <= 0) return 0;
-  if (i >= ctas) return P[batch] * hr;
-  const Place a = place_of(P, batch, hr, total * i / ctas, kUnitCost);
-  const int d = min(snap, a.T / 2);
-  const int t = a.t <= d ? 0 : a.T - a.t <= d ? a.T : a.t;
-  return P[a.b] * hr + a.u * a.T + t;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -305,47 +207,6 @@ __device__ __forceinline__ void zero(float (&x)[A][4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[a][e] = 0.f;
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// the barrier gets one (counted) arrival once this thread's earlier cp.async have landed
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= -kLowest ? a : 0.f;
-}
-__device__ __forceinline__ float scaled(float x, float f) {  // what is not finite becomes NaN
-  return fabsf(x) <= -kLowest ? x * f : __int_as_float(0x7fffffff);
-}
-// V (a multiple of 4) contiguous values
-template <typename T, int V>
-__device__ __forceinline__ void load_vals(const T* p, bool vec, float (&x)[V]) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      if constexpr (std::is_same<T, float>::value) {
-        const float4 v = *reinterpret_cast<const float4*>(p + i);
-        x[i] = v.x;
-        x[i + 1] = v.y;
-        x[i + 2] = v.z;
-        x[i + 3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(p + i);
-        x[i] = __uint_as_float(v.x << 16);
-        x[i + 1] = __uint_as_float(v.x & 0xffff0000u);
-        x[i + 2] = __uint_as_float(v.y << 16);
-        x[i + 3] = __uint_as_float(v.y & 0xffff0000u);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = ld_f(p, i);
-  }
-}
-
 // 16 of the block's own rows as B fragments of f16 terms, and their exponents, in words
 __host__ __device__ constexpr int mma_block_words(int hd, int terms) {
   return 2 * (hd / 16) * terms * 64 + hd / 8 * terms * 64 + 32;
@@ -399,7 +260,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   const int gq = lane >> 2, cq = lane & 3;
   const int mg = pl.mg, tl = kWarps / mg, S = pl.depth * tl;
   const int my_mg = warp / tl, my_tl = warp % tl;
-  const int hr = p.n_kv * pl.row_blocks;
+  const int hr = p.n_kv * pl.sp.row_blocks;
   const int cta_rows = kWarpRows * mg;
   const int row_r = tid / TPR, row_d = tid % TPR * VB;  // this thread's row (of 16) and first column in staging
 
@@ -411,8 +272,8 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   fence_mbar_init();
   scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
   const int ctas = gridDim.x;
-  const int start = cut(P, p.batch, hr, blockIdx.x, ctas, pl.snap, pl.least);
-  const int n_tiles = cut(P, p.batch, hr, blockIdx.x + 1, ctas, pl.snap, pl.least) - start;
+  const int start = cut(P, p.batch, hr, blockIdx.x, ctas, pl.sp);
+  const int n_tiles = cut(P, p.batch, hr, blockIdx.x + 1, ctas, pl.sp) - start;
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -436,7 +297,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       mbar_arrive(bar);
       return;
     }
-    const int64_t ph = int64_t(pg) * p.n_kv + a.u / pl.row_blocks;
+    const int64_t ph = int64_t(pg) * p.n_kv + a.u / pl.sp.row_blocks;
     const int64_t off = ph * p.page * HD + int64_t((a.t * kTile % p.page) / kTile) * kKeyBytes;
     cp_async4(smem_u32(sc), (half ? p.v_scale : p.k_scale) + ph);
     cp_async_arrive(bar);
@@ -474,8 +335,8 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     const Place un = place_of(P, p.batch, hr, start + a0, 0);
     const int a1 = min(n_tiles, a0 + un.T - un.t);
     const bool last = un.t + a1 - a0 == un.T, whole = last && un.t == 0;
-    const int g = un.u / pl.row_blocks, r0 = (un.u % pl.row_blocks) * cta_rows;
-    const int n_rows = min(cta_rows, pl.rows - r0);
+    const int g = un.u / pl.sp.row_blocks, r0 = (un.u % pl.sp.row_blocks) * cta_rows;
+    const int n_rows = min(cta_rows, pl.sp.rows - r0);
     const int len = seq_len(p, un.b);
     const int group = p.n_heads / p.n_kv;
 
@@ -982,11 +843,11 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
                 *reinterpret_cast<__nv_bfloat162*>(out + 8 * n) = __floats2bfloat162_rn(y0, y1);
             }
           } else {
-            float* dst = pl.part + (int64_t(slot) * cta_rows + r) * HD + 2 * cq;
+            float* dst = pl.sp.part + (int64_t(slot) * cta_rows + r) * HD + 2 * cq;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-            if (cq == 0) pl.ml[int64_t(slot) * cta_rows + r] = make_float4(M[mt][h], W[mt][h], E, 0.f);
+            if (cq == 0) pl.sp.ml[int64_t(slot) * cta_rows + r] = make_float4(M[mt][h], W[mt][h], E, 0.f);
           }
         }
     }
@@ -1000,35 +861,35 @@ constexpr int kCombineWarps = 8;
 // first, it joins the unit's rows y * 8 .. y * 8 + 7, a warp each: the partial sums of its ranges in
 // order, then the division and the one rounding to T.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(const AttnArgs p, const MmaPlan pl,
-                                                                               int ctas, int cta_rows) {
+__global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(const AttnArgs p, const KvSplit sp) {
   constexpr int V = HD / 32;
+  const int ctas = sp.ctas, cta_rows = sp.cta_rows;
   extern __shared__ __align__(16) int P[];
   __shared__ int sums[kCombineWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hr = p.n_kv * pl.row_blocks;
+  const int hr = p.n_kv * sp.row_blocks;
   int* cuts = P + p.batch + 1;
   scan_tiles<kCombineWarps * 32>(p, P, sums);
   const int i = blockIdx.x;
   const int total = P[p.batch] * hr;
-  const int x = cut(P, p.batch, hr, i + 1, ctas, pl.snap, pl.least);
+  const int x = cut(P, p.batch, hr, i + 1, ctas, sp);
   if (x >= total || x == 0) return;
   const Place un = place_of(P, p.batch, hr, x, 0);
   const int u0 = x - un.t, u1 = u0 + un.T;
-  if (un.t == 0 || cut(P, p.batch, hr, i, ctas, pl.snap, pl.least) > u0) return;
-  for (int k = i + tid; k <= ctas; k += kCombineWarps * 32) cuts[k] = cut(P, p.batch, hr, k, ctas, pl.snap, pl.least);
+  if (un.t == 0 || cut(P, p.batch, hr, i, ctas, sp) > u0) return;
+  for (int k = i + tid; k <= ctas; k += kCombineWarps * 32) cuts[k] = cut(P, p.batch, hr, k, ctas, sp);
   __syncthreads();
   int last = i + 1;  // the range that holds the unit's last tile
   while (cuts[last + 1] < u1) ++last;
-  const int g = un.u / pl.row_blocks, r0 = (un.u % pl.row_blocks) * cta_rows;
+  const int g = un.u / sp.row_blocks, r0 = (un.u % sp.row_blocks) * cta_rows;
   const int r = blockIdx.y * kCombineWarps + warp;
-  if (r >= min(cta_rows, pl.rows - r0)) return;
+  if (r >= min(cta_rows, sp.rows - r0)) return;
   // range i's part is its last (slot 2 i + 1), the others' their first (slot 2 k); empty ranges have none
   auto slot_of = [&](int k) { return int64_t(k == i ? 2 * i + 1 : 2 * k) * cta_rows + r; };
   float M = -INFINITY, E = -200.f;
   for (int k = i + lane; k <= last; k += 32)
     if (cuts[k] < cuts[k + 1]) {
-      const float4 w = pl.ml[slot_of(k)];
+      const float4 w = sp.ml[slot_of(k)];
       M = fmaxf(M, w.x);
       E = fmaxf(E, w.z);
     }
@@ -1042,9 +903,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   for (int k = i; k <= last; ++k) {
     if (cuts[k] == cuts[k + 1]) continue;
     const int64_t s = slot_of(k);
-    const float4 w = pl.ml[s];
+    const float4 w = sp.ml[s];
     const float f = ex2(w.x - ref), fo = f * ex2(fmaxf(w.z - E, -126.f));
-    const float* src = pl.part + s * HD + lane * V;
+    const float* src = sp.part + s * HD + lane * V;
     l = fmaf(w.y, f, l);
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = fmaf(src[j], fo, o[j]);
@@ -1082,45 +943,39 @@ int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cuda
   int depth = std::max(kMaxDepth, sh.mg);
   while (depth > 1 && mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes > kMmaSmemMax) --depth;
   const int smem = mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes;
-  if (smem > kMmaSmemMax) return fail(DSM_ERR_UNSUPPORTED, "dsm_gqa_attn_kv8: batch too large for shared memory");
+  if (smem > kMmaSmemMax) return DSM_ERR_UNSUPPORTED;
   pl.depth = depth;
   auto k = kv8_attn_mma_kernel<T, HD, MT>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("gqa_attn_kv8 smem attribute");
   k<<<unsigned(ctas), mma_warps(HD) * 32, size_t(smem), s>>>(a, pl);
   const int st = check_launch("gqa_attn_kv8");
-  if (st != DSM_OK || ctas == 1) return st;
-  const dim3 grid(unsigned(ctas - 1), unsigned(ceil_div(std::min(sh.cta_rows, pl.rows), kCombineWarps)));
-  kv8_attn_combine_kernel<T, HD><<<grid, kCombineWarps * 32, size_t(a.batch + ctas + 2) * 4, s>>>(a, pl, ctas,
-                                                                                                   sh.cta_rows);
-  return check_launch("gqa_attn_kv8 combine");
+  return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, std::is_same<T, float>::value ? DSM_DT_F32 : DSM_DT_BF16, s);
 }
 
 size_t mma_ws_bytes(int cta_rows, int hd) { return size_t(2 * num_sms()) * cta_rows * (size_t(hd) + 4) * 4; }
-
-bool vec_ok(const void* p, int64_t s0, int64_t s1, int64_t s2, size_t bytes) {
-  const size_t e = bytes / 4;  // one load takes four values
-  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && s0 * e % bytes == 0 && s1 * e % bytes == 0 && s2 * e % bytes == 0;
-}
 
 template <typename T>
 int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd, sizeof(T) == 4 ? DSM_DT_F32 : DSM_DT_BF16);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * sh.row_blocks;
-  if (most > 0x7fffffff) return fail(DSM_ERR_UNSUPPORTED, "dsm_gqa_attn_kv8: block table too large");
+  if (most > 0x7fffffff) return DSM_ERR_UNSUPPORTED;
   const int ctas = int(std::min<int64_t>(num_sms(), most));
   MmaPlan pl;
   pl.mg = sh.mg;
-  pl.row_blocks = sh.row_blocks;
-  pl.rows = a.n_heads / a.n_kv * a.block;
+  pl.sp.row_blocks = sh.row_blocks;
+  pl.sp.rows = a.n_heads / a.n_kv * a.block;
+  pl.sp.cta_rows = sh.cta_rows;
+  pl.sp.cost = kUnitCost;
+  pl.sp.snap = std::max(1, mma_warps(hd) / sh.mg / 2);
+  pl.sp.least = kUnitCost;
+  pl.sp.ctas = ctas;
   pl.depth = 0;
-  pl.snap = std::max(1, mma_warps(hd) / sh.mg / 2);
-  pl.least = kUnitCost;
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 4 * sizeof(T));
   pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 4 * sizeof(T)) &&
                vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 4 * sizeof(T));
-  pl.part = static_cast<float*>(ws);
-  pl.ml = reinterpret_cast<float4*>(pl.part + size_t(2 * num_sms()) * sh.cta_rows * hd);
+  pl.sp.part = static_cast<float*>(ws);
+  pl.sp.ml = reinterpret_cast<float4*>(pl.sp.part + size_t(2 * num_sms()) * sh.cta_rows * hd);
   constexpr int kWide = sizeof(T) == 4 ? 1 : 2;
   switch (hd) {
     case 64: return sh.mt == 1 ? launch_mma<T, 64, 1>(a, sh, pl, ctas, s) : launch_mma<T, 64, kWide>(a, sh, pl, ctas, s);
@@ -1130,6 +985,20 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
 }
 
 }  // namespace
+
+int kv8_combine(const AttnArgs& a, const KvSplit& sp, int hd, int dtype, cudaStream_t s) {
+  if (sp.ctas == 1) return DSM_OK;
+  const dim3 grid(unsigned(sp.ctas - 1), unsigned(ceil_div(std::min(sp.cta_rows, sp.rows), kCombineWarps)));
+  const size_t smem = size_t(a.batch + sp.ctas + 2) * 4;
+  const bool bf = dtype == DSM_DT_BF16;
+  using B = __nv_bfloat16;
+  auto k = hd == 64    ? (bf ? kv8_attn_combine_kernel<B, 64> : kv8_attn_combine_kernel<float, 64>)
+           : hd == 128 ? (bf ? kv8_attn_combine_kernel<B, 128> : kv8_attn_combine_kernel<float, 128>)
+                       : (bf ? kv8_attn_combine_kernel<B, 256> : kv8_attn_combine_kernel<float, 256>);
+  k<<<grid, kCombineWarps * 32, smem, s>>>(a, sp);
+  return check_launch("gqa_attn_kv8 combine");
+}
+
 }  // namespace dsm
 
 using namespace dsm;
@@ -1139,8 +1008,7 @@ extern "C" size_t dsm_gqa_attn_kv8_workspace_bytes(int batch, int block, int n_h
       !kv8_head_dim_ok(head_dim))
     return 0;
   const int rows = n_heads / n_kv * block;
-  return mma_ws_bytes(std::max(mma_shape(rows, head_dim, DSM_DT_F32).cta_rows, mma_shape(rows, head_dim, DSM_DT_BF16).cta_rows),
-                      head_dim);
+  return std::max(mma_ws_bytes(mma_shape(rows, head_dim, DSM_DT_F32).cta_rows, head_dim), kv8_umma_ws_bytes(rows, head_dim));
 }
 
 extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const int32_t* block_table,
@@ -1196,8 +1064,14 @@ extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const
                       d->scale,
                       out};
   cudaStream_t s = as_stream(stream);
-  if (attn_kernel() == 0)
-    return d->dtype == DSM_DT_BF16 ? run_mma<__nv_bfloat16>(a, d->head_dim, ws, s) : run_mma<float>(a, d->head_dim, ws, s);
+  if (attn_kernel() == 0) {
+    int st = DSM_ERR_UNSUPPORTED;
+    if (d->dtype == DSM_DT_F32)
+      st = run_mma<float>(a, d->head_dim, ws, s);
+    else if (d->block <= kUmmaMaxBlock)
+      st = kv8_umma(a, d->head_dim, ws, s);
+    if (st != DSM_ERR_UNSUPPORTED) return st;
+  }
   if (d->dtype == DSM_DT_BF16) {
     switch (d->head_dim) {
       case 64: return launch_core<__nv_bfloat16, 64>(a, s);
