@@ -271,9 +271,8 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   }
   fence_mbar_init();
   scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
-  const int ctas = gridDim.x;
-  const int start = cut(P, p.batch, hr, blockIdx.x, ctas, pl.sp);
-  const int n_tiles = cut(P, p.batch, hr, blockIdx.x + 1, ctas, pl.sp) - start;
+  int start;
+  const int n_tiles = my_range(p, P, pl.sp, start);
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -863,56 +862,50 @@ constexpr int kCombineWarps = 8;
 template <typename T, int HD>
 __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(const AttnArgs p, const KvSplit sp) {
   constexpr int V = HD / 32;
-  const int ctas = sp.ctas, cta_rows = sp.cta_rows;
-  extern __shared__ __align__(16) int P[];
-  __shared__ int sums[kCombineWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hr = p.n_kv * sp.row_blocks;
-  int* cuts = P + p.batch + 1;
-  scan_tiles<kCombineWarps * 32>(p, P, sums);
-  const int i = blockIdx.x;
-  const int total = P[p.batch] * hr;
-  const int x = cut(P, p.batch, hr, i + 1, ctas, sp);
-  if (x >= total || x == 0) return;
-  const Place un = place_of(P, p.batch, hr, x, 0);
-  const int u0 = x - un.t, u1 = u0 + un.T;
-  if (un.t == 0 || cut(P, p.batch, hr, i, ctas, sp) > u0) return;
-  for (int k = i + tid; k <= ctas; k += kCombineWarps * 32) cuts[k] = cut(P, p.batch, hr, k, ctas, sp);
-  __syncthreads();
-  int last = i + 1;  // the range that holds the unit's last tile
-  while (cuts[last + 1] < u1) ++last;
-  const int g = un.u / sp.row_blocks, r0 = (un.u % sp.row_blocks) * cta_rows;
-  const int r = blockIdx.y * kCombineWarps + warp;
-  if (r >= min(cta_rows, sp.rows - r0)) return;
-  // range i's part is its last (slot 2 i + 1), the others' their first (slot 2 k); empty ranges have none
-  auto slot_of = [&](int k) { return int64_t(k == i ? 2 * i + 1 : 2 * k) * cta_rows + r; };
-  float M = -INFINITY, E = -200.f;
-  for (int k = i + lane; k <= last; k += 32)
-    if (cuts[k] < cuts[k + 1]) {
-      const float4 w = sp.ml[slot_of(k)];
-      M = fmaxf(M, w.x);
-      E = fmaxf(E, w.z);
-    }
-  M = kv8_warp_max(M);
-  E = kv8_warp_max(E);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float l = 0.f, o[V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i = blockIdx.x, r = blockIdx.y * kCombineWarps + warp;
+  const int4 at = sp.places[i + 1];  // sequence, unit, tile, tiles
+  const int x = sp.cuts[i + 1], before = sp.cuts[i], end = sp.cuts[sp.ctas];
+  const int u0 = x - at.z, u1 = u0 + at.w;
+  if (x >= end || at.z == 0 || before > u0) return;
+  const int g = at.y / sp.row_blocks, r0 = (at.y % sp.row_blocks) * sp.cta_rows;
+  if (r >= min(sp.cta_rows, sp.rows - r0)) return;
+  // 32 ranges at a time, a lane each: range i's part is its last (slot 2 i + 1), the others' their first (slot
+  // 2 k); empty ranges have none
+  float M = -INFINITY, E = -200.f, l = 0.f, o[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) o[j] = 0.f;
-#pragma unroll 4
-  for (int k = i; k <= last; ++k) {
-    if (cuts[k] == cuts[k + 1]) continue;
-    const int64_t s = slot_of(k);
-    const float4 w = sp.ml[s];
-    const float f = ex2(w.x - ref), fo = f * ex2(fmaxf(w.z - E, -126.f));
-    const float* src = sp.part + s * HD + lane * V;
-    l = fmaf(w.y, f, l);
+  for (int base = i; base < sp.ctas; base += 32) {
+    const int k = base + lane;
+    const int c0 = sp.cuts[min(k, sp.ctas)], c1 = sp.cuts[min(k + 1, sp.ctas)];
+    const bool mine = c0 < c1 && c0 < u1;
+    const int64_t slot = int64_t(k == i ? 2 * i + 1 : 2 * k) * sp.cta_rows + r;
+    const float4 w = mine ? sp.ml[slot] : make_float4(-INFINITY, 0.f, -200.f, 0.f);
+    const float M2 = fmaxf(M, kv8_warp_max(w.x)), E2 = fmaxf(E, kv8_warp_max(w.z));
+    const float ref = M2 == -INFINITY ? 0.f : M2;
+    const float keep = ex2(M - ref) * ex2(fmaxf(E - E2, -126.f));
+    l *= ex2(M - ref);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = fmaf(src[j], fo, o[j]);
+    for (int j = 0; j < V; ++j) o[j] *= keep;
+    M = M2;
+    E = E2;
+    const float f = mine ? ex2(w.x - ref) : 0.f, fo = f * ex2(fmaxf(w.z - E, -126.f));
+    l += kv8_warp_sum(w.y * f);
+    const unsigned parts = __ballot_sync(0xffffffffu, mine);
+    const float* src = sp.part + lane * V;
+#pragma unroll 4
+    for (int j = 0; j < 32 - __clz(parts); ++j) {
+      const float fj = __shfl_sync(0xffffffffu, fo, j);
+      const int64_t sj = __shfl_sync(0xffffffffu, slot, j);
+      if (parts >> j & 1)
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = fmaf(src[sj * HD + v], fj, o[v]);
+    }
+    if (__shfl_sync(0xffffffffu, c1, 31) >= u1) break;  // the unit's last tile lies in these ranges
   }
   const int rr = r0 + r, group = p.n_heads / p.n_kv;
   T* out = static_cast<T*>(p.out) +
-           ((int64_t(un.b) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + lane * V;
+           ((int64_t(at.x) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + lane * V;
   const float inv = 1.f / l, fe = kv8_exp2i(max(int(E), -126));
 #pragma unroll
   for (int j = 0; j < V; ++j) out[j] = st_f<T>(l == 0.f ? 0.f : o[j] * inv * fe);
@@ -953,7 +946,7 @@ int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cuda
   return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, std::is_same<T, float>::value ? DSM_DT_F32 : DSM_DT_BF16, s);
 }
 
-size_t mma_ws_bytes(int cta_rows, int hd) { return size_t(2 * num_sms()) * cta_rows * (size_t(hd) + 4) * 4; }
+size_t mma_ws_bytes(int cta_rows, int hd) { return split_ws_bytes(num_sms(), cta_rows, hd); }
 
 template <typename T>
 int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
@@ -974,8 +967,7 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 4 * sizeof(T));
   pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 4 * sizeof(T)) &&
                vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 4 * sizeof(T));
-  pl.sp.part = static_cast<float*>(ws);
-  pl.sp.ml = reinterpret_cast<float4*>(pl.sp.part + size_t(2 * num_sms()) * sh.cta_rows * hd);
+  split_ws(pl.sp, ws, hd);
   constexpr int kWide = sizeof(T) == 4 ? 1 : 2;
   switch (hd) {
     case 64: return sh.mt == 1 ? launch_mma<T, 64, 1>(a, sh, pl, ctas, s) : launch_mma<T, 64, kWide>(a, sh, pl, ctas, s);
@@ -989,13 +981,12 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
 int kv8_combine(const AttnArgs& a, const KvSplit& sp, int hd, int dtype, cudaStream_t s) {
   if (sp.ctas == 1) return DSM_OK;
   const dim3 grid(unsigned(sp.ctas - 1), unsigned(ceil_div(std::min(sp.cta_rows, sp.rows), kCombineWarps)));
-  const size_t smem = size_t(a.batch + sp.ctas + 2) * 4;
   const bool bf = dtype == DSM_DT_BF16;
   using B = __nv_bfloat16;
   auto k = hd == 64    ? (bf ? kv8_attn_combine_kernel<B, 64> : kv8_attn_combine_kernel<float, 64>)
            : hd == 128 ? (bf ? kv8_attn_combine_kernel<B, 128> : kv8_attn_combine_kernel<float, 128>)
                        : (bf ? kv8_attn_combine_kernel<B, 256> : kv8_attn_combine_kernel<float, 256>);
-  k<<<grid, kCombineWarps * 32, smem, s>>>(a, sp);
+  k<<<grid, kCombineWarps * 32, 0, s>>>(a, sp);
   return check_launch("gqa_attn_kv8 combine");
 }
 

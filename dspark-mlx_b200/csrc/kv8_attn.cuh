@@ -40,7 +40,18 @@ struct KvSplit {
   int ctas;
   float* part;     // [2 * ctas][cta_rows][head_dim] partial sums: a range's first unit, its last
   float4* ml;      // [2 * ctas][cta_rows] their reference, weight and value exponent
+  int4* places;    // [ctas] where each range starts: sequence, unit, tile, the sequence's tiles
+  int* cuts;       // [ctas + 1] the line's tile there
 };
+inline size_t split_ws_bytes(int ctas, int cta_rows, int hd) {
+  return size_t(2 * ctas) * cta_rows * (size_t(hd) + 4) * 4 + size_t(ctas) * 16 + size_t(ctas + 1) * 4;
+}
+inline void split_ws(KvSplit& sp, void* ws, int hd) {
+  sp.part = static_cast<float*>(ws);
+  sp.ml = reinterpret_cast<float4*>(sp.part + size_t(2 * sp.ctas) * sp.cta_rows * hd);
+  sp.places = reinterpret_cast<int4*>(sp.ml + size_t(2 * sp.ctas) * sp.cta_rows);
+  sp.cuts = reinterpret_cast<int*>(sp.places + sp.ctas);
+}
 
 // tiles before each sequence, for one KV head and row block (P [batch + 1]); a sequence without a
 // cached row counts as one tile: its block's own rows still have to be attended
@@ -109,6 +120,20 @@ __device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, int c
   const int d = min(snap, a.T / 2);
   const int t = a.t <= d ? 0 : a.T - a.t <= d ? a.T : a.t;
   return P[a.b] * hr + a.u * a.T + t;
+}
+
+// this CTA's range [first, first + n) of the line, noted down for the join
+__device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const KvSplit& sp, int& first) {
+  const int hr = p.n_kv * sp.row_blocks, i = blockIdx.x;
+  first = cut(P, p.batch, hr, i, sp.ctas, sp);
+  const int end = cut(P, p.batch, hr, i + 1, sp.ctas, sp);
+  if (threadIdx.x == 0) {
+    const Place a = place_of(P, p.batch, hr, min(first, P[p.batch] * hr - 1), 0);
+    sp.places[i] = make_int4(a.b, a.u, a.t, a.T);
+    sp.cuts[i] = first;
+    if (i == sp.ctas - 1) sp.cuts[i + 1] = end;
+  }
+  return end - first;
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -44,12 +44,15 @@ constexpr float kPExp = 8.f;   // weights at the reference: 2^8
 constexpr float kPMax = 8.75f;  // 2^8.75 = 431 still fits e4m3
 constexpr float kPHead = 1.f;  // a new reference lies this much above the maximum
 
+__host__ __device__ constexpr int mma_cols(int nr) { return nr <= 16 ? 16 : nr <= 32 ? 32 : 64; }
+__host__ __device__ constexpr int weight_buffers(int nr) { return nr > 32 ? 1 : 2; }
+
 template <int HD, int NR>
 struct Cfg {
-  static constexpr int NM = NR < 16 ? 16 : NR;          // columns of the products
+  static constexpr int NM = mma_cols(NR);               // columns of the products
   static constexpr int NH = HD <= 128 ? 1 : 2;          // 128-row halves of the output
   static constexpr int CTAS = HD == 256 ? 1 : 2;        // per SM
-  static constexpr int PB = NR == 64 ? 1 : 2;           // buffers of weights
+  static constexpr int PB = weight_buffers(NR);         // buffers of weights
   static constexpr int kHalf = kTile * HD;              // bytes of 64 keys, or of their values
   static constexpr int kStage = 4 * kHalf;              // keys, then values, of 128
   static constexpr int kQTerm = NM * HD;                // bytes of one term of q
@@ -72,7 +75,7 @@ struct UmmaSmem {
 constexpr int kRowFloats = 9;
 __host__ __device__ inline UmmaSmem umma_smem(int hd, int nr, int stages, int block, int batch) {
   UmmaSmem s;
-  const int nm = nr < 16 ? 16 : nr, pb = nr == 64 ? 1 : 2;
+  const int nm = mma_cols(nr), pb = weight_buffers(nr);
   s.q = stages * 4 * kTile * hd;
   s.p = s.q + 2 * nm * hd;
   s.w = s.p + pb * 2 * nm * kStepKeys;
@@ -98,9 +101,19 @@ __device__ __forceinline__ uint64_t desc_sw64(uint32_t saddr) {
   return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(512 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(4) << 61);
 }
-// kind::f8f6f4: D f32, A e4m3, B e4m3 or e5m2, both K-major
-__device__ __forceinline__ uint32_t idesc_f8(int n, bool b_e5m2) {
-  return (1u << 4) | (b_e5m2 ? 1u << 10 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+// the weights, rows of 16, 32 or 64 bytes per key (the operand's N dimension contiguous): 16-byte rows
+// unswizzled with groups of 8 keys at 128 B (the leading offset), 32- and 64-byte rows in the swizzle of their
+// width with groups of 8 keys at 256 and 512 B (the stride)
+template <int NM>
+__device__ __forceinline__ uint64_t desc_weights(uint32_t saddr) {
+  constexpr uint64_t lead = NM == 16 ? 128 >> 4 : 1, stride = NM == 16 ? 128 >> 4 : 8 * NM >> 4;
+  constexpr uint64_t swizzle = NM == 16 ? 0 : NM == 32 ? 6 : 4;
+  return uint64_t((saddr >> 4) & 0x3FFFu) | (lead << 16) | (stride << 32) | (uint64_t(1) << 46) | (swizzle << 61);
+}
+// kind::f8f6f4: D f32, A e4m3 K-major, B e4m3 or e5m2, K-major or (b_rows) N-major
+__device__ __forceinline__ uint32_t idesc_f8(int n, bool b_e5m2, bool b_rows) {
+  return (1u << 4) | (b_e5m2 ? 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(128 >> 4) << 24);
 }
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   const uint32_t no_mask = 0u, acc = accumulate ? 1u : 0u;
@@ -113,21 +126,27 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_
 // this thread's lane: N consecutive columns
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, float* x) {
-  if constexpr (N == 8) {
+  if constexpr (N >= 16) {
+    uint32_t r[16];
+    tc::tmem_ld16(addr, r);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+    if constexpr (N > 16) tmem_ld<N - 16>(addr + 16, x + 16);
+  } else if constexpr (N >= 8) {
     uint32_t r[8];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(addr));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
+    if constexpr (N > 8) tmem_ld<N - 8>(addr + 8, x + 8);
   } else {
+    uint32_t r[4];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
 #pragma unroll
-    for (int c = 0; c < N; c += 16) {
-      uint32_t r[16];
-      tc::tmem_ld16(addr + c, r);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[c + i] = __uint_as_float(r[i]);
-    }
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
   }
 }
 __device__ __forceinline__ bool any_of_softmax(bool x) {  // over the four softmax warps, with a barrier
@@ -163,6 +182,35 @@ __device__ __forceinline__ void weight_terms(float x0, float x1, float x2, float
       " mov.b32 %1, {c, d};\n}"
       : "=&r"(hi), "=&r"(lo)
       : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+}
+__device__ __forceinline__ void store_words(uint32_t at, const uint32_t (&w)[4], int n) {  // n is a constant
+  if (n == 4)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+  else if (n == 2)
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(w[0]), "r"(w[1]) : "memory");
+  else
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w[0]) : "memory");
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
 }
 // four values of a query row -> two e4m3 terms
 __device__ __forceinline__ void q_terms(const float* x, uint32_t& hi, uint32_t& lo) {
@@ -237,8 +285,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
   }
   if (warp == 5) tc::tmem_alloc(slot, C::kAlloc);
   scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
-  const int start = cut(P, p.batch, hr, blockIdx.x, pl.sp.ctas, pl.sp);
-  const int n_tiles = cut(P, p.batch, hr, blockIdx.x + 1, pl.sp.ctas, pl.sp) - start;
+  int start;
+  const int n_tiles = my_range(p, P, pl.sp, start);
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -328,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
   } else if (warp == 5) {
     // ---------------------------------------------------------------- products
     if (lane == 0) {
-      const uint32_t id_s = idesc_f8(NM, false), id_hi = idesc_f8(NM, false), id_lo = idesc_f8(NM, true);
+      const uint32_t id_s = idesc_f8(NM, false, false), id_hi = idesc_f8(NM, false, true), id_lo = idesc_f8(NM, true, true);
       const uint32_t base = smem_u32(smem), qa = base + L.q, pa = base + L.p;
       int k = 0, seg = 0;  // steps, and units with steps, so far
       for (int a0 = 0; a0 < n_tiles;) {
@@ -350,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks)
                 umma_f8(t_o + nh * NM, desc_sw64(v + (ks >> 1) * C::kHalf + nh * 128 * 64 + (ks & 1) * 32),
-                        tc::umma_desc_sw128(w + x * C::kPTerm + ks * 32), x ? id_lo : id_hi, !first || x > 0 || ks > 0);
+                        desc_weights<NM>(w + x * C::kPTerm + ks * 32 * NM), x ? id_lo : id_hi, !first || x > 0 || ks > 0);
           tc::umma_commit(empty + j % S);
           tc::umma_commit(p_empty + pb);
         };
@@ -390,11 +438,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
     const uint32_t t_lane = uint32_t(warp * 32) << 16;
     const int group = p.n_heads / p.n_kv;
     uint8_t* const q8 = smem + L.q;
-    // where this thread's key lies in the rows of weights: chunk tid / 16 of a row's 128 bytes, swizzled by
-    // the row
-    uint32_t p_at[8];
+    // where this thread's key's weights go, 16 rows at a time
+    uint32_t p_at[NM / 16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p_at[j] = smem_u32(smem) + L.p + j * 128 + (((tid >> 4) ^ j) << 4) + (tid & 15);
+    for (int c = 0; c < NM / 16; ++c)
+      p_at[c] = smem_u32(smem) + L.p + tid * NM + ((c ^ (NM == 32 ? (tid >> 2) & 1 : NM == 64 ? (tid >> 1) & 3 : 0)) << 4);
 
     int k = 0, outs = 0;  // steps, and units with steps, so far
     for (int a0 = 0; a0 < n_tiles;) {
@@ -492,15 +540,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_empty + sb);
-        // the weights' exponents: row_m is the reference less kPExp
+        // the weights' exponents: row_m is kPExp less the reference
         float top = kLowest;
 #pragma unroll
         for (int r = 0; r < NR; r += 4) {
           const float4 c = *reinterpret_cast<const float4*>(row_c + r), m = *reinterpret_cast<const float4*>(row_m + r);
-          y[r] = fmaf(y[r], c.x * ks, -m.x);
-          y[r + 1] = fmaf(y[r + 1], c.y * ks, -m.y);
-          y[r + 2] = fmaf(y[r + 2], c.z * ks, -m.z);
-          y[r + 3] = fmaf(y[r + 3], c.w * ks, -m.w);
+          const float2 ks2 = make_float2(ks, ks);
+          const float2 a = fma2(make_float2(y[r], y[r + 1]), mul2(make_float2(c.x, c.y), ks2), make_float2(m.x, m.y));
+          const float2 b = fma2(make_float2(y[r + 2], y[r + 3]), mul2(make_float2(c.z, c.w), ks2), make_float2(m.z, m.w));
+          y[r] = a.x;
+          y[r + 1] = a.y;
+          y[r + 2] = b.x;
+          y[r + 3] = b.y;
           top = fmaxf(top, fmaxf(fmaxf(y[r], y[r + 1]), fmaxf(y[r + 2], y[r + 3])));
         }
         if (any_of_softmax((live && top > kPMax) || i == 0 || want_rv != rv)) {
@@ -514,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
           if (tid < NR) {
             const float x = fmaxf(fmaxf(red[tid], red[NR + tid]), fmaxf(red[2 * NR + tid], red[3 * NR + tid]));
             const float up = x == kLowest ? 0.f : i == 0 || x > kPExp ? x + (kPHead - kPExp) : 0.f;
-            row_m[tid] += up;
+            row_m[tid] -= up;
             red[tid] = up;
             const float fv = rv <= -200 ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
             row_a[tid] = ex2(-up) * fv;
@@ -552,9 +603,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         const int dv = max((half ? e1 : e0) - rv, -60);  // <= 0
         const float fv = kv8_exp2i(dv);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          y[r] = live ? ex2(y[r]) : 0.f;
-          l[r] += y[r];
+        for (int r = 0; r < NR; ++r) y[r] = ex2(y[r]);
+        if (!__all_sync(0xffffffffu, live)) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) y[r] = live ? y[r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < NR; r += 2) {
+          const float2 a = add2(make_float2(l[r], l[r + 1]), make_float2(y[r], y[r + 1]));
+          l[r] = a.x;
+          l[r + 1] = a.y;
         }
         if (dv != 0) {
 #pragma unroll
@@ -563,15 +621,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         const int pb = C::PB == 2 ? k & 1 : 0, use = C::PB == 2 ? k >> 1 : k;
         if (ok && use > 0) ok = mbar_wait(p_empty + pb, (use - 1) & 1);
 #pragma unroll
-        for (int r = 0; r < NR; r += 4) {
-          uint32_t hi, lo;
-          weight_terms(y[r], y[r + 1], y[r + 2], y[r + 3], hi, lo);
+        for (int r = 0; r < NR; r += 16) {
+          constexpr int kWords = NR < 16 ? NR / 4 : 4;
+          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t at = p_at[(r + j) & 7] + pb * 2 * C::kPTerm + ((r + j) >> 3) * 1024;
-            asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "r"(hi >> (8 * j)) : "memory");
-            asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + C::kPTerm), "r"(lo >> (8 * j)) : "memory");
-          }
+          for (int w = 0; w < kWords; ++w)
+            if (r + 4 * w < NR) weight_terms(y[r + 4 * w], y[r + 4 * w + 1], y[r + 4 * w + 2], y[r + 4 * w + 3], hi[w], lo[w]);
+          const uint32_t at = p_at[r / 16] + pb * 2 * C::kPTerm;
+          store_words(at, hi, min(4, (NR - r) / 4));
+          store_words(at + C::kPTerm, lo, min(4, (NR - r) / 4));
         }
         // value codes without a key (behind the length, or of a page that is none) are cleared: a weight of
         // zero would not take a NaN there out
@@ -607,28 +665,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
       if (sg.steps > 0) {
         softmax_sync();  // every warp is done with `red`
         // halves of the rows change hands until a lane holds one row's (two rows') sum over the warp
-        int n = NR;
+        constexpr int NP = NR <= 4 ? 4 : NR <= 8 ? 8 : NR <= 16 ? 16 : NR <= 32 ? 32 : 64;
+        float x[NP];
+#pragma unroll
+        for (int r = 0; r < NP; ++r) x[r] = r < NR ? l[r] : 0.f;
+        int n = NP;
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) {
           if (n > 1) {
             n /= 2;
 #pragma unroll
-            for (int r = 0; r < NR / 2; ++r)
+            for (int r = 0; r < NP / 2; ++r)
               if (r < n) {
-                const float give = (lane & off) ? l[r] : l[r + n];
-                const float keep = (lane & off) ? l[r + n] : l[r];
-                l[r] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+                const float give = (lane & off) ? x[r] : x[r + n];
+                const float keep = (lane & off) ? x[r + n] : x[r];
+                x[r] = keep + __shfl_xor_sync(0xffffffffu, give, off);
               }
           } else {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
+            x[0] += __shfl_xor_sync(0xffffffffu, x[0], off);
           }
         }
-        if constexpr (NR == 64) {
-          red[warp * NR + 2 * lane] = l[0];
-          red[warp * NR + 2 * lane + 1] = l[1];
+        if constexpr (NP == 64) {
+          if (2 * lane < NR) {
+            red[warp * NR + 2 * lane] = x[0];
+            red[warp * NR + 2 * lane + 1] = x[1];
+          }
         } else {
-          constexpr int per = 32 / NR;  // lanes that hold the same row
-          if (lane % per == 0) red[warp * NR + lane / per] = l[0];
+          constexpr int per = 32 / NP;  // lanes that hold the same row
+          if (lane % per == 0 && lane / per < NR) red[warp * NR + lane / per] = x[0];
         }
       }
       softmax_sync();
@@ -636,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         // o and l are relative to row_m, o in units of 2^rv; the block's to mb
         const bool ctx = sg.steps > 0;
         const float lc = ctx ? red[tid] + red[NR + tid] + red[2 * NR + tid] + red[3 * NR + tid] : 0.f;
-        const float m = lc == 0.f ? -INFINITY : row_m[tid], mb = blk ? row_mb[tid] : -INFINITY;
+        const float m = lc == 0.f ? -INFINITY : -row_m[tid], mb = blk ? row_mb[tid] : -INFINITY;
         const float M = fmaxf(m, mb), ref = M == -INFINITY ? 0.f : M;
         const float fa = ex2(m - ref), fb = blk ? ex2(mb - ref) : 0.f;
         const float den = lc * fa + (blk ? row_lb[tid] * fb : 0.f);
@@ -740,7 +804,8 @@ int byte_map(CUtensorMap* map, const void* base, int64_t rows, int width, int bo
   return DSM_OK;
 }
 
-int rows_of(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// query rows per CTA: multiples of 8, since the softmax costs by the row, and 4 for single tokens
+int rows_of(int rows) { return rows <= 4 ? 4 : std::min(64, (rows + 7) / 8 * 8); }
 int ctas_per_sm(int hd) { return hd == 256 ? 1 : 2; }
 
 template <int HD, int NR>
@@ -771,9 +836,14 @@ int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
 template <int HD>
 int launch_rows(int nr, const AttnArgs& a, const UmmaPlan& pl, cudaStream_t s) {
   switch (nr) {
+    case 4: return launch<HD, 4>(a, pl, s);
     case 8: return launch<HD, 8>(a, pl, s);
     case 16: return launch<HD, 16>(a, pl, s);
+    case 24: return launch<HD, 24>(a, pl, s);
     case 32: return launch<HD, 32>(a, pl, s);
+    case 40: return launch<HD, 40>(a, pl, s);
+    case 48: return launch<HD, 48>(a, pl, s);
+    case 56: return launch<HD, 56>(a, pl, s);
     default: return launch<HD, 64>(a, pl, s);
   }
 }
@@ -781,7 +851,7 @@ int launch_rows(int nr, const AttnArgs& a, const UmmaPlan& pl, cudaStream_t s) {
 }  // namespace
 
 size_t kv8_umma_ws_bytes(int rows, int hd) {
-  return size_t(2 * ctas_per_sm(hd) * num_sms()) * rows_of(rows) * (size_t(hd) + 4) * 4;
+  return split_ws_bytes(ctas_per_sm(hd) * num_sms(), rows_of(rows), hd);
 }
 
 int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
@@ -799,8 +869,7 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   pl.sp.cost = 6;
   pl.sp.snap = 4;
   pl.sp.least = 12;
-  pl.sp.part = static_cast<float*>(ws);
-  pl.sp.ml = reinterpret_cast<float4*>(pl.sp.part + size_t(2 * most_ctas) * nr * hd);
+  split_ws(pl.sp, ws, hd);
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 8);
   pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 8);
   switch (hd) {
