@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   fence_mbar_init();
   scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
   int start;
-  const int n_tiles = my_range(p, P, pl.sp, start);
+  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 12, start);
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -952,7 +952,6 @@ template <typename T>
 int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd, sizeof(T) == 4 ? DSM_DT_F32 : DSM_DT_BF16);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * sh.row_blocks;
-  if (most > 0x7fffffff) return DSM_ERR_UNSUPPORTED;
   const int ctas = int(std::min<int64_t>(num_sms(), most));
   MmaPlan pl;
   pl.mg = sh.mg;
@@ -963,6 +962,7 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   pl.sp.snap = std::max(1, mma_warps(hd) / sh.mg / 2);
   pl.sp.least = kUnitCost;
   pl.sp.ctas = ctas;
+  if (!split_fits(a, pl.sp)) return DSM_ERR_UNSUPPORTED;
   pl.depth = 0;
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 4 * sizeof(T));
   pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 4 * sizeof(T)) &&

@@ -43,6 +43,10 @@ struct KvSplit {
   int4* places;    // [ctas] where each range starts: sequence, unit, tile, the sequence's tiles
   int* cuts;       // [ctas + 1] the line's tile there
 };
+// tiles and their units' costs stay in 32 bits
+inline bool split_fits(const AttnArgs& a, const KvSplit& sp) {
+  return (int64_t(a.max_pages) * (a.page / kTile) + sp.cost) * a.batch * a.n_kv * sp.row_blocks <= 0x7fffffff;
+}
 inline size_t split_ws_bytes(int ctas, int cta_rows, int hd) {
   return size_t(2 * ctas) * cta_rows * (size_t(hd) + 4) * 4 + size_t(ctas) * 16 + size_t(ctas + 1) * 4;
 }
@@ -72,6 +76,7 @@ __device__ __forceinline__ void scan_tiles(const AttnArgs& p, int* P, int* warp_
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
+    if (base > 0) __syncthreads();  // warp_sums have been read
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
     int pre = before;
@@ -81,7 +86,6 @@ __device__ __forceinline__ void scan_tiles(const AttnArgs& p, int* P, int* warp_
       before += warp_sums[w];
     }
     if (b < p.batch) P[b] = pre + x - mine;
-    __syncthreads();
   }
   if (tid == 0) P[p.batch] = before;
   __syncthreads();
@@ -92,11 +96,11 @@ struct Place {
   int b, u, t, T;
 };
 // with `cost` > 0, x counts that many more tiles in front of each unit (t < 0 there)
-__device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int64_t x, int cost) {
+__device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int x, int cost) {
   int lo = 0, hi = batch;  // the last sequence that starts at or before x
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((int64_t(P[mid]) + int64_t(mid) * cost) * hr <= x)
+    if ((P[mid] + mid * cost) * hr <= x)
       lo = mid;
     else
       hi = mid;
@@ -104,36 +108,42 @@ __device__ __forceinline__ Place place_of(const int* P, int batch, int hr, int64
   Place r;
   r.b = lo;
   r.T = P[lo + 1] - P[lo];
-  const int64_t rem = x - (int64_t(P[lo]) + int64_t(lo) * cost) * hr;
-  r.u = int(rem / (r.T + cost));
-  r.t = int(rem - int64_t(r.u) * (r.T + cost)) - cost;
+  const unsigned rem = x - (P[lo] + lo * cost) * hr, each = r.T + cost;
+  r.u = rem / each;
+  r.t = int(rem - r.u * each) - cost;
   return r;
 }
 // the first tile of CTA i's range; short lines go to fewer CTAs
-__device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, int ctas, const KvSplit& sp) {
-  const int cost = sp.cost, snap = sp.snap, least = sp.least;
-  const int64_t total = (int64_t(P[batch]) + int64_t(batch) * cost) * hr;
-  ctas = int(min(int64_t(ctas), (total + least - 1) / least));
+__device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, const KvSplit& sp) {
+  const unsigned total = (P[batch] + batch * sp.cost) * hr;
+  const unsigned ctas = min(unsigned(sp.ctas), (total + sp.least - 1) / sp.least);
   if (i <= 0) return 0;
-  if (i >= ctas) return P[batch] * hr;
-  const Place a = place_of(P, batch, hr, total * i / ctas, cost);
-  const int d = min(snap, a.T / 2);
+  if (i >= int(ctas)) return P[batch] * hr;
+  const unsigned q = total / ctas, rest = total - q * ctas;
+  const Place a = place_of(P, batch, hr, q * i + rest * i / ctas, sp.cost);
+  const int d = min(sp.snap, a.T / 2);
   const int t = a.t <= d ? 0 : a.T - a.t <= d ? a.T : a.t;
   return P[a.b] * hr + a.u * a.T + t;
 }
 
-// this CTA's range [first, first + n) of the line, noted down for the join
-__device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const KvSplit& sp, int& first) {
-  const int hr = p.n_kv * sp.row_blocks, i = blockIdx.x;
-  first = cut(P, p.batch, hr, i, sp.ctas, sp);
-  const int end = cut(P, p.batch, hr, i + 1, sp.ctas, sp);
-  if (threadIdx.x == 0) {
-    const Place a = place_of(P, p.batch, hr, min(first, P[p.batch] * hr - 1), 0);
-    sp.places[i] = make_int4(a.b, a.u, a.t, a.T);
-    sp.cuts[i] = first;
-    if (i == sp.ctas - 1) sp.cuts[i + 1] = end;
+// this CTA's range [first, first + n) of the line, noted down for the join; ends[2] in shared memory. All
+// threads call it, a warp for either end.
+__device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const KvSplit& sp, int* ends, int& first) {
+  const int hr = p.n_kv * sp.row_blocks, i = blockIdx.x, tid = threadIdx.x;
+  if (tid == 0 || tid == 32) {
+    const int x = cut(P, p.batch, hr, i + (tid >> 5), sp);
+    ends[tid >> 5] = x;
+    if (tid == 0) {
+      const Place a = place_of(P, p.batch, hr, min(x, P[p.batch] * hr - 1), 0);
+      sp.places[i] = make_int4(a.b, a.u, a.t, a.T);
+      sp.cuts[i] = x;
+    } else if (i == sp.ctas - 1) {
+      sp.cuts[i + 1] = x;
+    }
   }
-  return end - first;
+  __syncthreads();
+  first = ends[0];
+  return ends[1] - first;
 }
 
 __device__ __forceinline__ float ex2(float x) {

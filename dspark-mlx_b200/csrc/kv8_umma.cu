@@ -12,7 +12,7 @@
 // set, plus one; it is set again when a weight would pass 2^8.75, and the sums in tensor memory are then
 // rescaled. The page's value exponent is folded into the weights relative to a reference rv that moves
 // when an exponent leaves [rv - 10, rv]; the scores' page factor is one per thread. Scores, sums and weights'
-// sums are fp32. The block's own rows take fp32 products on CUDA cores: they are few.
+// sums are fp32. The block's own rows are a unit's first step, in two e4m3 terms per row like q.
 //
 // What bounds it: reading 2 * head_dim bytes per key and KV head. At the copy peak an SM gets 128 keys of
 // head_dim 128 per ~1400 cycles; their products take ~300 cycles of the tensor cores for 32 rows, the
@@ -21,12 +21,15 @@
 // need 1,700 unrolled instructions per 64 keys and 32 rows, which the instruction cache does not hold
 // (measured: 116 us for 131,071 keys x 8 heads x 20 rows, against 41 us for the bytes).
 //
-// Layout. Two CTAs per SM (one at head_dim 256), each over its range of the line of units (kv8_attn.cuh),
-// 128 keys a step:
-//   warps 0-3  softmax: thread = key for the weights, thread = column for the result
-//   warp 4     producer: pages from the block table, 64 keys each; bulk copies (keys of head_dim 128,
-//              stored in the operand's 128-byte swizzle) and TMA boxes (the rest, swizzled on the way)
-//   warp 5     one thread issues the products: scores of step i + 1 before the sums of step i
+// Layout. Two CTAs per SM (one at head_dim 256 or 64 rows), each over its range of the line of units
+// (kv8_attn.cuh), 128 keys a step:
+//   softmax groups  of four warps, 16 query rows each and independent of one another: thread = key for the
+//                   weights, thread = column for the result. Four warps with 32 rows took 3,300 cycles a step at
+//                   two CTAs per SM, most of it waiting for their own results
+//   producer warp   pages from the block table, 64 keys each; bulk copies (keys of head_dim 128, stored
+//                   in the operand's 128-byte swizzle) and TMA boxes (the rest, swizzled on the way)
+//   product warp    one thread issues the products: scores of step i + 1 before the sums of step i
+// Code that runs once per unit is kept short: a CTA meets it with a cold instruction cache.
 #include <algorithm>
 #include <mutex>
 
@@ -38,53 +41,53 @@ namespace {
 
 using B16 = __nv_bfloat16;
 
-constexpr int kThreads = 192;
 constexpr int kStepKeys = 128;
-constexpr float kPExp = 8.f;   // weights at the reference: 2^8
+constexpr int kGroupRows = 16;  // query rows of a softmax group
+constexpr float kPExp = 8.f;    // weights at the reference: 2^8
 constexpr float kPMax = 8.75f;  // 2^8.75 = 431 still fits e4m3
-constexpr float kPHead = 1.f;  // a new reference lies this much above the maximum
+constexpr float kPHead = 1.f;   // a new reference lies this much above the maximum
 
-__host__ __device__ constexpr int mma_cols(int nr) { return nr <= 16 ? 16 : nr <= 32 ? 32 : 64; }
-__host__ __device__ constexpr int weight_buffers(int nr) { return nr > 32 ? 1 : 2; }
-
-template <int HD, int NR>
+template <int HD, int NR>  // NR query rows per CTA: 4, 8, 16, 32 or 64
 struct Cfg {
-  static constexpr int NM = mma_cols(NR);               // columns of the products
-  static constexpr int NH = HD <= 128 ? 1 : 2;          // 128-row halves of the output
-  static constexpr int CTAS = HD == 256 ? 1 : 2;        // per SM
-  static constexpr int PB = weight_buffers(NR);         // buffers of weights
-  static constexpr int kHalf = kTile * HD;              // bytes of 64 keys, or of their values
-  static constexpr int kStage = 4 * kHalf;              // keys, then values, of 128
-  static constexpr int kQTerm = NM * HD;                // bytes of one term of q
-  static constexpr int kPTerm = NM * kStepKeys;         // bytes of one term of the weights
-  static constexpr int kCols = 2 * NM + NH * NM;        // tensor memory: two score buffers, the sums
+  static constexpr int NM = NR < 16 ? 16 : NR;  // columns of the products
+  static constexpr int G = NM / kGroupRows;     // softmax groups
+  static constexpr int RW = NR < 16 ? NR : 16;  // rows that a group computes
+  static constexpr int NH = HD <= 128 ? 1 : 2;  // 128-row halves of the output
+  static constexpr int CTAS = HD == 256 || NM == 64 ? 1 : 2;  // per SM
+  static constexpr int kSoftmax = 128 * G;                    // threads
+  static constexpr int kThreads = kSoftmax + 64;
+  static constexpr int kHalf = kTile * HD;       // bytes of 64 keys, or of their values
+  static constexpr int kSlot = 2 * kHalf;        // a step's keys, or its values
+  static constexpr int kQTerm = NM * HD;         // bytes of one term of q
+  static constexpr int kPTerm = NM * kStepKeys;  // bytes of one term of the weights; two buffers of two
+  static constexpr int kCols = 2 * NM + NH * NM; // tensor memory: two score buffers, the sums
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
 };
 
 struct UmmaPlan {
   KvSplit sp;
-  int stages;
+  int k_slots, v_slots;  // steps' keys and values in shared memory: keys are done with earlier
   bool vec_q, vec_blk;
 };
 
 struct UmmaSmem {
-  int q, p, w, rows, info, bars, sums, P, bytes;
+  int q, p, rows, keys, info, bars, sums, P, bytes;
 };
-// per row: c (score factor), m (reference), a (rescaling), mb / lb (the block's maximum and weight), and four
-// warps' partial results
-constexpr int kRowFloats = 9;
-__host__ __device__ inline UmmaSmem umma_smem(int hd, int nr, int stages, int block, int batch) {
+// per row: c (score factor), m (less its reference), a (rescaling), where its result goes, and four warps' partial
+// results
+constexpr int kRowFloats = 8;
+constexpr int kInfos = 8;  // steps whose scales are noted down: more than there are slots
+constexpr int kMaxSlots = 6;
+__host__ __device__ inline UmmaSmem umma_smem(int hd, int nm, int slots, int batch) {
   UmmaSmem s;
-  const int nm = mma_cols(nr), pb = weight_buffers(nr);
-  s.q = stages * 4 * kTile * hd;
+  s.q = slots * 2 * kTile * hd;
   s.p = s.q + 2 * nm * hd;
-  s.w = s.p + pb * 2 * nm * kStepKeys;
-  s.rows = s.w + block * nr * 4;
-  s.info = s.rows + kRowFloats * nr * 4;
-  s.info = (s.info + 15) / 16 * 16;
-  s.bars = s.info + stages * 16;
-  s.sums = s.bars + (2 * stages + 10) * 8;
-  s.P = s.sums + 64;
+  s.rows = s.p + 4 * nm * kStepKeys;
+  s.keys = s.rows + kRowFloats * nm * 4;  // the block's rows: key scale and value exponent
+  s.info = s.keys + kUmmaMaxBlock * 8;
+  s.bars = s.info + kInfos * 16;
+  s.sums = s.bars + (4 * kMaxSlots + 2 * kInfos + 10) * 8;
+  s.P = s.sums + 128;
   s.bytes = 1024 + s.P + (batch + 1) * 4;  // the start is moved to 1024 bytes
   return s;
 }
@@ -149,16 +152,32 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, float* x) {
     for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
   }
 }
-__device__ __forceinline__ bool any_of_softmax(bool x) {  // over the four softmax warps, with a barrier
+// Wait for a phase, for a bounded number of tries (each suspends for a while in the hardware). Short on
+// purpose, and no call: it stands in loops that keep their registers.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  uint32_t tries = 0;
+  while (!mbar_try_wait(bar, parity))
+    if (++tries == 1u << 24) {
+      raise_device_error(DSM_DEV_ERR_PIPELINE_TIMEOUT);
+      return false;
+    }
+  return true;
+}
+// barriers of one softmax group (id 1 + group), and of all of them (id 8)
+__device__ __forceinline__ bool any_of_group(int group, bool x) {
   uint32_t r;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
       : "=r"(r)
-      : "r"(x ? 1u : 0u)
+      : "r"(group + 1), "r"(x ? 1u : 0u)
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void group_sync(int group) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(group + 1) : "memory"); }
+template <int N>
+__device__ __forceinline__ void softmax_sync() {
+  asm volatile("barrier.cta.sync 8, %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ float redux_max(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -234,61 +253,83 @@ __device__ __forceinline__ void q_terms(const float* x, uint32_t& hi, uint32_t& 
 struct Segment {
   Place un;
   int t0, t1, steps, g, r0, n_rows, len;
-  bool last, whole;
+  bool whole, blk;  // all of the unit; the block's own rows come first, as a step more
 };
 
 template <int HD, int NR>
-__global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
+__global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
     kv8_umma_kernel(const AttnArgs p, const UmmaPlan pl, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<HD, NR>;
-  constexpr int NM = C::NM;
+  constexpr int NM = C::NM, RW = C::RW, kProducer = 4 * C::G, kProduct = kProducer + 1;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  const UmmaSmem L = umma_smem(HD, NR, pl.stages, p.blk_k ? p.block : 0, p.batch);
-  const int S = pl.stages;
-  float* W = reinterpret_cast<float*>(smem + L.w);  // [block][NR] weights of the block's own rows
+  const int KN = pl.k_slots, VN = pl.v_slots;
+  const UmmaSmem L = umma_smem(HD, NM, KN + VN, p.batch);
+  uint8_t* const v_slots = smem + KN * C::kSlot;
   float* row_c = reinterpret_cast<float*>(smem + L.rows);
-  float* row_m = row_c + NR;
-  float* row_a = row_m + NR;
-  float* row_mb = row_a + NR;
-  float* row_lb = row_mb + NR;
-  float* red = row_lb + NR;  // [4][NR]
-  float4* info = reinterpret_cast<float4*>(smem + L.info);  // per stage: key and value scale of each half
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
-  uint64_t* empty = full + S;
-  uint64_t* s_full = empty + S;    // [2]
-  uint64_t* s_empty = s_full + 2;  // [2]
-  uint64_t* p_full = s_empty + 2;  // [2]
-  uint64_t* p_empty = p_full + 2;  // [2]
+  float* row_m = row_c + NM;
+  float* row_a = row_m + NM;
+  int* row_out = reinterpret_cast<int*>(row_a + NM);
+  float* const reds = row_a + 2 * NM;  // [group][4 warps][16]
+  float2* keys = reinterpret_cast<float2*>(smem + L.keys);
+  float4* info = reinterpret_cast<float4*>(smem + L.info);  // per step: key and value scale of each half
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L.bars);
+  uint64_t* k_empty = k_full + kMaxSlots;
+  uint64_t* v_full = k_empty + kMaxSlots;
+  uint64_t* v_empty = v_full + kMaxSlots;
+  uint64_t* i_full = v_empty + kMaxSlots;  // [kInfos]
+  uint64_t* granted = i_full + kInfos;     // [kInfos]: a step's slots wait for the block's own rows
+  uint64_t* s_full = granted + kInfos;     // [2]
+  uint64_t* s_empty = s_full + 2;          // [2]
+  uint64_t* p_full = s_empty + 2;          // [2]
+  uint64_t* p_empty = p_full + 2;          // [2]
   uint64_t* q_full = p_empty + 2;
   uint64_t* o_full = q_full + 1;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L.sums + 32);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L.sums + 112);
   int* P = reinterpret_cast<int*>(smem + L.P);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hr = p.n_kv * pl.sp.row_blocks;
-  if (tid == 0) {
-    for (int i = 0; i < S; ++i) {
-      mbar_init(full + i, 2);  // the copies' expect_tx, and the scales
-      mbar_init(empty + i, 1);
+  // translations that the first loads from each of these would wait for
+  if (tid < 8) {
+    const void* at = tid == 0   ? p.q
+                     : tid == 1 ? p.blk_k
+                     : tid == 2 ? p.blk_v
+                     : tid == 3 ? static_cast<const void*>(p.table)
+                     : tid == 4 ? static_cast<const void*>(p.k_scale)
+                     : tid == 5 ? static_cast<const void*>(p.v_scale)
+                     : tid == 6 ? p.out
+                                : static_cast<const void*>(pl.sp.part);
+    if (at) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+  }
+  if (tid == 32) {
+    for (int i = 0; i < kMaxSlots; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
+    }
+    for (int i = 0; i < kInfos; ++i) {
+      mbar_init(i_full + i, 1);
+      mbar_init(granted + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, 4);
-      mbar_init(p_full + i, 4);
+      mbar_init(s_empty + i, 4 * C::G);
+      mbar_init(p_full + i, 4 * C::G);
       mbar_init(p_empty + i, 1);
     }
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 4 * C::G);
     mbar_init(o_full, 1);
     fence_mbar_init();
   }
-  if (warp == 5) tc::tmem_alloc(slot, C::kAlloc);
-  scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
+  if (warp == kProduct) tc::tmem_alloc(slot, C::kAlloc);
+  scan_tiles<C::kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
   int start;
-  const int n_tiles = my_range(p, P, pl.sp, start);
+  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 24, start);
   if (blockIdx.x == 0)
-    for (int b = tid; b < p.batch; b += kThreads)
+    for (int b = tid; b < p.batch; b += C::kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
   tc::tc_fence_before();
   __syncthreads();
@@ -300,24 +341,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
     s.un = place_of(P, p.batch, hr, start + a0, 0);
     s.t0 = s.un.t;
     s.t1 = min(s.un.T, s.un.t + n_tiles - a0);
-    s.last = s.t1 == s.un.T;
-    s.whole = s.last && s.t0 == 0;
+    s.blk = s.t1 == s.un.T && p.blk_k;
+    s.whole = s.t1 == s.un.T && s.t0 == 0;
     s.g = s.un.u / pl.sp.row_blocks;
-    s.r0 = (s.un.u % pl.sp.row_blocks) * NR;
+    s.r0 = (s.un.u - s.g * pl.sp.row_blocks) * NR;
     s.n_rows = min(NR, pl.sp.rows - s.r0);
     s.len = seq_len(p, s.un.b);
-    s.steps = s.len == 0 ? 0 : (s.t1 - s.t0 + 1) / 2;
+    s.steps = (s.len == 0 ? 0 : (s.t1 - s.t0 + 1) / 2) + s.blk;
     return s;
   };
   bool ok = true;  // no wait has run out; after one has, loops go through without waiting, copying or multiplying
 
-  if (warp == 4) {
+  if (warp == kProducer) {
     // ---------------------------------------------------------------- producer
+    const int per_page = p.page / kTile;
     int k = 0;  // steps so far
     for (int a0 = 0; a0 < n_tiles;) {
       const Segment sg = segment(a0);
       a0 += sg.t1 - sg.t0;
-      const int tiles = sg.steps == 0 ? 0 : sg.t1 - sg.t0;
+      const int tiles = sg.len == 0 ? 0 : sg.t1 - sg.t0;
+      if (sg.blk) {  // the softmax warps fill this step's slots
+        if (ok && k >= KN) ok = wait(k_empty + k % KN, (k / KN - 1) & 1);
+        if (ok && k >= VN) ok = wait(v_empty + k % VN, (k / VN - 1) & 1);
+        if (lane == 0 && ok) {
+          mbar_arrive(granted + k % kInfos);
+          mbar_arrive(i_full + k % kInfos);
+        }
+        ++k;
+      }
       for (int base = 0; base < tiles; base += 32) {
         // a lane per tile: its page, then its scales (used when the first copies are on their way)
         const int t = sg.t0 + base + lane;
@@ -335,45 +386,53 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
           vs = __ldg(p.v_scale + int64_t(pg) * p.n_kv + sg.g);
         }
         for (int i = 0; i < min(32, tiles - base); i += 2, ++k) {
-          const int st = k % S;
-          if (ok && k >= S) ok = mbar_wait(empty + st, (k / S - 1) & 1);
+          const int kn = k % KN, vn = k % VN;
           const int pg0 = __shfl_sync(0xffffffffu, pg, i), pg1 = __shfl_sync(0xffffffffu, pg, i + 1);
+          const int live = (pg0 >= 0) + (pg1 >= 0);
+          const int64_t ph0 = int64_t(max(pg0, 0)) * p.n_kv + sg.g, ph1 = int64_t(max(pg1, 0)) * p.n_kv + sg.g;
+          const int sub = (sg.t0 + base + i) % per_page, sub1 = sub + 1 == per_page ? 0 : sub + 1;
+          const int64_t group0 = ph0 * per_page + sub, group1 = ph1 * per_page + sub1;  // of 64 tokens
+          if (ok && k >= KN) ok = wait(k_empty + kn, (k / KN - 1) & 1);
           if (lane == 0 && ok) {
-            mbar_arrive_expect_tx(full + st, ((pg0 >= 0) + (pg1 >= 0)) * 2 * C::kHalf);
-            const uint32_t kdst = smem_u32(smem) + st * C::kStage, vdst = kdst + 2 * C::kHalf;
+            mbar_arrive_expect_tx(k_full + kn, live * C::kHalf);
+            uint8_t* const dst = smem + kn * C::kSlot;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int page = h ? pg1 : pg0;
-              if (page < 0) continue;
-              const int64_t ph = int64_t(page) * p.n_kv + sg.g;
-              const int sub = ((sg.t0 + base + i + h) * kTile % p.page) / kTile;
-              const int64_t group = ph * (p.page / kTile) + sub;  // of 64 tokens
+              if ((h ? pg1 : pg0) < 0) continue;
+              const int64_t g64 = h ? group1 : group0;
               if constexpr (HD == 128) {
-                bulk_g2s(smem + st * C::kStage + h * C::kHalf, p.k_codes + group * C::kHalf, C::kHalf, full + st,
-                         policy_evict_first());
+                bulk_g2s(dst + h * C::kHalf, p.k_codes + g64 * C::kHalf, C::kHalf, k_full + kn, policy_evict_first());
               } else if constexpr (HD == 64) {
-                tma_2d(kdst + h * C::kHalf, &kmap, 0, int(group * kTile), full + st);
+                tma_2d(smem_u32(dst) + h * C::kHalf, &kmap, 0, int(g64 * kTile), k_full + kn);
               } else {  // two slabs of 128 bytes
-                tma_2d(kdst + h * (C::kHalf / 2), &kmap, 0, int(group * kTile), full + st);
-                tma_2d(kdst + C::kHalf + h * (C::kHalf / 2), &kmap, 128, int(group * kTile), full + st);
+                tma_2d(smem_u32(dst) + h * (C::kHalf / 2), &kmap, 0, int(g64 * kTile), k_full + kn);
+                tma_2d(smem_u32(dst) + C::kHalf + h * (C::kHalf / 2), &kmap, 128, int(g64 * kTile), k_full + kn);
               }
-              tma_2d(vdst + h * C::kHalf, &vmap, 0, int(group * HD), full + st);
             }
+          }
+          if (ok && k >= VN) ok = wait(v_empty + vn, (k / VN - 1) & 1);
+          if (lane == 0 && ok) {
+            mbar_arrive_expect_tx(v_full + vn, live * C::kHalf);
+            const uint32_t dst = smem_u32(v_slots + vn * C::kSlot);
+            if (pg0 >= 0) tma_2d(dst, &vmap, 0, int(group0 * HD), v_full + vn);
+            if (pg1 >= 0) tma_2d(dst + C::kHalf, &vmap, 0, int(group1 * HD), v_full + vn);
           }
           const float4 sc = make_float4(__shfl_sync(0xffffffffu, ks, i), __shfl_sync(0xffffffffu, vs, i),
                                         __shfl_sync(0xffffffffu, ks, i + 1), __shfl_sync(0xffffffffu, vs, i + 1));
           if (lane == 0 && ok) {
-            info[st] = sc;
-            mbar_arrive(full + st);
+            info[k % kInfos] = sc;
+            mbar_arrive(i_full + k % kInfos);
           }
           __syncwarp();
         }
       }
     }
     // after a wait that ran out, copies may still be on their way: see them land
-    if (!ok)
-      for (int i = max(0, k - S); i < k; ++i) mbar_wait(full + i % S, (i / S) & 1);
-  } else if (warp == 5) {
+    if (!ok) {
+      for (int i = max(0, k - KN); i < k; ++i) wait(k_full + i % KN, (i / KN) & 1);
+      for (int i = max(0, k - VN); i < k; ++i) wait(v_full + i % VN, (i / VN) & 1);
+    }
+  } else if (warp == kProduct) {
     // ---------------------------------------------------------------- products
     if (lane == 0) {
       const uint32_t id_s = idesc_f8(NM, false, false), id_hi = idesc_f8(NM, false, true), id_lo = idesc_f8(NM, true, true);
@@ -383,48 +442,72 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         const Segment sg = segment(a0);
         a0 += sg.t1 - sg.t0;
         if (sg.steps == 0) continue;
-        if (ok) ok = mbar_wait(q_full, seg++ & 1);
+        if (ok) ok = wait(q_full, seg++ & 1);
         tc::tc_fence_after();
-        auto sums = [&](int j, bool first) {  // step j's
-          const int pb = C::PB == 2 ? j & 1 : 0, use = C::PB == 2 ? j >> 1 : j;
-          if (ok) ok = mbar_wait(p_full + pb, use & 1);
+        auto sums = [&](int j, bool first, bool blk) {  // step j's
+          const int pb = j & 1;
+          if (ok) ok = wait(v_full + j % VN, (j / VN) & 1);
           tc::tc_fence_after();
           if (!ok) return;
-          const uint32_t v = base + (j % S) * C::kStage + 2 * C::kHalf, w = pa + pb * 2 * C::kPTerm;
+          const uint32_t v = base + KN * C::kSlot + (j % VN) * C::kSlot, w = pa + pb * 2 * C::kPTerm;
+          // 32 keys a product
+          const uint64_t av = desc_sw64(v), bw = desc_weights<NM>(w);
+          if (!blk) {
 #pragma unroll
-          for (int nh = 0; nh < C::NH; ++nh)
+            for (int nh = 0; nh < C::NH; ++nh)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+              for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                umma_f8(t_o + nh * NM, desc_sw64(v + (ks >> 1) * C::kHalf + nh * 128 * 64 + (ks & 1) * 32),
-                        desc_weights<NM>(w + x * C::kPTerm + ks * 32 * NM), x ? id_lo : id_hi, !first || x > 0 || ks > 0);
-          tc::umma_commit(empty + j % S);
+                for (int ks = 0; ks < 4; ++ks)
+                  umma_f8(t_o + nh * NM, av + (((ks >> 1) * C::kHalf + nh * 128 * 64 + (ks & 1) * 32) >> 4),
+                          bw + ((x * C::kPTerm + ks * 32 * NM) >> 4), x ? id_lo : id_hi, !first || x > 0 || ks > 0);
+          } else {  // its values' two terms lie where others have keys 0-63 and 64-127
+            const int n = (p.block + 31) / 32;
+#pragma unroll 1
+            for (int i = 0; i < 4 * C::NH * n; ++i) {
+              const int ks = i % n, term = i / n & 1, x = i / n >> 1 & 1, nh = i / n >> 2;
+              umma_f8(t_o + nh * NM, av + ((term * C::kHalf + nh * 128 * 64 + ks * 32) >> 4),
+                      bw + ((x * C::kPTerm + ks * 32 * NM) >> 4), x ? id_lo : id_hi, !first || i % (4 * n) > 0);
+            }
+          }
+          tc::umma_commit(v_empty + j % VN);
           tc::umma_commit(p_empty + pb);
         };
-        for (int i = 0; i < sg.steps; ++i) {
-          const int kk = k + i, st = kk % S, sb = kk & 1;
-          if (ok) ok = mbar_wait(full + st, (kk / S) & 1);
-          if (ok && kk >= 2) ok = mbar_wait(s_empty + sb, ((kk >> 1) - 1) & 1);
-          tc::tc_fence_after();
-          if (ok) {
-            const uint32_t kt = base + st * C::kStage;
+        // step i's scores, step j's sums: whichever can go
+        uint32_t idle = 0;
+        for (int i = 0, j = 0; j < sg.steps && ok;) {
+          const int kk = k + i, sb = kk & 1, jj = k + j;
+          if (i < sg.steps && i < j + 2 && mbar_try_wait(k_full + kk % KN, (kk / KN) & 1) &&
+              (kk < 2 || mbar_try_wait(s_empty + sb, ((kk >> 1) - 1) & 1))) {
+            tc::tc_fence_after();
+            // the block's step: its keys' hi terms are rows 0-63, their lo terms rows 64-127, multiplied as
+            // rows 0-63 once more
+            const uint32_t kt = base + (kk % KN) * C::kSlot;
+            const uint64_t ak = HD == 64 ? desc_sw64(kt) : tc::umma_desc_sw128(kt);
+            const uint64_t bq = HD == 64 ? desc_sw64(qa) : tc::umma_desc_sw128(qa);
+#pragma unroll 1
+            for (int lo = 0; lo <= (sg.blk && i == 0); ++lo)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+              for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int ks = 0; ks < HD / 32; ++ks) {
-                const uint64_t a = HD == 64 ? desc_sw64(kt + ks * 32)
-                                            : tc::umma_desc_sw128(kt + (ks >> 2) * 2 * 64 * 128 + (ks & 3) * 32);
-                const uint32_t qt = qa + x * C::kQTerm;
-                const uint64_t b = HD == 64 ? desc_sw64(qt + ks * 32)
-                                            : tc::umma_desc_sw128(qt + (ks >> 2) * NM * 128 + (ks & 3) * 32);
-                umma_f8(tmem + sb * NM, a, b, id_s, x > 0 || ks > 0);
-              }
+                for (int ks = 0; ks < HD / 32; ++ks)
+                  umma_f8(tmem + sb * NM,
+                          ak + (((ks >> 2) * 2 * 64 * 128 + (ks & 3) * 32) >> 4) + lo * ((HD == 64 ? 64 * 64 : 64 * 128) >> 4),
+                          bq + ((x * C::kQTerm + (ks >> 2) * NM * 128 + (ks & 3) * 32) >> 4), id_s,
+                          lo > 0 || x > 0 || ks > 0);
             tc::umma_commit(s_full + sb);
+            tc::umma_commit(k_empty + kk % KN);
+            ++i;
+            idle = 0;
+          } else if (j < i && mbar_try_wait(p_full + (jj & 1), (jj >> 1) & 1)) {
+            sums(jj, j == 0, sg.blk && j == 0);
+            ++j;
+            idle = 0;
+          } else if (++idle == 1u << 24) {
+            raise_device_error(DSM_DEV_ERR_PIPELINE_TIMEOUT);
+            ok = false;
           }
-          if (i > 0) sums(kk - 1, i == 1);
         }
-        sums(k + sg.steps - 1, sg.steps == 1);
         if (ok) tc::umma_commit(o_full);
         k += sg.steps;
       }
@@ -432,48 +515,76 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, results
-    constexpr int TPR = 8, VB = HD / TPR;  // staging: 16 rows at a time, threads per row, values per thread
-    const int half = tid >> 6;             // which 64 keys of a step this thread's key is in
+    constexpr int TPR = 16, VB = HD / TPR, kPass = C::kSoftmax / TPR;  // staging: threads per row, values per thread
+    const int grp = C::G == 1 ? 0 : warp >> 2, gtid = C::G == 1 ? tid : tid & 127;
+    const int g0 = grp * kGroupRows;  // its first row
+    const int half = gtid >> 6;       // which 64 keys of a step this thread's key is in
     const int row_r = tid / TPR, row_d = tid % TPR * VB;
-    const uint32_t t_lane = uint32_t(warp * 32) << 16;
+    const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const int group = p.n_heads / p.n_kv;
+    float* const red = reds + grp * 4 * kGroupRows;
+    const float* const my_c = row_c + g0;
+    const float* const my_m = row_m + g0;
+    const float* const my_a = row_a + g0;
     uint8_t* const q8 = smem + L.q;
-    // where this thread's key's weights go, 16 rows at a time
-    uint32_t p_at[NM / 16];
-#pragma unroll
-    for (int c = 0; c < NM / 16; ++c)
-      p_at[c] = smem_u32(smem) + L.p + tid * NM + ((c ^ (NM == 32 ? (tid >> 2) & 1 : NM == 64 ? (tid >> 1) & 3 : 0)) << 4);
+    // where this thread's key's weights go, 16 rows
+    const uint32_t p_at = smem_u32(smem) + L.p + gtid * NM +
+                          ((grp ^ (NM == 32 ? (gtid >> 2) & 1 : NM == 64 ? (gtid >> 1) & 3 : 0)) << 4);
 
-    int k = 0, outs = 0;  // steps, and units with steps, so far
+    int k = 0, outs = 0;   // steps, and units with steps, so far
+    unsigned blocks = 0;  // per step modulo kInfos, whether an odd number of blocks' own rows has been granted
     for (int a0 = 0; a0 < n_tiles;) {
       const Segment sg = segment(a0);
-      const bool blk = sg.last && p.blk_k;
-      // ---- q's terms, and the scores of the block's own rows
-      softmax_sync();  // the previous unit's row statistics are used up
-      const B16* qg = static_cast<const B16*>(p.q) + sg.un.b * p.q_batch;
-      const B16* bk = static_cast<const B16*>(p.blk_k) + sg.un.b * p.bk_batch + sg.g * p.bk_head + row_d;
-      for (int r = row_r; r < NM; r += 16) {
-        float x[VB];
+      // ---- q's terms, and the block's own rows: 16 rows at a time, the next ones' loads ahead of this ones' work
+      softmax_sync<C::kSoftmax>();  // the previous unit's row statistics are used up
+      uint8_t* const kt = smem + (k % KN) * C::kSlot;
+      uint8_t* const vt = v_slots + (k % VN) * C::kSlot;
+      constexpr int kQPasses = NR <= kPass ? 1 : NR / kPass;
+      const int n_blk = sg.blk ? (p.block + kPass - 1) / kPass : 0, n_tasks = kQPasses + 2 * n_blk;
+      auto load_rows = [&](int task, float(&x)[VB]) {
+        const int j = task - kQPasses;
+        const bool of_v = j >= n_blk;
+        const int r = (j < 0 ? task : of_v ? j - n_blk : j) * kPass + row_r;
+        const B16* src;
+        if (j < 0) {
+          const int rr = sg.r0 + r, h = unsigned(rr) / unsigned(p.block);
+          src = static_cast<const B16*>(p.q) + sg.un.b * p.q_batch + (rr - h * p.block) * p.q_row +
+                (sg.g * group + h) * p.q_head;
+        } else {
+          src = of_v ? static_cast<const B16*>(p.blk_v) + sg.un.b * p.bv_batch + sg.g * p.bv_head + r * p.bv_row
+                     : static_cast<const B16*>(p.blk_k) + sg.un.b * p.bk_batch + sg.g * p.bk_head + r * p.bk_row;
+        }
 #pragma unroll
         for (int i = 0; i < VB; ++i) x[i] = 0.f;
-        const bool live = r < sg.n_rows;
-        if (live) {
-          const int rr = sg.r0 + r;
-          load_vals<B16, VB>(qg + (rr % p.block) * p.q_row + (sg.g * group + rr / p.block) * p.q_head + row_d, pl.vec_q, x);
+        if (r < (j < 0 ? sg.n_rows : p.block)) load_vals<B16, VB>(src + row_d, j < 0 ? pl.vec_q : pl.vec_blk, x);
+      };
+      float x[VB], x1[VB];
+      load_rows(0, x);
+      if (n_tasks > 1) load_rows(1, x1);
+      if (tid < NR) {  // where the row's result goes
+        const int rr = sg.r0 + tid, h = unsigned(rr) / unsigned(p.block);
+        row_out[tid] = ((rr - h * p.block) * p.n_heads + sg.g * group + h) * HD;
+      }
+      if (sg.blk) {
+        if (ok) ok = wait(granted + k % kInfos, blocks >> k % kInfos & 1);
+        blocks ^= 1u << k % kInfos;
+        // values: columns of 32 (64) keys, zero where there is no key
+        const int n = p.block > 32 ? 64 : 32, per = 2 * HD * n / 16;
+#pragma unroll 1
+        for (int i = tid; i < per; i += C::kSoftmax) {
+          const int t = i & 1, d = (i >> 1) % HD, c = (i >> 1) / HD;
+          *reinterpret_cast<uint4*>(vt + t * C::kHalf + d * 64 + ((c ^ ((d >> 1) & 3)) << 4)) = make_uint4(0, 0, 0, 0);
         }
-        if (blk && r < NR) {
-          const float f = p.scale * kLog2e;
-#pragma unroll 2
-          for (int j = 0; j < p.block; ++j) {
-            float y[VB], s = 0.f;
-            load_vals<B16, VB>(bk + j * p.bk_row, pl.vec_blk, y);
-#pragma unroll
-            for (int i = 0; i < VB; ++i) s = fmaf(x[i], y[i], s);
-#pragma unroll
-            for (int w = TPR / 2; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-            if (row_d == 0) W[j * NR + r] = live ? s * f : 0.f;
-          }
-        }
+        softmax_sync<C::kSoftmax>();
+      }
+#pragma unroll 1
+      for (int task = 0; task < n_tasks; ++task) {
+        float x2[VB];  // two rows ahead
+        if (task + 2 < n_tasks) load_rows(task + 2, x2);
+        const int j = task - kQPasses;
+        const bool of_q = j < 0, of_v = j >= n_blk;
+        const int r = (of_q ? task : of_v ? j - n_blk : j) * kPass + row_r;
+        // scaled by a power of two to at most 448
         float mx = 0.f;
 #pragma unroll
         for (int i = 0; i < VB; ++i) mx = fmaxf(mx, finite_abs(x[i]));
@@ -481,61 +592,97 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         for (int w = TPR / 2; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
         const int e = kv8_scale_exp(mx);
         const float inv = kv8_exp2i(-e);
-#pragma unroll
-        for (int i = 0; i < VB; ++i) x[i] = scaled(x[i], inv);
-        if (row_d == 0 && r < NR) {
-          row_c[r] = live ? p.scale * kLog2e * kv8_exp2i(e) : 0.f;
-          row_m[r] = 0.f;
+        if (row_d == 0) {
+          if (of_q && r < NM) {
+            row_c[r] = r < sg.n_rows ? p.scale * kLog2e * kv8_exp2i(e) : 0.f;
+            row_m[r] = 0.f;
+          } else if (!of_q && r < p.block) {
+            if (of_v)
+              keys[r].y = float(e);
+            else
+              keys[r].x = kv8_exp2i(e);
+          }
         }
+        // rows of q and of keys: K-major in the swizzle of their width; of values: bytes of its columns
+        uint8_t* const at = of_q ? q8 : kt;
+        const int rows = of_q ? NM : 128, term = of_q ? C::kQTerm : HD == 64 ? 64 * 64 : 64 * 128;
 #pragma unroll
         for (int i = 0; i < VB; i += 4) {
-          uint32_t hi, lo;
-          q_terms(x + i, hi, lo);
+          float y[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) y[w] = scaled(x[i + w], inv);
+          uint32_t t[2];
+          q_terms(y, t[0], t[1]);
           const int d = row_d + i;
-          uint8_t* at = HD == 64 ? q8 + r * 64 + ((((d >> 4) & 3) ^ ((r >> 1) & 3)) << 4) + (d & 15)
-                                 : q8 + (d >> 7) * NM * 128 + r * 128 + ((((d >> 4) & 7) ^ (r & 7)) << 4) + (d & 15);
-          *reinterpret_cast<uint32_t*>(at) = hi;
-          *reinterpret_cast<uint32_t*>(at + C::kQTerm) = lo;
+          if (of_v) {
+            if (r < p.block) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                uint8_t* b = vt + (d + w) * 64 + (((r >> 4) ^ (((d + w) >> 1) & 3)) << 4) + (r & 15);
+                b[0] = uint8_t(t[0] >> (8 * w));
+                b[C::kHalf] = uint8_t(t[1] >> (8 * w));
+              }
+            }
+          } else if (r < (of_q ? NM : kTile)) {
+            uint8_t* b = HD == 64 ? at + r * 64 + ((((d >> 4) & 3) ^ ((r >> 1) & 3)) << 4) + (d & 15)
+                                  : at + (d >> 7) * rows * 128 + r * 128 + ((((d >> 4) & 7) ^ (r & 7)) << 4) + (d & 15);
+            *reinterpret_cast<uint32_t*>(b) = t[0];
+            *reinterpret_cast<uint32_t*>(b + term) = t[1];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+          x[i] = x1[i];
+          x1[i] = x2[i];
         }
       }
       tc::fence_async_smem();
-      softmax_sync();
+      softmax_sync<C::kSoftmax>();
       if (lane == 0 && sg.steps > 0) mbar_arrive(q_full);
-      if (blk && tid < NR) {  // the block's weights of row tid, relative to their maximum
-        float mb = kLowest, lb = 0.f;
-        for (int j = 0; j < p.block; ++j) mb = fmaxf(mb, W[j * NR + tid]);
-        for (int j = 0; j < p.block; ++j) {
-          const float w = ex2(W[j * NR + tid] - mb);
-          W[j * NR + tid] = w;
-          lb += w;
-        }
-        row_mb[tid] = mb;
-        row_lb[tid] = lb;
+      if (sg.blk && tid == 0) {
+        mbar_arrive(k_full + k % KN);
+        mbar_arrive(v_full + k % VN);
       }
 
       // ---- the cached rows, 128 a step
-      float l[NR];
+      float l[RW];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) l[r] = 0.f;
+      for (int r = 0; r < RW; ++r) l[r] = 0.f;
       int rv = -200, top_rv = -200;
       for (int i = 0; i < sg.steps; ++i, ++k) {
-        const int st = k % S, sb = k & 1;
-        if (ok) ok = mbar_wait(full + st, (k / S) & 1);
-        const float4 sc = info[st];
-        const int t0 = sg.t0 + 2 * i;  // first tile of the step
-        const int left = sg.len - t0 * kTile;
-        const int n0 = sc.x == sc.x ? max(0, min(kTile, left)) : 0;
-        const int n1 = t0 + 1 < sg.t1 && sc.z == sc.z ? max(0, min(kTile, left - kTile)) : 0;
-        const bool live = (tid & 63) < (half ? n1 : n0);
-        const float ks = half ? sc.z : sc.x;
-        const int e0 = n0 ? kv8_exponent(sc.y) : -200, e1 = n1 ? kv8_exponent(sc.w) : -200;
-        const int ev = max(e0, e1), low = min(n0 ? e0 : ev, n1 ? e1 : ev);
+        const int sb = k & 1;
+        if (ok) ok = wait(i_full + k % kInfos, (k / kInfos) & 1);
+        const bool own = sg.blk && i == 0;  // the block's own rows: key = thread, a scale each
+        int n0 = 0, n1 = 0, e_key = -200, ev = -200, low = 200;
+        float ks = 0.f;
+        bool live;
+        if (own) {
+          for (int j = 0; j < p.block; ++j) ev = max(ev, int(keys[j].y));
+          low = ev;
+          live = gtid < p.block;
+          if (live) {
+            ks = keys[gtid].x;
+            e_key = int(keys[gtid].y);
+          }
+        } else {
+          const float4 sc = info[k % kInfos];
+          const int t0 = sg.t0 + 2 * (i - sg.blk);  // first tile of the step
+          const int left = sg.len - t0 * kTile;
+          n0 = sc.x == sc.x ? max(0, min(kTile, left)) : 0;
+          n1 = t0 + 1 < sg.t1 && sc.z == sc.z ? max(0, min(kTile, left - kTile)) : 0;
+          live = (gtid & 63) < (half ? n1 : n0);
+          ks = half ? sc.z : sc.x;
+          const int e0 = n0 ? kv8_exponent(sc.y) : -200, e1 = n1 ? kv8_exponent(sc.w) : -200;
+          e_key = half ? e1 : e0;
+          ev = max(e0, e1);
+          low = min(n0 ? e0 : ev, n1 ? e1 : ev);
+        }
         top_rv = max(top_rv, ev);
         const int want_rv = ev > rv || low < rv - 10 ? max(ev, top_rv - 40) : rv;
-        if (ok) ok = mbar_wait(s_full + sb, (k >> 1) & 1);
+        if (ok) ok = wait(s_full + sb, (k >> 1) & 1);
         tc::tc_fence_after();
-        float y[NR];
-        tmem_ld<NR>(tmem + t_lane + sb * NM, y);
+        float y[RW];
+        tmem_ld<RW>(tmem + t_lane + sb * NM + g0, y);
         tc::tmem_ld_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -543,8 +690,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
         // the weights' exponents: row_m is kPExp less the reference
         float top = kLowest;
 #pragma unroll
-        for (int r = 0; r < NR; r += 4) {
-          const float4 c = *reinterpret_cast<const float4*>(row_c + r), m = *reinterpret_cast<const float4*>(row_m + r);
+        for (int r = 0; r < RW; r += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(my_c + r), m = *reinterpret_cast<const float4*>(my_m + r);
           const float2 ks2 = make_float2(ks, ks);
           const float2 a = fma2(make_float2(y[r], y[r + 1]), mul2(make_float2(c.x, c.y), ks2), make_float2(m.x, m.y));
           const float2 b = fma2(make_float2(y[r + 2], y[r + 3]), mul2(make_float2(c.z, c.w), ks2), make_float2(m.z, m.w));
@@ -554,92 +701,88 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
           y[r + 3] = b.y;
           top = fmaxf(top, fmaxf(fmaxf(y[r], y[r + 1]), fmaxf(y[r + 2], y[r + 3])));
         }
-        if (any_of_softmax((live && top > kPMax) || i == 0 || want_rv != rv)) {
+        if (any_of_group(grp, (live && top > kPMax) || i == 0 || want_rv != rv)) {
           // new references: every row whose maximum lies above its own (all of them at first)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
+          for (int r = 0; r < RW; ++r) {
             const float x = redux_max(live ? y[r] : kLowest);
-            if (lane == (r & 31)) red[warp * NR + r] = x;
+            if (lane == r) red[(warp & 3) * kGroupRows + r] = x;
           }
-          softmax_sync();
-          if (tid < NR) {
-            const float x = fmaxf(fmaxf(red[tid], red[NR + tid]), fmaxf(red[2 * NR + tid], red[3 * NR + tid]));
+          group_sync(grp);
+          if (gtid < RW) {
+            const float x = fmaxf(fmaxf(red[gtid], red[16 + gtid]), fmaxf(red[32 + gtid], red[48 + gtid]));
             const float up = x == kLowest ? 0.f : i == 0 || x > kPExp ? x + (kPHead - kPExp) : 0.f;
-            row_m[tid] -= up;
-            red[tid] = up;
+            row_m[g0 + gtid] -= up;
+            red[gtid] = up;
             const float fv = rv <= -200 ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
-            row_a[tid] = ex2(-up) * fv;
+            row_a[g0 + gtid] = ex2(-up) * fv;
           }
-          softmax_sync();
+          group_sync(grp);
           rv = want_rv;
           if (i > 0) {  // the sums so far, after the products that make them
-            const int j = k - 1, pb = C::PB == 2 ? j & 1 : 0, use = C::PB == 2 ? j >> 1 : j;
-            if (ok) ok = mbar_wait(p_empty + pb, use & 1);
+            const int j = k - 1;
+            if (ok) ok = wait(p_empty + (j & 1), (j >> 1) & 1);
             tc::tc_fence_after();
-#pragma unroll
-            for (int nh = 0; nh < C::NH; ++nh)
 #pragma unroll 1
-              for (int c = 0; c < NM && c < NR; c += 8) {
-                float o[8];
-                uint32_t u[8];
-                const uint32_t at = t_o + t_lane + nh * NM + c;
-                tmem_ld<8>(at, o);
-                tc::tmem_ld_wait();
-#pragma unroll
-                for (int x = 0; x < 8; ++x) u[x] = __float_as_uint(o[x] * row_a[c + x]);
-                asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(u[0]),
-                             "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
-                             : "memory");
-              }
+            for (int c = 0; c < C::NH * RW; c += 4) {
+              const int at_r = C::NH == 1 ? c : c % RW;
+              float o[4];
+              const uint32_t at = t_o + t_lane + (C::NH == 1 ? 0 : c / RW * NM) + g0 + at_r;
+              tmem_ld<4>(at, o);
+              tc::tmem_ld_wait();
+              const float4 a = *reinterpret_cast<const float4*>(my_a + at_r);
+              asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at),
+                           "r"(__float_as_uint(o[0] * a.x)), "r"(__float_as_uint(o[1] * a.y)),
+                           "r"(__float_as_uint(o[2] * a.z)), "r"(__float_as_uint(o[3] * a.w))
+                           : "memory");
+            }
             tc::tmem_st_wait();
           }
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
+          for (int r = 0; r < RW; ++r) {
             const float up = red[r];
             if (i > 0) l[r] *= ex2(-up);
             y[r] -= up;
           }
         }
-        const int dv = max((half ? e1 : e0) - rv, -60);  // <= 0
+        const int dv = max(e_key - rv, -60);  // <= 0
         const float fv = kv8_exp2i(dv);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) y[r] = ex2(y[r]);
+        for (int r = 0; r < RW; ++r) y[r] = ex2(y[r]);
         if (!__all_sync(0xffffffffu, live)) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) y[r] = live ? y[r] : 0.f;
+          for (int r = 0; r < RW; ++r) y[r] = live ? y[r] : 0.f;
         }
 #pragma unroll
-        for (int r = 0; r < NR; r += 2) {
+        for (int r = 0; r < RW; r += 2) {
           const float2 a = add2(make_float2(l[r], l[r + 1]), make_float2(y[r], y[r + 1]));
           l[r] = a.x;
           l[r + 1] = a.y;
         }
-        if (dv != 0) {
+        if (__any_sync(0xffffffffu, dv != 0)) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) y[r] *= fv;
+          for (int r = 0; r < RW; ++r) y[r] *= fv;
         }
-        const int pb = C::PB == 2 ? k & 1 : 0, use = C::PB == 2 ? k >> 1 : k;
-        if (ok && use > 0) ok = mbar_wait(p_empty + pb, (use - 1) & 1);
-#pragma unroll
-        for (int r = 0; r < NR; r += 16) {
-          constexpr int kWords = NR < 16 ? NR / 4 : 4;
+        const int pb = k & 1;
+        if (ok && k >= 2) ok = wait(p_empty + pb, ((k >> 1) - 1) & 1);
+        {
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int w = 0; w < kWords; ++w)
-            if (r + 4 * w < NR) weight_terms(y[r + 4 * w], y[r + 4 * w + 1], y[r + 4 * w + 2], y[r + 4 * w + 3], hi[w], lo[w]);
-          const uint32_t at = p_at[r / 16] + pb * 2 * C::kPTerm;
-          store_words(at, hi, min(4, (NR - r) / 4));
-          store_words(at + C::kPTerm, lo, min(4, (NR - r) / 4));
+          for (int w = 0; w < RW / 4; ++w) weight_terms(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3], hi[w], lo[w]);
+          const uint32_t at = p_at + pb * 2 * C::kPTerm;
+          store_words(at, hi, RW / 4);
+          store_words(at + C::kPTerm, lo, RW / 4);
         }
         // value codes without a key (behind the length, or of a page that is none) are cleared: a weight of
         // zero would not take a NaN there out
-        if (n0 < kTile || n1 < kTile) {
-#pragma unroll
+        if (!own && (n0 < kTile || n1 < kTile)) {
+          if (ok) ok = wait(v_full + k % VN, (k / VN) & 1);
+#pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             const int n = h ? n1 : n0;
-            uint8_t* v = smem + st * C::kStage + 2 * C::kHalf + h * C::kHalf;
-            for (int d = tid; d < HD; d += 128)
-#pragma unroll
+            uint8_t* v = v_slots + (k % VN) * C::kSlot + h * C::kHalf;
+            for (int d = tid; d < HD; d += C::kSoftmax)
+#pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 const int keep = n - c * 16;
                 if (keep >= 16) continue;
@@ -662,109 +805,67 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
       }
 
       // ---- the unit's result: l over all keys, then thread = column
-      if (sg.steps > 0) {
-        softmax_sync();  // every warp is done with `red`
-        // halves of the rows change hands until a lane holds one row's (two rows') sum over the warp
-        constexpr int NP = NR <= 4 ? 4 : NR <= 8 ? 8 : NR <= 16 ? 16 : NR <= 32 ? 32 : 64;
-        float x[NP];
-#pragma unroll
-        for (int r = 0; r < NP; ++r) x[r] = r < NR ? l[r] : 0.f;
-        int n = NP;
+      group_sync(grp);  // every warp is done with `red`
+      {
+        // halves of the rows change hands until a lane holds one row's sum over the warp
+        int n = RW;
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) {
           if (n > 1) {
             n /= 2;
 #pragma unroll
-            for (int r = 0; r < NP / 2; ++r)
+            for (int r = 0; r < RW / 2; ++r)
               if (r < n) {
-                const float give = (lane & off) ? x[r] : x[r + n];
-                const float keep = (lane & off) ? x[r + n] : x[r];
-                x[r] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+                const float give = (lane & off) ? l[r] : l[r + n];
+                const float keep = (lane & off) ? l[r + n] : l[r];
+                l[r] = keep + __shfl_xor_sync(0xffffffffu, give, off);
               }
           } else {
-            x[0] += __shfl_xor_sync(0xffffffffu, x[0], off);
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
           }
         }
-        if constexpr (NP == 64) {
-          if (2 * lane < NR) {
-            red[warp * NR + 2 * lane] = x[0];
-            red[warp * NR + 2 * lane + 1] = x[1];
-          }
-        } else {
-          constexpr int per = 32 / NP;  // lanes that hold the same row
-          if (lane % per == 0 && lane / per < NR) red[warp * NR + lane / per] = x[0];
-        }
+        constexpr int per = 32 / RW;  // lanes that hold the same row
+        if (lane % per == 0) red[(warp & 3) * kGroupRows + lane / per] = l[0];
       }
-      softmax_sync();
-      if (tid < NR) {
-        // o and l are relative to row_m, o in units of 2^rv; the block's to mb
-        const bool ctx = sg.steps > 0;
-        const float lc = ctx ? red[tid] + red[NR + tid] + red[2 * NR + tid] + red[3 * NR + tid] : 0.f;
-        const float m = lc == 0.f ? -INFINITY : -row_m[tid], mb = blk ? row_mb[tid] : -INFINITY;
-        const float M = fmaxf(m, mb), ref = M == -INFINITY ? 0.f : M;
-        const float fa = ex2(m - ref), fb = blk ? ex2(mb - ref) : 0.f;
-        const float den = lc * fa + (blk ? row_lb[tid] * fb : 0.f);
-        if (sg.whole) {
-          const float inv = den == 0.f ? 0.f : 1.f / den;
-          row_a[tid] = fa * inv * (rv <= -200 ? 0.f : kv8_exp2i(min(max(rv, -126), 126)));
-          row_mb[tid] = fb * inv;
-        } else {  // parts are in units of 2^E, E >= rv, and E >= 0 with the block's own rows in them
-          const float E = blk ? fmaxf(float(rv), 0.f) : float(rv);
-          row_a[tid] = fa * ex2(fmaxf(float(rv) - E, -126.f));
-          row_mb[tid] = fb * ex2(-E);
-          if (tid < sg.n_rows) {
-            const int part = 2 * blockIdx.x + (a0 == 0 && sg.un.t > 0 ? 0 : 1);
-            pl.sp.ml[int64_t(part) * NR + tid] = make_float4(M, den, E, 0.f);
-          }
-        }
+      group_sync(grp);
+      const int part = 2 * blockIdx.x + (a0 == 0 && sg.un.t > 0 ? 0 : 1);
+      if (gtid < RW) {
+        // o and l are relative to row_m, o in units of 2^rv
+        const int r = g0 + gtid;
+        const float den = red[gtid] + red[16 + gtid] + red[32 + gtid] + red[48 + gtid];
+        row_a[r] = den == 0.f ? 0.f : kv8_exp2i(min(max(rv, -126), 126)) / den;
+        if (!sg.whole && r < sg.n_rows)
+          pl.sp.ml[int64_t(part) * NR + r] = make_float4(den == 0.f ? -INFINITY : -row_m[r], den, float(rv), 0.f);
       }
-      softmax_sync();
-      if (blk) {  // the block's weights with their row's factor
-        for (int x = tid; x < p.block * NR; x += 128) W[x] *= row_mb[x % NR];
-        softmax_sync();
-      }
+      group_sync(grp);
       if (sg.steps > 0) {
-        if (ok) ok = mbar_wait(o_full, outs & 1);
+        if (ok) ok = wait(o_full, outs & 1);
         ++outs;
         tc::tc_fence_after();
       }
 #pragma unroll 1
       for (int nh = 0; nh < C::NH; ++nh) {
-        const int d = nh * 128 + tid;
-        float o[NR];
+        const int d = nh * 128 + gtid;
+        float o[RW];
         if (sg.steps > 0) {
-          tmem_ld<NR>(t_o + t_lane + nh * NM, o);
+          tmem_ld<RW>(t_o + t_lane + nh * NM + g0, o);
           tc::tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) o[r] = 0.f;
+          for (int r = 0; r < RW; ++r) o[r] = 0.f;
         }
         if (d >= HD) continue;  // head_dim 64: the other lanes multiplied whatever followed
-#pragma unroll
-        for (int r = 0; r < NR; ++r) o[r] *= row_a[r];
-        if (blk) {
-          const B16* bv = static_cast<const B16*>(p.blk_v) + sg.un.b * p.bv_batch + sg.g * p.bv_head + d;
-#pragma unroll 4
-          for (int j = 0; j < p.block; ++j) {
-            const float v = ld_f(bv, j * p.bv_row);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) o[r] = fmaf(W[j * NR + r], v, o[r]);
-          }
-        }
         if (sg.whole) {
           B16* out = static_cast<B16*>(p.out) + int64_t(sg.un.b) * p.block * p.n_heads * HD + d;
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (r < sg.n_rows) {
-              const int rr = sg.r0 + r;
-              out[(int64_t(rr % p.block) * p.n_heads + sg.g * group + rr / p.block) * HD] = __float2bfloat16_rn(o[r]);
-            }
+          for (int r = 0; r < RW; ++r)
+            if (g0 + r < sg.n_rows)
+              out[row_out[g0 + r]] = __float2bfloat16_rn(my_a[r] == 0.f ? 0.f : o[r] * my_a[r]);
         } else {
-          const int part = 2 * blockIdx.x + (a0 == 0 && sg.un.t > 0 ? 0 : 1);
-          float* out = pl.sp.part + int64_t(part) * NR * HD + d;
+          float* out = pl.sp.part + (int64_t(part) * NR + g0) * HD + d;
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (r < sg.n_rows) out[int64_t(r) * HD] = o[r];
+          for (int r = 0; r < RW; ++r)
+            if (g0 + r < sg.n_rows) out[r * HD] = o[r];
         }
       }
       tc::tc_fence_before();
@@ -774,7 +875,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, NR>::CTAS)
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  if (warp == 5) tc::tmem_dealloc(tmem, C::kAlloc);
+  if (warp == kProduct) tc::tmem_dealloc(tmem, C::kAlloc);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -804,21 +905,22 @@ int byte_map(CUtensorMap* map, const void* base, int64_t rows, int width, int bo
   return DSM_OK;
 }
 
-// query rows per CTA: multiples of 8, since the softmax costs by the row, and 4 for single tokens
-int rows_of(int rows) { return rows <= 4 ? 4 : std::min(64, (rows + 7) / 8 * 8); }
-int ctas_per_sm(int hd) { return hd == 256 ? 1 : 2; }
+int rows_of(int rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+int ctas_per_sm(int nr, int hd) { return hd == 256 || nr == 64 ? 1 : 2; }
 
 template <int HD, int NR>
 int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
   using C = Cfg<HD, NR>;
   // 227 KB per SM, 1 KB of it taken by each CTA
-  const int room = 228 * 1024 / C::CTAS - 1024, block = a.blk_k ? a.block : 0;
-  // two stages at least: a step's scores are issued before the previous step's sums. A large batch's prefix
-  // and a large block may leave room for one CTA per SM only
-  pl.stages = 4;
-  while (pl.stages > 2 && umma_smem(HD, NR, pl.stages, block, a.batch).bytes > room) --pl.stages;
-  const int smem = umma_smem(HD, NR, pl.stages, block, a.batch).bytes;
+  const int room = 228 * 1024 / C::CTAS - 1024;
+  // two slots of each at least: a step's scores are issued before the previous step's sums. A large batch's
+  // prefix may leave room for one CTA per SM only
+  int slots = 2 * kMaxSlots;
+  while (slots > 4 && umma_smem(HD, C::NM, slots, a.batch).bytes > room) --slots;
+  const int smem = umma_smem(HD, C::NM, slots, a.batch).bytes;
   if (smem > 227 * 1024) return DSM_ERR_UNSUPPORTED;
+  pl.k_slots = slots / 2;
+  pl.v_slots = slots - pl.k_slots;
   CUtensorMap kmap{}, vmap{};
   const int64_t groups = int64_t(a.n_pages) * a.n_kv * (a.page / kTile);
   int st = byte_map(&vmap, a.v_codes, groups * HD, kTile, kTile, HD, true);
@@ -828,7 +930,7 @@ int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
   auto kern = kv8_umma_kernel<HD, NR>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("gqa_attn_kv8 smem attribute");
-  kern<<<unsigned(pl.sp.ctas), kThreads, size_t(smem), s>>>(a, pl, kmap, vmap);
+  kern<<<unsigned(pl.sp.ctas), C::kThreads, size_t(smem), s>>>(a, pl, kmap, vmap);
   st = check_launch("gqa_attn_kv8");
   return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, DSM_DT_BF16, s);
 }
@@ -839,11 +941,7 @@ int launch_rows(int nr, const AttnArgs& a, const UmmaPlan& pl, cudaStream_t s) {
     case 4: return launch<HD, 4>(a, pl, s);
     case 8: return launch<HD, 8>(a, pl, s);
     case 16: return launch<HD, 16>(a, pl, s);
-    case 24: return launch<HD, 24>(a, pl, s);
     case 32: return launch<HD, 32>(a, pl, s);
-    case 40: return launch<HD, 40>(a, pl, s);
-    case 48: return launch<HD, 48>(a, pl, s);
-    case 56: return launch<HD, 56>(a, pl, s);
     default: return launch<HD, 64>(a, pl, s);
   }
 }
@@ -851,7 +949,8 @@ int launch_rows(int nr, const AttnArgs& a, const UmmaPlan& pl, cudaStream_t s) {
 }  // namespace
 
 size_t kv8_umma_ws_bytes(int rows, int hd) {
-  return split_ws_bytes(ctas_per_sm(hd) * num_sms(), rows_of(rows), hd);
+  const int nr = rows_of(rows);
+  return split_ws_bytes(ctas_per_sm(nr, hd) * num_sms(), nr, hd);
 }
 
 int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
@@ -862,13 +961,13 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   pl.sp.cta_rows = nr;
   const int64_t groups = int64_t(a.n_pages) * a.n_kv * (a.page / kTile);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * pl.sp.row_blocks;
-  // tile numbers, and rows of the TMA maps, stay in 32 bits
-  if (most > 0x7fffffff || groups * std::max(hd, kTile) > 0x7fffffff) return DSM_ERR_UNSUPPORTED;
-  const int most_ctas = ctas_per_sm(hd) * num_sms();
+  if (groups * std::max(hd, kTile) > 0x7fffffff) return DSM_ERR_UNSUPPORTED;  // rows of the TMA maps
+  const int most_ctas = ctas_per_sm(nr, hd) * num_sms();
   pl.sp.ctas = int(std::min<int64_t>(most_ctas, most));
   pl.sp.cost = 6;
   pl.sp.snap = 4;
   pl.sp.least = 12;
+  if (!split_fits(a, pl.sp)) return DSM_ERR_UNSUPPORTED;
   split_ws(pl.sp, ws, hd);
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 8);
   pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 8);
