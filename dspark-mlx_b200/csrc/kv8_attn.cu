@@ -271,8 +271,10 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
   }
   fence_mbar_init();
   scan_tiles<kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may take its place and wait
   int start;
-  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 12, start);
+  Place first;
+  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 8, start, first);
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -864,23 +866,32 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   constexpr int V = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.x, r = blockIdx.y * kCombineWarps + warp;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the ranges run: see all that they wrote
+  // everything that a unit of two ranges needs is asked for at once. Range i's part is its last (slot 2 i + 1),
+  // the others' their first (slot 2 k)
   const int4 at = sp.places[i + 1];  // sequence, unit, tile, tiles
-  const int x = sp.cuts[i + 1], before = sp.cuts[i], end = sp.cuts[sp.ctas];
+  const int x = sp.cuts[i + 1], end = sp.cuts[sp.ctas];
+  int c0 = sp.cuts[min(i + lane, sp.ctas)], c1 = sp.cuts[min(i + lane + 1, sp.ctas)];
+  const int row = min(r, sp.cta_rows - 1);
+  auto slot_of = [&](int k) { return int64_t(k == i ? 2 * i + 1 : 2 * min(k, sp.ctas - 1)) * sp.cta_rows + row; };
+  float4 w = sp.ml[slot_of(i + lane)];
+  float p0[V], p1[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    p0[j] = sp.part[slot_of(i) * HD + lane * V + j];
+    p1[j] = sp.part[slot_of(i + 1) * HD + lane * V + j];
+  }
   const int u0 = x - at.z, u1 = u0 + at.w;
-  if (x >= end || at.z == 0 || before > u0) return;
+  if (x >= end || at.z == 0 || __shfl_sync(0xffffffffu, c0, 0) > u0) return;
   const int g = at.y / sp.row_blocks, r0 = (at.y % sp.row_blocks) * sp.cta_rows;
   if (r >= min(sp.cta_rows, sp.rows - r0)) return;
-  // 32 ranges at a time, a lane each: range i's part is its last (slot 2 i + 1), the others' their first (slot
-  // 2 k); empty ranges have none
+  // 32 ranges at a time, a lane each; empty ranges have no part
   float M = -INFINITY, E = -200.f, l = 0.f, o[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) o[j] = 0.f;
-  for (int base = i; base < sp.ctas; base += 32) {
-    const int k = base + lane;
-    const int c0 = sp.cuts[min(k, sp.ctas)], c1 = sp.cuts[min(k + 1, sp.ctas)];
+  for (int base = i;;) {
     const bool mine = c0 < c1 && c0 < u1;
-    const int64_t slot = int64_t(k == i ? 2 * i + 1 : 2 * k) * sp.cta_rows + r;
-    const float4 w = mine ? sp.ml[slot] : make_float4(-INFINITY, 0.f, -200.f, 0.f);
+    if (!mine) w = make_float4(-INFINITY, 0.f, -200.f, 0.f);
     const float M2 = fmaxf(M, kv8_warp_max(w.x)), E2 = fmaxf(E, kv8_warp_max(w.z));
     const float ref = M2 == -INFINITY ? 0.f : M2;
     const float keep = ex2(M - ref) * ex2(fmaxf(E - E2, -126.f));
@@ -892,16 +903,23 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
     const float f = mine ? ex2(w.x - ref) : 0.f, fo = f * ex2(fmaxf(w.z - E, -126.f));
     l += kv8_warp_sum(w.y * f);
     const unsigned parts = __ballot_sync(0xffffffffu, mine);
-    const float* src = sp.part + lane * V;
 #pragma unroll 4
     for (int j = 0; j < 32 - __clz(parts); ++j) {
       const float fj = __shfl_sync(0xffffffffu, fo, j);
-      const int64_t sj = __shfl_sync(0xffffffffu, slot, j);
-      if (parts >> j & 1)
+      if (parts >> j & 1) {
+        const float* src = sp.part + slot_of(base + j) * HD + lane * V;
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = fmaf(src[sj * HD + v], fj, o[v]);
+        for (int v = 0; v < V; ++v) {
+          const float y = base == i && j == 0 ? p0[v] : base == i && j == 1 ? p1[v] : src[v];
+          o[v] = fmaf(y, fj, o[v]);
+        }
+      }
     }
     if (__shfl_sync(0xffffffffu, c1, 31) >= u1) break;  // the unit's last tile lies in these ranges
+    base += 32;
+    c0 = sp.cuts[min(base + lane, sp.ctas)];
+    c1 = sp.cuts[min(base + lane + 1, sp.ctas)];
+    w = sp.ml[slot_of(base + lane)];
   }
   const int rr = r0 + r, group = p.n_heads / p.n_kv;
   T* out = static_cast<T*>(p.out) +
@@ -979,14 +997,25 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
 }  // namespace
 
 int kv8_combine(const AttnArgs& a, const KvSplit& sp, int hd, int dtype, cudaStream_t s) {
-  if (sp.ctas == 1) return DSM_OK;
+  // a unit of up to 2 * snap tiles is never cut
+  if (sp.ctas == 1 || a.max_pages * (a.page / kTile) <= 2 * sp.snap) return DSM_OK;
   const dim3 grid(unsigned(sp.ctas - 1), unsigned(ceil_div(std::min(sp.cta_rows, sp.rows), kCombineWarps)));
   const bool bf = dtype == DSM_DT_BF16;
   using B = __nv_bfloat16;
   auto k = hd == 64    ? (bf ? kv8_attn_combine_kernel<B, 64> : kv8_attn_combine_kernel<float, 64>)
            : hd == 128 ? (bf ? kv8_attn_combine_kernel<B, 128> : kv8_attn_combine_kernel<float, 128>)
                        : (bf ? kv8_attn_combine_kernel<B, 256> : kv8_attn_combine_kernel<float, 256>);
-  k<<<grid, kCombineWarps * 32, 0, s>>>(a, sp);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, a, sp);
+  if (e != cudaSuccess) return fail(DSM_ERR_CUDA, std::string("gqa_attn_kv8 combine: ") + cudaGetErrorString(e));
   return check_launch("gqa_attn_kv8 combine");
 }
 

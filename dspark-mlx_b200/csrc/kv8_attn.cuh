@@ -126,15 +126,20 @@ __device__ __forceinline__ int cut(const int* P, int batch, int hr, int i, const
   return P[a.b] * hr + a.u * a.T + t;
 }
 
-// this CTA's range [first, first + n) of the line, noted down for the join; ends[2] in shared memory. All
-// threads call it, a warp for either end.
-__device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const KvSplit& sp, int* ends, int& first) {
+// this CTA's range: n tiles of the line from tile first, which is at `at`; noted down for the join. ends[6] in
+// shared memory; all threads call it, a warp for either end.
+__device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const KvSplit& sp, int* ends, int& first,
+                                        Place& at) {
   const int hr = p.n_kv * sp.row_blocks, i = blockIdx.x, tid = threadIdx.x;
   if (tid == 0 || tid == 32) {
     const int x = cut(P, p.batch, hr, i + (tid >> 5), sp);
     ends[tid >> 5] = x;
     if (tid == 0) {
       const Place a = place_of(P, p.batch, hr, min(x, P[p.batch] * hr - 1), 0);
+      ends[2] = a.b;
+      ends[3] = a.u;
+      ends[4] = a.t;
+      ends[5] = a.T;
       sp.places[i] = make_int4(a.b, a.u, a.t, a.T);
       sp.cuts[i] = x;
     } else if (i == sp.ctas - 1) {
@@ -143,7 +148,19 @@ __device__ __forceinline__ int my_range(const AttnArgs& p, const int* P, const K
   }
   __syncthreads();
   first = ends[0];
+  at.b = ends[2];
+  at.u = ends[3];
+  at.t = ends[4];
+  at.T = ends[5];
   return ends[1] - first;
+}
+// the unit behind one
+__device__ __forceinline__ void next_unit(const int* P, int batch, int hr, Place& a) {
+  a.t = 0;
+  if (++a.u == hr) {
+    a.u = 0;
+    if (++a.b < batch) a.T = P[a.b + 1] - P[a.b];
+  }
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -7,10 +7,11 @@
 // kind::f8f6f4 multiplies the e4m3 codes themselves. q, scaled per row by a power of two to at most
 // 448, is the sum of two e4m3 terms (hi = e4m3(x), lo = e4m3(x - hi): exact for bf16's 8 bits wherever
 // the residual reaches e4m3's normals, 2^-10 of a unit off elsewhere, of a row maximum of 224 to 448).
-// The weights are p = 2^(s - m + 8), an e4m3 term and an e5m2 residual: 2^-7 of a weight off at most, and
-// nothing above 2^-25 of the largest is lost. m is the row's reference: its maximum when it was last
-// set, plus one; it is set again when a weight would pass 2^8.75, and the sums in tensor memory are then
-// rescaled. The page's value exponent is folded into the weights relative to a reference rv that moves
+// The weights are p = 2^(s - m + 8), an e4m3 term and an e5m2 residual: 2^-7 of a weight off at most where it
+// is above 2^-15 of the largest, and nothing above 2^-22 of it is lost. m is the row's reference: its maximum
+// when it was last set, plus three; it is set again when a weight would pass 2^8.75, and the sums in tensor
+// memory are then rescaled (2,200 cycles: with a reference just above the maximum most of a unit's first
+// steps paid that). The page's value exponent is folded into the weights relative to a reference rv that moves
 // when an exponent leaves [rv - 10, rv]; the scores' page factor is one per thread. Scores, sums and weights'
 // sums are fp32. The block's own rows are a unit's first step, in two e4m3 terms per row like q.
 //
@@ -45,7 +46,7 @@ constexpr int kStepKeys = 128;
 constexpr int kGroupRows = 16;  // query rows of a softmax group
 constexpr float kPExp = 8.f;    // weights at the reference: 2^8
 constexpr float kPMax = 8.75f;  // 2^8.75 = 431 still fits e4m3
-constexpr float kPHead = 1.f;   // a new reference lies this much above the maximum
+constexpr float kPHead = 3.f;   // a new reference lies this much above the maximum: the maximum's own weight is 2^5
 
 template <int HD, int NR>  // NR query rows per CTA: 4, 8, 16, 32 or 64
 struct Cfg {
@@ -163,6 +164,28 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
     }
   return true;
 }
+__device__ __forceinline__ bool done(uint64_t* bar, uint32_t parity) {  // without waiting
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[N]) {
+  if constexpr (N == 16)
+    tc::tmem_st16(addr, r);
+  else if constexpr (N == 8)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  else
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3])
+                 : "memory");
+}
 // barriers of one softmax group (id 1 + group), and of all of them (id 8)
 __device__ __forceinline__ bool any_of_group(int group, bool x) {
   uint32_t r;
@@ -251,8 +274,7 @@ __device__ __forceinline__ void q_terms(const float* x, uint32_t& hi, uint32_t& 
 
 // One CTA's part of a unit: tiles [t0, t1) of sequence b's KV head g, query rows [r0, r0 + n_rows)
 struct Segment {
-  Place un;
-  int t0, t1, steps, g, r0, n_rows, len;
+  int b, t0, t1, steps, g, r0, n_rows, len;
   bool whole, blk;  // all of the unit; the block's own rows come first, as a step more
 };
 
@@ -291,43 +313,19 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hr = p.n_kv * pl.sp.row_blocks;
-  // translations that the first loads from each of these would wait for
-  if (tid < 8) {
-    const void* at = tid == 0   ? p.q
-                     : tid == 1 ? p.blk_k
-                     : tid == 2 ? p.blk_v
-                     : tid == 3 ? static_cast<const void*>(p.table)
-                     : tid == 4 ? static_cast<const void*>(p.k_scale)
-                     : tid == 5 ? static_cast<const void*>(p.v_scale)
-                     : tid == 6 ? p.out
-                                : static_cast<const void*>(pl.sp.part);
-    if (at) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-  }
-  if (tid == 32) {
-    for (int i = 0; i < kMaxSlots; ++i) {
-      mbar_init(k_full + i, 1);
-      mbar_init(k_empty + i, 1);
-      mbar_init(v_full + i, 1);
-      mbar_init(v_empty + i, 1);
-    }
-    for (int i = 0; i < kInfos; ++i) {
-      mbar_init(i_full + i, 1);
-      mbar_init(granted + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, 4 * C::G);
-      mbar_init(p_full + i, 4 * C::G);
-      mbar_init(p_empty + i, 1);
-    }
-    mbar_init(q_full, 4 * C::G);
-    mbar_init(o_full, 1);
+  constexpr int kBars = 4 * kMaxSlots + 2 * kInfos + 10;
+  if (tid < kBars) {  // one arrival each, but what the softmax warps arrive on
+    const int i = tid - (4 * kMaxSlots + 2 * kInfos);
+    const bool by_softmax = i == 2 || i == 3 || i == 4 || i == 5 || i == 8;  // s_empty, p_full, q_full
+    mbar_init(k_full + tid, by_softmax ? 4 * C::G : 1);
     fence_mbar_init();
   }
   if (warp == kProduct) tc::tmem_alloc(slot, C::kAlloc);
   scan_tiles<C::kThreads>(p, P, reinterpret_cast<int*>(smem + L.sums));
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may take its place and wait
   int start;
-  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 24, start);
+  Place un;  // the unit that this warp is at
+  const int n_tiles = my_range(p, P, pl.sp, reinterpret_cast<int*>(smem + L.sums) + 20, start, un);
   if (blockIdx.x == 0)
     for (int b = tid; b < p.batch; b += C::kThreads)
       if (p.lengths[b] > int64_t(p.max_pages) * p.page) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
@@ -338,16 +336,21 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
 
   auto segment = [&](int a0) {
     Segment s;
-    s.un = place_of(P, p.batch, hr, start + a0, 0);
-    s.t0 = s.un.t;
-    s.t1 = min(s.un.T, s.un.t + n_tiles - a0);
-    s.blk = s.t1 == s.un.T && p.blk_k;
-    s.whole = s.t1 == s.un.T && s.t0 == 0;
-    s.g = s.un.u / pl.sp.row_blocks;
-    s.r0 = (s.un.u - s.g * pl.sp.row_blocks) * NR;
+    s.b = un.b;
+    s.t0 = un.t;
+    s.t1 = min(un.T, un.t + n_tiles - a0);
+    s.blk = s.t1 == un.T && p.blk_k;
+    s.whole = s.t1 == un.T && s.t0 == 0;
+    s.g = un.u;
+    s.r0 = 0;
+    if (pl.sp.row_blocks > 1) {
+      s.g = un.u / pl.sp.row_blocks;
+      s.r0 = (un.u - s.g * pl.sp.row_blocks) * NR;
+    }
     s.n_rows = min(NR, pl.sp.rows - s.r0);
-    s.len = seq_len(p, s.un.b);
+    s.len = seq_len(p, un.b);
     s.steps = (s.len == 0 ? 0 : (s.t1 - s.t0 + 1) / 2) + s.blk;
+    next_unit(P, p.batch, hr, un);
     return s;
   };
   bool ok = true;  // no wait has run out; after one has, loops go through without waiting, copying or multiplying
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         const int t = sg.t0 + base + lane;
         int pg = -1;
         if (base + lane < tiles) {
-          pg = __ldg(p.table + int64_t(sg.un.b) * p.table_stride + t * kTile / p.page);
+          pg = __ldg(p.table + int64_t(sg.b) * p.table_stride + t * kTile / p.page);
           if (pg < 0 || pg >= p.n_pages) {
             raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
             pg = -1;
@@ -477,8 +480,8 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         uint32_t idle = 0;
         for (int i = 0, j = 0; j < sg.steps && ok;) {
           const int kk = k + i, sb = kk & 1, jj = k + j;
-          if (i < sg.steps && i < j + 2 && mbar_try_wait(k_full + kk % KN, (kk / KN) & 1) &&
-              (kk < 2 || mbar_try_wait(s_empty + sb, ((kk >> 1) - 1) & 1))) {
+          if (i < sg.steps && i < j + 2 && done(k_full + kk % KN, (kk / KN) & 1) &&
+              (kk < 2 || done(s_empty + sb, ((kk >> 1) - 1) & 1))) {
             tc::tc_fence_after();
             // the block's step: its keys' hi terms are rows 0-63, their lo terms rows 64-127, multiplied as
             // rows 0-63 once more
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
             tc::umma_commit(k_empty + kk % KN);
             ++i;
             idle = 0;
-          } else if (j < i && mbar_try_wait(p_full + (jj & 1), (jj >> 1) & 1)) {
+          } else if (j < i && done(p_full + (jj & 1), (jj >> 1) & 1)) {
             sums(jj, j == 0, sg.blk && j == 0);
             ++j;
             idle = 0;
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, results
-    constexpr int TPR = 16, VB = HD / TPR, kPass = C::kSoftmax / TPR;  // staging: threads per row, values per thread
+    constexpr int TPR = 8, VB = HD / TPR, kPass = C::kSoftmax / TPR;  // staging: threads per row, values per thread
     const int grp = C::G == 1 ? 0 : warp >> 2, gtid = C::G == 1 ? tid : tid & 127;
     const int g0 = grp * kGroupRows;  // its first row
     const int half = gtid >> 6;       // which 64 keys of a step this thread's key is in
@@ -539,32 +542,30 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
       softmax_sync<C::kSoftmax>();  // the previous unit's row statistics are used up
       uint8_t* const kt = smem + (k % KN) * C::kSlot;
       uint8_t* const vt = v_slots + (k % VN) * C::kSlot;
-      constexpr int kQPasses = NR <= kPass ? 1 : NR / kPass;
-      const int n_blk = sg.blk ? (p.block + kPass - 1) / kPass : 0, n_tasks = kQPasses + 2 * n_blk;
-      auto load_rows = [&](int task, float(&x)[VB]) {
-        const int j = task - kQPasses;
-        const bool of_v = j >= n_blk;
-        const int r = (j < 0 ? task : of_v ? j - n_blk : j) * kPass + row_r;
+      // the rows in one list: q's (those past n_rows are zero), the block's keys', its values'
+      const int n_blk = sg.blk ? p.block : 0, n_list = NR + 2 * n_blk;
+      auto load_rows = [&](int r, float(&x)[VB]) {
         const B16* src;
-        if (j < 0) {
+        bool live, vec = pl.vec_blk;
+        if (r < NR) {
           const int rr = sg.r0 + r, h = unsigned(rr) / unsigned(p.block);
-          src = static_cast<const B16*>(p.q) + sg.un.b * p.q_batch + (rr - h * p.block) * p.q_row +
-                (sg.g * group + h) * p.q_head;
+          src = static_cast<const B16*>(p.q) + sg.b * p.q_batch + (rr - h * p.block) * p.q_row + (sg.g * group + h) * p.q_head;
+          live = r < sg.n_rows;
+          vec = pl.vec_q;
+          if (row_d == 0) row_out[r] = ((rr - h * p.block) * p.n_heads + sg.g * group + h) * HD;
+        } else if (r < NR + n_blk) {
+          src = static_cast<const B16*>(p.blk_k) + sg.b * p.bk_batch + sg.g * p.bk_head + (r - NR) * p.bk_row;
+          live = true;
         } else {
-          src = of_v ? static_cast<const B16*>(p.blk_v) + sg.un.b * p.bv_batch + sg.g * p.bv_head + r * p.bv_row
-                     : static_cast<const B16*>(p.blk_k) + sg.un.b * p.bk_batch + sg.g * p.bk_head + r * p.bk_row;
+          src = static_cast<const B16*>(p.blk_v) + sg.b * p.bv_batch + sg.g * p.bv_head + (r - NR - n_blk) * p.bv_row;
+          live = r < n_list;
         }
 #pragma unroll
         for (int i = 0; i < VB; ++i) x[i] = 0.f;
-        if (r < (j < 0 ? sg.n_rows : p.block)) load_vals<B16, VB>(src + row_d, j < 0 ? pl.vec_q : pl.vec_blk, x);
+        if (live) load_vals<B16, VB>(src + row_d, vec, x);
       };
-      float x[VB], x1[VB];
-      load_rows(0, x);
-      if (n_tasks > 1) load_rows(1, x1);
-      if (tid < NR) {  // where the row's result goes
-        const int rr = sg.r0 + tid, h = unsigned(rr) / unsigned(p.block);
-        row_out[tid] = ((rr - h * p.block) * p.n_heads + sg.g * group + h) * HD;
-      }
+      float x[VB];
+      load_rows(row_r, x);
       if (sg.blk) {
         if (ok) ok = wait(granted + k % kInfos, blocks >> k % kInfos & 1);
         blocks ^= 1u << k % kInfos;
@@ -578,12 +579,12 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         softmax_sync<C::kSoftmax>();
       }
 #pragma unroll 1
-      for (int task = 0; task < n_tasks; ++task) {
-        float x2[VB];  // two rows ahead
-        if (task + 2 < n_tasks) load_rows(task + 2, x2);
-        const int j = task - kQPasses;
-        const bool of_q = j < 0, of_v = j >= n_blk;
-        const int r = (of_q ? task : of_v ? j - n_blk : j) * kPass + row_r;
+      for (int at_row = row_r; at_row < (n_list + kPass - 1) / kPass * kPass; at_row += kPass) {
+        float next[VB];
+        if (at_row + kPass < n_list + row_r) load_rows(at_row + kPass, next);
+        const bool of_q = at_row < NR, of_v = at_row >= NR + n_blk;
+        const int r = of_q ? at_row : of_v ? at_row - NR - n_blk : at_row - NR;  // among its kind
+        const bool live = at_row < n_list;
         // scaled by a power of two to at most 448
         float mx = 0.f;
 #pragma unroll
@@ -593,10 +594,10 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         const int e = kv8_scale_exp(mx);
         const float inv = kv8_exp2i(-e);
         if (row_d == 0) {
-          if (of_q && r < NM) {
+          if (of_q) {
             row_c[r] = r < sg.n_rows ? p.scale * kLog2e * kv8_exp2i(e) : 0.f;
             row_m[r] = 0.f;
-          } else if (!of_q && r < p.block) {
+          } else if (live) {
             if (of_v)
               keys[r].y = float(e);
             else
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           q_terms(y, t[0], t[1]);
           const int d = row_d + i;
           if (of_v) {
-            if (r < p.block) {
+            if (live) {
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
                 uint8_t* b = vt + (d + w) * 64 + (((r >> 4) ^ (((d + w) >> 1) & 3)) << 4) + (r & 15);
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
                 b[C::kHalf] = uint8_t(t[1] >> (8 * w));
               }
             }
-          } else if (r < (of_q ? NM : kTile)) {
+          } else {
             uint8_t* b = HD == 64 ? at + r * 64 + ((((d >> 4) & 3) ^ ((r >> 1) & 3)) << 4) + (d & 15)
                                   : at + (d >> 7) * rows * 128 + r * 128 + ((((d >> 4) & 7) ^ (r & 7)) << 4) + (d & 15);
             *reinterpret_cast<uint32_t*>(b) = t[0];
@@ -631,10 +632,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           }
         }
 #pragma unroll
-        for (int i = 0; i < VB; ++i) {
-          x[i] = x1[i];
-          x1[i] = x2[i];
-        }
+        for (int i = 0; i < VB; ++i) x[i] = next[i];
       }
       tc::fence_async_smem();
       softmax_sync<C::kSoftmax>();
@@ -714,36 +712,32 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
             const float up = x == kLowest ? 0.f : i == 0 || x > kPExp ? x + (kPHead - kPExp) : 0.f;
             row_m[g0 + gtid] -= up;
             red[gtid] = up;
-            const float fv = rv <= -200 ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
-            row_a[g0 + gtid] = ex2(-up) * fv;
+            row_a[g0 + gtid] = ex2(-up);
           }
           group_sync(grp);
+          const float fv = rv <= -200 ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
           rv = want_rv;
           if (i > 0) {  // the sums so far, after the products that make them
             const int j = k - 1;
             if (ok) ok = wait(p_empty + (j & 1), (j >> 1) & 1);
             tc::tc_fence_after();
+#pragma unroll
+            for (int r = 0; r < RW; ++r) l[r] *= my_a[r];
 #pragma unroll 1
-            for (int c = 0; c < C::NH * RW; c += 4) {
-              const int at_r = C::NH == 1 ? c : c % RW;
-              float o[4];
-              const uint32_t at = t_o + t_lane + (C::NH == 1 ? 0 : c / RW * NM) + g0 + at_r;
-              tmem_ld<4>(at, o);
+            for (int nh = 0; nh < C::NH; ++nh) {
+              float o[RW];
+              uint32_t u[RW];
+              const uint32_t at = t_o + t_lane + nh * NM + g0;
+              tmem_ld<RW>(at, o);
               tc::tmem_ld_wait();
-              const float4 a = *reinterpret_cast<const float4*>(my_a + at_r);
-              asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at),
-                           "r"(__float_as_uint(o[0] * a.x)), "r"(__float_as_uint(o[1] * a.y)),
-                           "r"(__float_as_uint(o[2] * a.z)), "r"(__float_as_uint(o[3] * a.w))
-                           : "memory");
+#pragma unroll
+              for (int r = 0; r < RW; ++r) u[r] = __float_as_uint(o[r] * (my_a[r] * fv));
+              tmem_st(at, u);
             }
             tc::tmem_st_wait();
           }
 #pragma unroll
-          for (int r = 0; r < RW; ++r) {
-            const float up = red[r];
-            if (i > 0) l[r] *= ex2(-up);
-            y[r] -= up;
-          }
+          for (int r = 0; r < RW; ++r) y[r] -= red[r];
         }
         const int dv = max(e_key - rv, -60);  // <= 0
         const float fv = kv8_exp2i(dv);
@@ -828,7 +822,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         if (lane % per == 0) red[(warp & 3) * kGroupRows + lane / per] = l[0];
       }
       group_sync(grp);
-      const int part = 2 * blockIdx.x + (a0 == 0 && sg.un.t > 0 ? 0 : 1);
+      const int part = 2 * blockIdx.x + (a0 == 0 && sg.t0 > 0 ? 0 : 1);
       if (gtid < RW) {
         // o and l are relative to row_m, o in units of 2^rv
         const int r = g0 + gtid;
@@ -856,7 +850,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         }
         if (d >= HD) continue;  // head_dim 64: the other lanes multiplied whatever followed
         if (sg.whole) {
-          B16* out = static_cast<B16*>(p.out) + int64_t(sg.un.b) * p.block * p.n_heads * HD + d;
+          B16* out = static_cast<B16*>(p.out) + int64_t(sg.b) * p.block * p.n_heads * HD + d;
 #pragma unroll
           for (int r = 0; r < RW; ++r)
             if (g0 + r < sg.n_rows)
