@@ -858,6 +858,16 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
 
 constexpr int kCombineWarps = 8;
 
+template <int V>
+__device__ __forceinline__ void load_part(const float* p, float (&x)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p + i);
+    x[i] = v.x;
+    x[i + 1] = v.y;
+  }
+}
+
 // Joins the units that were cut: CTA (i, y) looks at the cut between ranges i and i + 1; if it is its unit's
 // first, it joins the unit's rows y * 8 .. y * 8 + 7, a warp each: the partial sums of its ranges in
 // order, then the division and the one rounding to T.
@@ -876,11 +886,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
   auto slot_of = [&](int k) { return int64_t(k == i ? 2 * i + 1 : 2 * min(k, sp.ctas - 1)) * sp.cta_rows + row; };
   float4 w = sp.ml[slot_of(i + lane)];
   float p0[V], p1[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    p0[j] = sp.part[slot_of(i) * HD + lane * V + j];
-    p1[j] = sp.part[slot_of(i + 1) * HD + lane * V + j];
-  }
+  load_part<V>(sp.part + slot_of(i) * HD + lane * V, p0);
+  load_part<V>(sp.part + slot_of(i + 1) * HD + lane * V, p1);
   const int u0 = x - at.z, u1 = u0 + at.w;
   if (x >= end || at.z == 0 || __shfl_sync(0xffffffffu, c0, 0) > u0) return;
   const int g = at.y / sp.row_blocks, r0 = (at.y % sp.row_blocks) * sp.cta_rows;
@@ -902,18 +909,35 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
     E = E2;
     const float f = mine ? ex2(w.x - ref) : 0.f, fo = f * ex2(fmaxf(w.z - E, -126.f));
     l += kv8_warp_sum(w.y * f);
-    const unsigned parts = __ballot_sync(0xffffffffu, mine);
-#pragma unroll 4
-    for (int j = 0; j < 32 - __clz(parts); ++j) {
-      const float fj = __shfl_sync(0xffffffffu, fo, j);
-      if (parts >> j & 1) {
-        const float* src = sp.part + slot_of(base + j) * HD + lane * V;
+    unsigned parts = __ballot_sync(0xffffffffu, mine);
+    if (base == i) {
+      const float f0 = __shfl_sync(0xffffffffu, fo, 0), f1 = __shfl_sync(0xffffffffu, fo, 1);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float y = base == i && j == 0 ? p0[v] : base == i && j == 1 ? p1[v] : src[v];
-          o[v] = fmaf(y, fj, o[v]);
-        }
+      for (int v = 0; v < V; ++v) {
+        o[v] = fmaf(p0[v], f0, o[v]);
+        if (parts & 2) o[v] = fmaf(p1[v], f1, o[v]);
       }
+      parts &= ~3u;
+    }
+    while (parts) {  // eight parts in flight
+      float y[8][V], fj[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int j = parts ? __ffs(parts) - 1 : 0;
+        fj[n] = __shfl_sync(0xffffffffu, fo, j);
+        if (parts) {
+          load_part<V>(sp.part + slot_of(base + j) * HD + lane * V, y[n]);
+        } else {
+          fj[n] = 0.f;
+#pragma unroll
+          for (int v = 0; v < V; ++v) y[n][v] = 0.f;
+        }
+        parts &= parts - 1;
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = fmaf(y[n][v], fj[n], o[v]);
     }
     if (__shfl_sync(0xffffffffu, c1, 31) >= u1) break;  // the unit's last tile lies in these ranges
     base += 32;
