@@ -71,6 +71,13 @@ __device__ __forceinline__ float kv8_warp_sum(float v) {
   return v;
 }
 
+// x / d == umulhi(x, kv8_per_page) for page = 64 d, d = 2 .. 16, and x < 2^28: ceil(2^32 / d) is off by less than
+// 1, so the product by less than x <= 2^32 / d, a step of the quotient. 0 stands for d = 1
+inline uint32_t kv8_per_page(int page) {
+  const int64_t d = page / kKv8Group;
+  return d == 1 ? 0u : uint32_t(((int64_t(1) << 32) + d - 1) / d);
+}
+
 inline bool kv8_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline bool kv8_head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 inline bool kv8_page_ok(int page) { return page > 0 && page % kKv8Group == 0 && page <= kKv8MaxPage; }

@@ -96,6 +96,7 @@ struct ExtendArgs {
   int64_t* slot_map;
   int32_t* positions;
   int64_t max_rows;
+  uint32_t per_page;  // kv8_per_page
 };
 
 // shared memory: cu [batch + 1], off [batch], len [batch] (len < 0: the sequence gets nothing)
@@ -169,20 +170,47 @@ __global__ void __launch_bounds__(kPagedThreads) paged_extend_kernel(const Exten
     const int j = (len[i] + p.page - 1) / p.page + (k - off[i]);
     p.table[int64_t(i) * p.table_stride + j] = p.free_pages[free0 - 1 - k];
   }
-  for (int64_t r = me; r < p.max_rows; r += all) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (r < total) {
-      const int i = last_not_above(cu, p.batch, int(r));
-      if (len[i] >= 0) {
-        pos = len[i] + int(r) - cu[i];
-        const int j = pos / p.page, have = (len[i] + p.page - 1) / p.page;
-        const int pg = j < have ? p.table[int64_t(i) * p.table_stride + j] : p.free_pages[free0 - 1 - off[i] - (j - have)];
-        slot = int64_t(pg) * p.page + (pos - j * p.page);
+  // rows: a run of them per warp, four per lane in flight; a lane keeps its sequence from row to row
+  constexpr int kRows = 4;
+  const int warps = ctas * kPagedWarps, lane = tid & 31;
+  const int64_t each = (p.max_rows + int64_t(warps) * 32 - 1) / (int64_t(warps) * 32) * 32;
+  const int64_t first = int64_t(rank * kPagedWarps + (tid >> 5)) * each, last = min(first + each, p.max_rows);
+  int i = -1, c0 = 0, c1 = 0, n0 = -1, have = 0;  // the lane's sequence: its rows, cached rows and pages
+  const int32_t *old_pages = nullptr, *new_pages = nullptr;
+  for (int64_t base = first; base < last; base += kRows * 32) {
+    int pos[kRows], at[kRows];
+    const int32_t* from[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int64_t r = base + u * 32 + lane;
+      pos[u] = 0;
+      from[u] = nullptr;
+      if (r >= total || r >= last) continue;
+      if (c1 <= int(r)) {
+        i += 1 + last_not_above(cu + i + 1, p.batch - i - 1, int(r));
+        c0 = cu[i];
+        c1 = cu[i + 1];
+        n0 = len[i];
+        have = (n0 + p.page - 1) / p.page;
+        old_pages = p.table + int64_t(i) * p.table_stride;
+        new_pages = p.free_pages + (free0 - 1 - off[i] + have);
       }
+      if (n0 < 0) continue;
+      pos[u] = n0 + int(r) - c0;
+      const int j = p.per_page ? int(__umulhi(unsigned(pos[u]) / kKv8Group, p.per_page)) : pos[u] / kKv8Group;
+      at[u] = pos[u] - j * p.page;
+      from[u] = j < have ? old_pages + j : new_pages - j;
     }
-    p.slot_map[r] = slot;
-    p.positions[r] = pos;
+    int pg[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) pg[u] = from[u] ? *from[u] : 0;
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int64_t r = base + u * 32 + lane;
+      if (r >= last) continue;
+      p.slot_map[r] = from[u] ? int64_t(pg[u]) * p.page + at[u] : -1;
+      p.positions[r] = pos[u];
+    }
   }
 }
 
@@ -292,8 +320,9 @@ extern "C" int dsm_paged_extend(int32_t* lengths, const int32_t* new_len, int ba
   DSM_REQUIRE(cu_rows && (max_rows == 0 || (slot_map && positions)) && free_pages && n_free &&
                   (batch == 0 || (lengths && new_len && block_table)),
               "dsm_paged_extend: NULL pointer");
+  const uint32_t per_page = kv8_per_page(page_size);
   const ExtendArgs a = {lengths,  new_len, batch,   page_size, block_table, table_stride, max_pages, free_pages,
-                        n_free,   n_pages, cu_rows, slot_map,  positions,   max_rows};
+                        n_free,   n_pages, cu_rows, slot_map,  positions,   max_rows, per_page};
   // one CTA covers a decode step; a prefill's rows are shared out over a cluster
   const int ctas = max_rows > 4 * kPagedThreads ? kPagedCluster : 1;
   return launch_cluster(paged_extend_kernel, a, ctas, size_t(3 * batch + 1) * 4, stream, "dsm_paged_extend");
