@@ -97,7 +97,11 @@ struct ExtendArgs {
   int32_t* positions;
   int64_t max_rows;
   uint32_t per_page;  // kv8_per_page
+  bool rows_after;    // paged_rows_kernel follows
 };
+__device__ __forceinline__ int page_of(const ExtendArgs& p, int pos) {
+  return p.per_page ? int(__umulhi(unsigned(pos) / kKv8Group, p.per_page)) : pos / kKv8Group;
+}
 
 // shared memory: cu [batch + 1], off [batch], len [batch] (len < 0: the sequence gets nothing)
 __global__ void __launch_bounds__(kPagedThreads) paged_extend_kernel(const ExtendArgs p) {
@@ -170,47 +174,79 @@ __global__ void __launch_bounds__(kPagedThreads) paged_extend_kernel(const Exten
     const int j = (len[i] + p.page - 1) / p.page + (k - off[i]);
     p.table[int64_t(i) * p.table_stride + j] = p.free_pages[free0 - 1 - k];
   }
-  // rows: a run of them per warp, four per lane in flight; a lane keeps its sequence from row to row
-  constexpr int kRows = 4;
-  const int warps = ctas * kPagedWarps, lane = tid & 31;
-  const int64_t each = (p.max_rows + int64_t(warps) * 32 - 1) / (int64_t(warps) * 32) * 32;
-  const int64_t first = int64_t(rank * kPagedWarps + (tid >> 5)) * each, last = min(first + each, p.max_rows);
-  int i = -1, c0 = 0, c1 = 0, n0 = -1, have = 0;  // the lane's sequence: its rows, cached rows and pages
-  const int32_t *old_pages = nullptr, *new_pages = nullptr;
-  for (int64_t base = first; base < last; base += kRows * 32) {
-    int pos[kRows], at[kRows];
-    const int32_t* from[kRows];
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int64_t r = base + u * 32 + lane;
-      pos[u] = 0;
-      from[u] = nullptr;
-      if (r >= total || r >= last) continue;
-      if (c1 <= int(r)) {
-        i += 1 + last_not_above(cu + i + 1, p.batch - i - 1, int(r));
-        c0 = cu[i];
-        c1 = cu[i + 1];
-        n0 = len[i];
-        have = (n0 + p.page - 1) / p.page;
-        old_pages = p.table + int64_t(i) * p.table_stride;
-        new_pages = p.free_pages + (free0 - 1 - off[i] + have);
+  // a row's slot: all rows, or each sequence's first (the others follow in paged_rows_kernel)
+  const int64_t rows = p.rows_after ? p.batch : p.max_rows;
+  for (int64_t x = me; x < rows; x += all) {
+    const int64_t r = p.rows_after ? cu[x] : x;
+    if (p.rows_after && (cu[x + 1] == r || r >= p.max_rows)) continue;
+    int64_t slot = -1;
+    int pos = 0;
+    if (r < total) {
+      const int i = p.rows_after ? int(x) : last_not_above(cu, p.batch, int(r));
+      if (len[i] >= 0) {
+        pos = len[i] + int(r) - cu[i];
+        const int j = page_of(p, pos), have = (len[i] + p.page - 1) / p.page;
+        const int pg = j < have ? p.table[int64_t(i) * p.table_stride + j] : p.free_pages[free0 - 1 - off[i] - (j - have)];
+        slot = int64_t(pg) * p.page + (pos - j * p.page);
       }
-      if (n0 < 0) continue;
-      pos[u] = n0 + int(r) - c0;
-      const int j = p.per_page ? int(__umulhi(unsigned(pos[u]) / kKv8Group, p.per_page)) : pos[u] / kKv8Group;
-      at[u] = pos[u] - j * p.page;
-      from[u] = j < have ? old_pages + j : new_pages - j;
     }
-    int pg[kRows];
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) pg[u] = from[u] ? *from[u] : 0;
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int64_t r = base + u * 32 + lane;
-      if (r >= last) continue;
-      p.slot_map[r] = from[u] ? int64_t(pg[u]) * p.page + at[u] : -1;
-      p.positions[r] = pos[u];
+    p.slot_map[r] = slot;
+    p.positions[r] = pos;
+  }
+}
+
+// The rows of a long step, from what paged_extend_kernel has left: a sequence's rows, its new length, its table, and
+// in its first row's slot whether it got what it asked for (that slot is written once more, as it is). A
+// warp takes 128 neighbouring rows, finds their sequence by a 32-way search, and a lane keeps its
+// sequence from row to row.
+constexpr int kRowThreads = 256, kRowsPerLane = 4;
+
+__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const ExtendArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t first = (int64_t(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5)) * (32 * kRowsPerLane);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while paged_extend_kernel runs
+  if (first >= p.max_rows) return;
+  const int64_t total = p.cu_rows[p.batch];
+  int i = 0;
+  if (first < total) {
+    for (int n = p.batch; n > 1;) {  // the last sequence that starts at or before `first` is among n from i on
+      const int step = (n + 31) / 32;
+      const unsigned m = __ballot_sync(0xffffffffu, lane * step < n && p.cu_rows[i + min(lane * step, n - 1)] <= first);
+      const int k = 31 - __clz(m);
+      i += k * step;
+      n = min(step, n - k * step);
     }
+  }
+  int c0 = 0, c1 = 0, n0 = -1;  // the lane's sequence: its rows, its cached rows (-1: it got nothing)
+  int64_t slot[kRowsPerLane];
+  int pos[kRowsPerLane], at[kRowsPerLane];
+  const int32_t* from[kRowsPerLane];
+#pragma unroll
+  for (int u = 0; u < kRowsPerLane; ++u) {
+    const int64_t r = first + u * 32 + lane;
+    pos[u] = 0;
+    from[u] = nullptr;
+    if (r >= total || r >= p.max_rows) continue;
+    if (c1 <= int(r)) {
+      i += last_not_above(p.cu_rows + i, p.batch - i, int(r));
+      c0 = p.cu_rows[i];
+      c1 = p.cu_rows[i + 1];
+      n0 = p.slot_map[c0] < 0 ? -1 : p.lengths[i] - (c1 - c0);
+    }
+    if (n0 < 0) continue;
+    pos[u] = n0 + int(r) - c0;
+    const int j = page_of(p, pos[u]);
+    at[u] = pos[u] - j * p.page;
+    from[u] = p.table + int64_t(i) * p.table_stride + j;
+  }
+#pragma unroll
+  for (int u = 0; u < kRowsPerLane; ++u) slot[u] = from[u] ? int64_t(*from[u]) * p.page + at[u] : -1;
+#pragma unroll
+  for (int u = 0; u < kRowsPerLane; ++u) {
+    const int64_t r = first + u * 32 + lane;
+    if (r >= p.max_rows) continue;
+    p.slot_map[r] = slot[u];
+    p.positions[r] = pos[u];
   }
 }
 
@@ -321,11 +357,25 @@ extern "C" int dsm_paged_extend(int32_t* lengths, const int32_t* new_len, int ba
                   (batch == 0 || (lengths && new_len && block_table)),
               "dsm_paged_extend: NULL pointer");
   const uint32_t per_page = kv8_per_page(page_size);
+  // one CTA covers a decode step's rows; a prefill's are written by the whole GPU, its tables by a cluster
+  const bool many = max_rows > 4 * kPagedThreads;
   const ExtendArgs a = {lengths,  new_len, batch,   page_size, block_table, table_stride, max_pages, free_pages,
-                        n_free,   n_pages, cu_rows, slot_map,  positions,   max_rows, per_page};
-  // one CTA covers a decode step; a prefill's rows are shared out over a cluster
-  const int ctas = max_rows > 4 * kPagedThreads ? kPagedCluster : 1;
-  return launch_cluster(paged_extend_kernel, a, ctas, size_t(3 * batch + 1) * 4, stream, "dsm_paged_extend");
+                        n_free,   n_pages, cu_rows, slot_map,  positions,   max_rows, per_page,    many};
+  const int st = launch_cluster(paged_extend_kernel, a, many ? kPagedCluster : 1, size_t(3 * batch + 1) * 4, stream,
+                                "dsm_paged_extend");
+  if (st != DSM_OK || !many) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ceil_div(max_rows, int64_t(kRowThreads * kRowsPerLane))));
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.stream = as_stream(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_rows_kernel, a);
+  if (e != cudaSuccess) return fail(DSM_ERR_CUDA, std::string("dsm_paged_extend rows: ") + cudaGetErrorString(e));
+  return check_launch("dsm_paged_extend rows");
 }
 
 extern "C" int dsm_paged_trim(int32_t* lengths, const int32_t* keep_len, int batch, int page_size,
