@@ -2,10 +2,12 @@
 // sequence's rows in the paged 8-bit cache (layout in kv8.cuh) and then the block's own rows, with no
 // mask: the paged form of Qwen3DSparkAttention.attend_cached (dspark_mlx/arch/qwen3.py:130-143).
 //
-//   kv8_attn_mma_kernel   tensor-core products, split over the keys; kv8_attn_combine_kernel joins what
-//                         was cut.
-//   kv8_attn_core_kernel  fp32 products on the CUDA cores.
-// dsm_set_attn_kernel picks between them (per host thread).
+//   kv8_umma_kernel       bf16 rows and blocks of up to 64 rows, on tcgen05 (kv8_umma.cu)
+//   kv8_attn_mma_kernel   fp32 rows: f16 products in two terms each, split over the keys
+//   kv8_attn_combine_kernel  joins what either has cut
+//   kv8_attn_core_kernel  fp32 products on the CUDA cores: what the others do not take (a longer block, a
+//                         batch whose prefix does not fit shared memory), and dsm_set_attn_kernel's other
+//                         choice (per host thread)
 #include <algorithm>
 
 #include "kv8_attn.cuh"
@@ -139,23 +141,21 @@ int launch_core(const AttnArgs& a, cudaStream_t s) {
 
 
 // ------------------------------------------------------------------------------------------
-// the tensor-core kernel
+// the tensor-core kernel for fp32 rows
 // ------------------------------------------------------------------------------------------
 // Mathematics. e4m3 codes are exact in f16, so keys and values enter mma.m16n8k16 as the codes'
 // values and the page's power-of-two scales stay outside. q, scaled per row by a power of two to at
-// most 448, is one f16 term for bf16 rows (their 8 bits fit f16's 11) and two for fp32 rows (hi + lo,
-// 2^-22). A row's weights are p = 2^(s - m) with a reference m that follows its running maximum only
-// when that has grown by more than 2^8, so that the sums are rescaled rarely; they enter f16
-// (in one or two terms as well) as p * 2^6 * 2^(ev - rv), ev the exponent of the page's value scale and
-// rv a reference that it moves when it leaves [rv - 10, rv]: the sums need no factor per page. Sums,
-// weights and maxima are fp32. The tensor cores' own additions cut off what they round: too coarse for
-// fp32 calls over long sums, whose products go into the fp32 sums a few steps at a time, by CUDA cores.
+// most 448, is two f16 terms (hi + lo, 2^-22). A row's weights are p = 2^(s - m) with a reference m that
+// follows its running maximum only when that has grown by more than 2^8, so that the sums are rescaled
+// rarely; they enter f16, in two terms as well, as p * 2^6 * 2^(ev - rv), ev the exponent of the page's
+// value scale and rv a reference that it moves when it leaves [rv - 10, rv]: the sums need no factor per
+// page. Sums, weights and maxima are fp32. The tensor cores' own additions cut off what they round, too
+// coarse for fp32 calls over long sums: products go into the fp32 sums a few steps at a time, by CUDA cores.
 //
-// What bounds it: reading 2 * head_dim bytes per key and KV head. At the copy peak an SM gets 64
-// keys of head_dim 128 per ~700 cycles. mma.sync's e4m3 form runs as f16 products on this GPU, with the
-// conversions and fp32 additions around every one of them (measured: twice the tensor instructions for
-// q in two e4m3 terms, 4,000 instructions per tile and 32 rows, 3,400 cycles); converting each code once
-// per warp and keeping q and the weights in single f16 terms takes a quarter of that.
+// What bounds it: the products, two terms of q (and of the weights) for each code at 0.46 mma.sync per clock
+// and SM: 64 keys of head_dim 128 and 16 rows take 512 of them, 1,100 cycles against the ~700 that their bytes
+// take at the copy peak. The tcgen05 kernel multiplies the codes without conversion, but e4m3 terms of an
+// fp32 row would be four. 23 us for 8 sequences of up to 1000 rows, 4 KV heads of 20 rows.
 //
 // Layout of the work. A unit is one sequence's KV head (and block of up to 128 query rows); its
 // tiles of 64 keys follow one another, and all units' tiles form one line that is cut into ranges of
@@ -185,14 +185,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// (x0, x1) as one or two f16 terms, t[0] + t[1]
-template <int TERMS>
-__device__ __forceinline__ void f16_terms(float x0, float x1, uint32_t (&t)[TERMS]) {
+// (x0, x1) as two f16 terms, t[0] + t[1]
+constexpr int kTerms = 2;
+__device__ __forceinline__ void f16_terms(float x0, float x1, uint32_t (&t)[kTerms]) {
   t[0] = pack_f16(x0, x1);
-  if constexpr (TERMS == 2) {
-    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&t[0]));
-    t[1] = pack_f16(x0 - h.x, x1 - h.y);
-  }
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&t[0]));
+  t[1] = pack_f16(x0 - h.x, x1 - h.y);
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm(
@@ -208,23 +206,23 @@ __device__ __forceinline__ void zero(float (&x)[A][4]) {
     for (int e = 0; e < 4; ++e) x[a][e] = 0.f;
 }
 // 16 of the block's own rows as B fragments of f16 terms, and their exponents, in words
-__host__ __device__ constexpr int mma_block_words(int hd, int terms) {
-  return 2 * (hd / 16) * terms * 64 + hd / 8 * terms * 64 + 32;
+__host__ __device__ constexpr int mma_block_words(int hd) {
+  return 2 * (hd / 16) * kTerms * 64 + hd / 8 * kTerms * 64 + 32;
 }
 // shared memory of the kernel, in bytes from its start
 struct MmaSmem {
   int buf, qf, rowf, ml, scales, full, empty, sums, P, bytes;
 };
-__host__ __device__ inline MmaSmem mma_smem(int hd, int mt, int mg, int terms, int depth, int batch) {
+__host__ __device__ inline MmaSmem mma_smem(int hd, int mg, int depth, int batch) {
   MmaSmem s;
-  const int warps = mma_warps(hd), rows = 16 * mt * mg, tl = warps / mg, stages = depth * tl;
+  const int warps = mma_warps(hd), rows = 16 * mg, tl = warps / mg, stages = depth * tl;
   s.buf = stages * 2 * kTile * hd;
   // the lanes that hand their sums over in the first round; before that, 16 rows of the block per lane
-  const int sums = tl / 2 * rows * hd * 4, block = mma_block_words(hd, terms) * 4;
+  const int sums = tl / 2 * rows * hd * 4, block = mma_block_words(hd) * 4;
   s.qf = s.buf + (sums > block ? sums : block);
-  s.rowf = s.qf + rows * hd * 2 * terms;
+  s.rowf = s.qf + rows * hd * 2 * kTerms;
   s.ml = s.rowf + rows * 4;
-  s.scales = s.ml + warps * 16 * mt * 16;
+  s.scales = s.ml + warps * 16 * 16;
   s.full = s.scales + stages * 8;
   s.empty = s.full + stages * 16;
   s.sums = s.empty + stages * 8;
@@ -233,20 +231,19 @@ __host__ __device__ inline MmaSmem mma_smem(int hd, int mt, int mg, int terms, i
   return s;
 }
 
-template <typename T, int HD, int MT>
+template <int HD>
 __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(const AttnArgs p, const MmaPlan pl) {
   constexpr int kWarps = mma_warps(HD);
   constexpr int kThreads = kWarps * 32;
-  constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
   constexpr int NT = HD / 8;   // column tiles of the output
   constexpr int KS = HD / 16;  // k16 steps of q k
   constexpr int CH = HD / 64;  // 16-byte chunks of a key row per thread
   constexpr int kKeyBytes = kTile * HD;
-  constexpr int kWarpRows = 16 * MT;
+  constexpr int kWarpRows = 16;
   constexpr int TPR = kThreads / 16, VB = HD / TPR;  // staging: 16 rows at a time, threads per row, values per thread
-  constexpr int kBlockWords = mma_block_words(HD, TERMS);
+  constexpr int kBlockWords = mma_block_words(HD);
   extern __shared__ __align__(128) uint8_t smem[];
-  const MmaSmem L = mma_smem(HD, MT, pl.mg, TERMS, pl.depth, p.batch);
+  const MmaSmem L = mma_smem(HD, pl.mg, pl.depth, p.batch);
   float* buf = reinterpret_cast<float*>(smem + L.buf);
   uint32_t* qf = reinterpret_cast<uint32_t*>(smem + L.qf);
   float* rowf = reinterpret_cast<float*>(smem + L.rowf);
@@ -362,19 +359,19 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     // 2 * (r / 4) + r % 2 of key tile (r / 2) % 2, so that a thread's four keys are 4 c .. 4 c + 3.
     auto load_block = [&](int kb, float(&x)[VB], float(&y)[VB]) {
       if (kb + row_r < p.block) {
-        load_vals<T, VB>(static_cast<const T*>(p.blk_k) + un.b * p.bk_batch + g * p.bk_head +
+        load_vals<float, VB>(static_cast<const float*>(p.blk_k) + un.b * p.bk_batch + g * p.bk_head +
                              (kb + row_r) * p.bk_row + row_d, pl.vec_blk, x);
-        load_vals<T, VB>(static_cast<const T*>(p.blk_v) + un.b * p.bv_batch + g * p.bv_head +
+        load_vals<float, VB>(static_cast<const float*>(p.blk_v) + un.b * p.bv_batch + g * p.bv_head +
                              (kb + row_r) * p.bv_row + row_d, pl.vec_blk, y);
       }
     };
     auto put_block = [&](int slot, float(&x)[VB], float(&y)[VB]) {
       uint32_t* kf = reinterpret_cast<uint32_t*>(buf) + slot * kBlockWords;
-      uint32_t* vf = kf + 2 * KS * TERMS * 64;
+      uint32_t* vf = kf + 2 * KS * kTerms * 64;
       const int ek = row_exp(x), ev = row_exp(y);
       const float ik = kv8_exp2i(-ek), iv = kv8_exp2i(-ev);
       if (row_d == 0) {
-        float* e = reinterpret_cast<float*>(vf + NT * TERMS * 64);
+        float* e = reinterpret_cast<float*>(vf + NT * kTerms * 64);
         e[row_r] = kv8_exp2i(ek);
         e[16 + row_r] = float(ev);
       }
@@ -384,15 +381,15 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         const int d = row_d + i;
         int c, ks, reg;
         k_place(d, c, ks, reg);
-        uint32_t f[TERMS];
-        f16_terms<TERMS>(scaled(x[i], ik), scaled(x[i + 1], ik), f);
+        uint32_t f[kTerms];
+        f16_terms(scaled(x[i], ik), scaled(x[i + 1], ik), f);
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t) kf[((jk * KS + ks) * TERMS + t) * 64 + (gk * 4 + c) * 2 + reg] = f[t];
-        f16_terms<TERMS>(scaled(y[i], iv), scaled(y[i + 1], iv), f);
+        for (int t = 0; t < kTerms; ++t) kf[((jk * KS + ks) * kTerms + t) * 64 + (gk * 4 + c) * 2 + reg] = f[t];
+        f16_terms(scaled(y[i], iv), scaled(y[i + 1], iv), f);
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
+        for (int t = 0; t < kTerms; ++t) {
           uint16_t* v16 = reinterpret_cast<uint16_t*>(
-              vf + ((d >> 3) * TERMS + t) * 64 + ((d & 7) * 4 + (row_r >> 2)) * 2 + ((row_r >> 1) & 1)) + (row_r & 1);
+              vf + ((d >> 3) * kTerms + t) * 64 + ((d & 7) * 4 + (row_r >> 2)) * 2 + ((row_r >> 1) & 1)) + (row_r & 1);
           v16[0] = uint16_t(f[t]);
           v16[16] = uint16_t(f[t] >> 16);  // the next column's thread, four on
         }
@@ -403,11 +400,11 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     // f16 terms, in the fragment order of the products
     __syncthreads();  // the previous unit's fragments and sums are used up
     {
-      const T* qg = static_cast<const T*>(p.q) + un.b * p.q_batch;
+      const float* qg = static_cast<const float*>(p.q) + un.b * p.q_batch;
       auto load_q = [&](int r, float(&x)[VB]) {
         const int rr = r0 + r;
         if (r < n_rows)
-          load_vals<T, VB>(qg + (rr % p.block) * p.q_row + (g * group + rr / p.block) * p.q_head + row_d, pl.vec_q, x);
+          load_vals<float, VB>(qg + (rr % p.block) * p.q_row + (g * group + rr / p.block) * p.q_head + row_d, pl.vec_q, x);
       };
       auto put_q = [&](int r, float(&x)[VB]) {
         const int e = row_exp(x);
@@ -418,20 +415,20 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         for (int i = 0; i < VB; i += 2) {
           int c, ks, reg;
           k_place(row_d + i, c, ks, reg);
-          uint32_t f[TERMS];
-          f16_terms<TERMS>(scaled(x[i], inv), scaled(x[i + 1], inv), f);
+          uint32_t f[kTerms];
+          f16_terms(scaled(x[i], inv), scaled(x[i + 1], inv), f);
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-            qf[((((r >> 4) * KS + ks) * TERMS + t) * 32 + (r & 7) * 4 + c) * 4 + 2 * reg + ((r >> 3) & 1)] = f[t];
+          for (int t = 0; t < kTerms; ++t)
+            qf[((((r >> 4) * KS + ks) * kTerms + t) * 32 + (r & 7) * 4 + c) * 4 + 2 * reg + ((r >> 3) & 1)] = f[t];
         }
       };
       float x[2][VB] = {}, y[2][VB] = {};
       if (last && p.blk_k) load_block(0, x[0], x[1]);
       load_q(row_r, y[0]);
-      if (MT * mg > 1) load_q(row_r + 16, y[1]);
+      if (mg > 1) load_q(row_r + 16, y[1]);
       if (last && p.blk_k) put_block(0, x[0], x[1]);
       put_q(row_r, y[0]);
-      if (MT * mg > 1) put_q(row_r + 16, y[1]);
+      if (mg > 1) put_q(row_r + 16, y[1]);
       for (int r = row_r + 32; r < cta_rows; r += 32) {
         float z[2][VB] = {};
         load_q(r, z[0]);
@@ -441,25 +438,19 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       }
     }
     __syncthreads();
-    float cf[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      cf[mt][0] = rowf[my_mg * kWarpRows + mt * 16 + gq];
-      cf[mt][1] = rowf[my_mg * kWarpRows + mt * 16 + gq + 8];
-    }
-    const uint4* my_q = reinterpret_cast<const uint4*>(qf) + my_mg * MT * KS * TERMS * 32 + lane;
+    float cf[2];
+    cf[0] = rowf[my_mg * kWarpRows + gq];
+    cf[1] = rowf[my_mg * kWarpRows + gq + 8];
+    const uint4* my_q = reinterpret_cast<const uint4*>(qf) + my_mg * KS * kTerms * 32 + lane;
 
-    float o[MT][NT][4], m[MT][2], l[MT][2];
+    float o[NT][4], m[2], l[2];
     int rv = -200, top_rv = -200;  // the sums' value exponent, and the largest seen
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.f;
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
-    }
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
 
     // scores s of NJ 8-key tiles -> weights in place (f16-ready), sums and references brought up to date.
     // bad(j, e): key column e of tile j is not to be attended; `some`: there are such.
@@ -470,78 +461,63 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (bad(j, e)) {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = s[mt][j][2 + e] = kLowest;
-            }
+            if (bad(j, e)) s[j][e] = s[j][2 + e] = kLowest;
       }
-      float top[MT][2];
+      float top[2];
       bool grown = false;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int h = 0; h < 2; ++h) {
+        float mx = kLowest;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = kLowest;
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * h], s[mt][j][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          top[mt][h] = mx * (cf[mt][h] * k_scale);
-          grown |= top[mt][h] > m[mt][h] + kPGrow;
-        }
+        for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        top[h] = mx * (cf[h] * k_scale);
+        grown |= top[h] > m[h] + kPGrow;
+      }
       top_rv = max(top_rv, ev);
       const int want_rv = ev > rv || ev < rv - 10 ? max(ev, top_rv - 40) : rv;
       if (__any_sync(0xffffffffu, grown) || want_rv != rv) {
         const float fv = rv <= -200 ? 0.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
         rv = want_rv;
+        float f[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float f[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float mn = top[mt][h] > m[mt][h] + kPGrow ? top[mt][h] : m[mt][h];
-            const float a = m[mt][h] == mn ? 1.f : ex2(m[mt][h] - mn);
-            m[mt][h] = mn;
-            l[mt][h] *= a;
-            f[h] = a * fv;
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][n][e] *= f[e >> 1];
+        for (int h = 0; h < 2; ++h) {
+          const float mn = top[h] > m[h] + kPGrow ? top[h] : m[h];
+          const float a = m[h] == mn ? 1.f : ex2(m[h] - mn);
+          m[h] = mn;
+          l[h] *= a;
+          f[h] = a * fv;
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] *= f[e >> 1];
       }
       const int dv = max(ev - rv, -60);  // <= 0
       const float back = kv8_exp2i(-dv);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int h = 0; h < 2; ++h) {
+        const float c = cf[h] * k_scale, off = kPScale + float(dv) - m[h];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float c = cf[mt][h] * k_scale, off = kPScale + float(dv) - m[mt][h];
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) s[mt][j][2 * h + e] = ex2(fmaf(s[mt][j][2 * h + e], c, off));
-        }
+          for (int e = 0; e < 2; ++e) s[j][2 * h + e] = ex2(fmaf(s[j][2 * h + e], c, off));
+      }
       if (some) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (bad(j, e)) {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = s[mt][j][2 + e] = 0.f;
-            }
+            if (bad(j, e)) s[j][e] = s[j][2 + e] = 0.f;
       }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int h = 0; h < 2; ++h) {
+        float sum = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) sum += s[mt][j][2 * h] + s[mt][j][2 * h + 1];
-          l[mt][h] = fmaf(sum, back, l[mt][h]);
-        }
+        for (int j = 0; j < NJ; ++j) sum += s[j][2 * h] + s[j][2 * h + 1];
+        l[h] = fmaf(sum, back, l[h]);
+      }
     };
 
     // ---- the block's own rows, 16 at a time: the first by the lane behind the unit's last tile, while the
@@ -549,25 +525,22 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     if (last && p.blk_k) {
       auto block_tile = [&](int kb) {
         const uint2* kf = reinterpret_cast<const uint2*>(buf) + lane;
-        const uint2* vf = kf + 2 * KS * TERMS * 32;
+        const uint2* vf = kf + 2 * KS * kTerms * 32;
         const float* ex = reinterpret_cast<const float*>(reinterpret_cast<uint32_t*>(buf) + kBlockWords - 32);
-        float s[MT][2][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) zero(s[mt]);
+        float s[2][4];
+        zero(s);
 #pragma unroll 4
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int tq = 0; tq < TERMS; ++tq) {
-            uint4 q[MT];
+          for (int tq = 0; tq < kTerms; ++tq) {
+            uint4 q;
+            q = my_q[((ks) * kTerms + tq) * 32];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) q[mt] = my_q[((mt * KS + ks) * TERMS + tq) * 32];
-#pragma unroll
-            for (int tk = 0; tk < TERMS; ++tk)
+            for (int tk = 0; tk < kTerms; ++tk)
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const uint2 k = kf[((j * KS + ks) * TERMS + tk) * 32];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) mma(s[mt][j], q[mt], k.x, k.y);
+                const uint2 k = kf[((j * KS + ks) * kTerms + tk) * 32];
+                mma(s[j], q, k.x, k.y);
               }
           }
         float ev = -200.f;
@@ -578,36 +551,28 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float f = ex[4 * cq + 2 * j + e];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              s[mt][j][e] *= f;
-              s[mt][j][2 + e] *= f;
-            }
+            s[j][e] *= f;
+            s[j][2 + e] *= f;
           }
         weigh(std::integral_constant<int, 2>(), s, 1.f, int(ev), kb + 16 > p.block,
               [&](int j, int e) { return kb + 4 * cq + 2 * j + e >= p.block; });
-        uint4 pf[MT][TERMS];
+        uint4 pf[kTerms];
+        uint32_t f[4][kTerms];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t f[4][TERMS];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = i >> 1;
-            const float f0 = ex2(ex[16 + 4 * cq + 2 * j] - ev), f1 = ex2(ex[16 + 4 * cq + 2 * j + 1] - ev);
-            f16_terms<TERMS>(s[mt][j][2 * (i & 1)] * f0, s[mt][j][2 * (i & 1) + 1] * f1, f[i]);
-          }
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t) pf[mt][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
+        for (int i = 0; i < 4; ++i) {
+          const int j = i >> 1;
+          const float f0 = ex2(ex[16 + 4 * cq + 2 * j] - ev), f1 = ex2(ex[16 + 4 * cq + 2 * j + 1] - ev);
+          f16_terms(s[j][2 * (i & 1)] * f0, s[j][2 * (i & 1) + 1] * f1, f[i]);
         }
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) pf[t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int tv = 0; tv < TERMS; ++tv) {
-            const uint2 v = vf[(n * TERMS + tv) * 32];
+          for (int tv = 0; tv < kTerms; ++tv) {
+            const uint2 v = vf[(n * kTerms + tv) * 32];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int tp = 0; tp < TERMS; ++tp) mma(o[mt][n], pf[mt][tp], v.x, v.y);
+            for (int tp = 0; tp < kTerms; ++tp) mma(o[n], pf[tp], v.x, v.y);
           }
       };
       for (int kb = 0; kb < p.block; kb += 16) {
@@ -634,17 +599,15 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
       const uint8_t* kt = smem + st * 2 * kKeyBytes;
       const uint8_t* vt = kt + kKeyBytes;
       if (any) {
-        float s[MT][8][4];
+        float s[8][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
         // scores: column n of key tile j is key 16 * (n / 2) + 2 j + n % 2, so that a thread ends up with
         // the 16 keys whose codes of one value column lie together
         const uint8_t* krow = kt + (16 * (gq >> 1) + (gq & 1)) * HD;
-        // four key tiles at a time: their products are independent, a chain's steps are 4 MT products apart
+        // four key tiles at a time: their products are independent, a chain's steps are four products apart
 #pragma unroll 1
         for (int ch = 0; ch < CH; ++ch) {
           const uint32_t chunk = HD == 64 ? cq : 2 * cq + (ch & 1);
@@ -658,28 +621,24 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
               k[j] = *reinterpret_cast<const uint4*>(krow + t * HD + at * 16);
             }
 #pragma unroll
-            for (int tq = 0; tq < TERMS; ++tq) {
+            for (int tq = 0; tq < kTerms; ++tq) {
               float t4[4][4];
-              if constexpr (TERMS == 2) zero(t4);
+              zero(t4);
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
-                uint4 q[MT];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) q[mt] = my_q[((mt * KS + ch * 4 + w) * TERMS + tq) * 32];
+                uint4 q;
+                q = my_q[((ch * 4 + w) * kTerms + tq) * 32];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   uint32_t b0, b1;
                   e4m3x4_to_f16(w == 0 ? k[j].x : w == 1 ? k[j].y : w == 2 ? k[j].z : k[j].w, b0, b1);
-#pragma unroll
-                  for (int mt = 0; mt < MT; ++mt) mma(TERMS == 2 ? t4[j] : s[mt][j4 + j], q[mt], b0, b1);
+                  mma(t4[j], q, b0, b1);
                 }
               }
-              if constexpr (TERMS == 2) {  // MT is 1
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+              for (int j = 0; j < 4; ++j)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) s[0][j4 + j][e] += t4[j][e];
-              }
+                for (int e = 0; e < 4; ++e) s[j4 + j][e] += t4[j][e];
             }
           }
         }
@@ -690,18 +649,16 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
         ok = mbar_wait(full + 2 * st + 1, (i / S) & 1);
         weigh(std::integral_constant<int, 8>(), s, k_scale, kv8_exponent(scales[st].y), nv < kTile,
                                      [&](int j, int e) { return 16 * cq + 2 * j + e >= nv; });
-        uint4 pf[MT][4][TERMS];
+        uint4 pf[4][kTerms];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int w = 0; w < 4; ++w) {
+          uint32_t f[4][kTerms];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t f[4][TERMS];
+          for (int x = 0; x < 4; ++x)
+            f16_terms(s[2 * w + (x >> 1)][2 * (x & 1)], s[2 * w + (x >> 1)][2 * (x & 1) + 1], f[x]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              f16_terms<TERMS>(s[mt][2 * w + (x >> 1)][2 * (x & 1)], s[mt][2 * w + (x >> 1)][2 * (x & 1) + 1], f[x]);
-#pragma unroll
-            for (int t = 0; t < TERMS; ++t) pf[mt][w][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
-          }
+          for (int t = 0; t < kTerms; ++t) pf[w][t] = make_uint4(f[0][t], f[1][t], f[2][t], f[3][t]);
+        }
         // values: columns 8 n + gq, this thread's 16 keys. Codes behind the length are cleared: a weight of
         // zero would not take a NaN there out
         const uint8_t* vrow = vt + gq * kTile + cq * 16;
@@ -726,7 +683,7 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
             }
           }
           float t4[4][4];
-          if constexpr (TERMS == 2) zero(t4);
+          zero(t4);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -734,16 +691,12 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
               uint32_t b0, b1;
               e4m3x4_to_f16(w == 0 ? v[n].x : w == 1 ? v[n].y : w == 2 ? v[n].z : v[n].w, b0, b1);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) mma(TERMS == 2 ? t4[n] : o[mt][n4 + n], pf[mt][w][t], b0, b1);
+              for (int t = 0; t < kTerms; ++t) mma(t4[n], pf[w][t], b0, b1);
             }
-          if constexpr (TERMS == 2) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[0][n4 + n][e] += t4[n][e];
-          }
+            for (int e = 0; e < 4; ++e) o[n4 + n][e] += t4[n][e];
         }
       } else if (ok) {  // nothing to read; its values' half may still be on its way
         ok = mbar_wait(full + 2 * st + 1, (i / S) & 1);
@@ -767,90 +720,77 @@ __global__ void __launch_bounds__(mma_warps(HD) * 32, 1) kv8_attn_mma_kernel(con
     const int busy = min(tl, a1 - a0 + (last && p.blk_k ? (p.block + 15) / 16 : 0));
     const int wrow = warp * kWarpRows;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = l[mt][h];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (cq == 0) ml[wrow + mt * 16 + h * 8 + gq] = make_float4(m[mt][h], x, float(rv), 0.f);
-      }
+    for (int h = 0; h < 2; ++h) {
+      float x = l[h];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if (cq == 0) ml[wrow + h * 8 + gq] = make_float4(m[h], x, float(rv), 0.f);
+    }
     __syncthreads();
-    float M[MT][2], W[MT][2], E = -200.f;
+    float M[2], W[2], E = -200.f;
     for (int t = 0; t < tl; ++t) E = fmaxf(E, ml[(my_mg * tl + t) * kWarpRows].z);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h) {
+      const float4* row = ml + my_mg * tl * kWarpRows + h * 8 + gq;
+      float a = -INFINITY, w = 0.f;
+      for (int t = 0; t < tl; ++t) a = fmaxf(a, row[t * kWarpRows].x);
+      const float ref = a == -INFINITY ? 0.f : a;
+      for (int t = 0; t < tl; ++t) w = fmaf(row[t * kWarpRows].y, ex2(row[t * kWarpRows].x - ref), w);
+      M[h] = a;
+      W[h] = w;
+      const float f = ex2(m[h] - ref + fmaxf(float(rv) - E, -126.f));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4* row = ml + my_mg * tl * kWarpRows + mt * 16 + h * 8 + gq;
-        float a = -INFINITY, w = 0.f;
-        for (int t = 0; t < tl; ++t) a = fmaxf(a, row[t * kWarpRows].x);
-        const float ref = a == -INFINITY ? 0.f : a;
-        for (int t = 0; t < tl; ++t) w = fmaf(row[t * kWarpRows].y, ex2(row[t * kWarpRows].x - ref), w);
-        M[mt][h] = a;
-        W[mt][h] = w;
-        const float f = ex2(m[mt][h] - ref + fmaxf(float(rv) - E, -126.f));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[mt][n][2 * h] *= f;
-          o[mt][n][2 * h + 1] *= f;
-        }
+      for (int n = 0; n < NT; ++n) {
+        o[n][2 * h] *= f;
+        o[n][2 * h + 1] *= f;
       }
+    }
     for (int half = tl / 2; half >= 1; half /= 2) {
       if (half >= busy) continue;
       float4* slot = reinterpret_cast<float4*>(buf) + (my_mg * half + x_tl % half) * (kWarpRows * HD / 4) + lane;
       if (x_tl >= half && x_tl < min(2 * half, busy)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            slot[(mt * NT + n) * 32] = make_float4(o[mt][n][0], o[mt][n][1], o[mt][n][2], o[mt][n][3]);
+        for (int n = 0; n < NT; ++n)
+          slot[n * 32] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
       }
       __syncthreads();
       if (x_tl < half && x_tl + half < busy) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float4 x = slot[(mt * NT + n) * 32];
-            o[mt][n][0] += x.x;
-            o[mt][n][1] += x.y;
-            o[mt][n][2] += x.z;
-            o[mt][n][3] += x.w;
-          }
+        for (int n = 0; n < NT; ++n) {
+          const float4 x = slot[n * 32];
+          o[n][0] += x.x;
+          o[n][1] += x.y;
+          o[n][2] += x.z;
+          o[n][3] += x.w;
+        }
       }
       __syncthreads();
     }
     if (x_tl == 0) {
       const int slot = 2 * blockIdx.x + (a0 == 0 && un.t > 0 ? 0 : 1);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int h = 0; h < 2; ++h) {
+        const int r = my_mg * kWarpRows + h * 8 + gq;
+        if (whole) {
+          if (r >= n_rows) continue;
+          const int rr = r0 + r;
+          float* out = static_cast<float*>(p.out) +
+                   ((int64_t(un.b) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + 2 * cq;
+          const float inv = W[h] == 0.f ? 0.f : 1.f / W[h], fe = kv8_exp2i(max(int(E), -126));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = my_mg * kWarpRows + mt * 16 + h * 8 + gq;
-          if (whole) {
-            if (r >= n_rows) continue;
-            const int rr = r0 + r;
-            T* out = static_cast<T*>(p.out) +
-                     ((int64_t(un.b) * p.block + rr % p.block) * p.n_heads + g * group + rr / p.block) * HD + 2 * cq;
-            const float inv = W[mt][h] == 0.f ? 0.f : 1.f / W[mt][h], fe = kv8_exp2i(max(int(E), -126));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float y0 = W[mt][h] == 0.f ? 0.f : o[mt][n][2 * h] * inv * fe;
-              const float y1 = W[mt][h] == 0.f ? 0.f : o[mt][n][2 * h + 1] * inv * fe;
-              if constexpr (std::is_same<T, float>::value)
-                *reinterpret_cast<float2*>(out + 8 * n) = make_float2(y0, y1);
-              else
-                *reinterpret_cast<__nv_bfloat162*>(out + 8 * n) = __floats2bfloat162_rn(y0, y1);
-            }
-          } else {
-            float* dst = pl.sp.part + (int64_t(slot) * cta_rows + r) * HD + 2 * cq;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-            if (cq == 0) pl.sp.ml[int64_t(slot) * cta_rows + r] = make_float4(M[mt][h], W[mt][h], E, 0.f);
+          for (int n = 0; n < NT; ++n) {
+            const float y0 = W[h] == 0.f ? 0.f : o[n][2 * h] * inv * fe;
+            const float y1 = W[h] == 0.f ? 0.f : o[n][2 * h + 1] * inv * fe;
+            *reinterpret_cast<float2*>(out + 8 * n) = make_float2(y0, y1);
           }
+        } else {
+          float* dst = pl.sp.part + (int64_t(slot) * cta_rows + r) * HD + 2 * cq;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+          if (cq == 0) pl.sp.ml[int64_t(slot) * cta_rows + r] = make_float4(M[h], W[h], E, 0.f);
         }
+      }
     }
     a0 = a1;
   }
@@ -956,43 +896,38 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv8_attn_combine_kernel(co
 constexpr int kMmaSmemMax = 232448;  // 227 KB
 
 struct MmaShape {
-  int mt, mg, row_blocks, cta_rows;
+  int mg, row_blocks, cta_rows;
 };
-// Query rows of a KV head -> rows per warp and warps per tile: 16 rows where that is all, else 32 (one
-// 16-row tile at head_dim 256 and in two terms, whose sums or weights fill the registers), and more
-// warps over the same tile up to 128 rows (64 at head_dim 256).
-MmaShape mma_shape(int rows, int hd, int dtype) {
+// Query rows of a KV head -> warps per tile: 16 rows each, up to 128 rows (64 at head_dim 256).
+MmaShape mma_shape(int rows, int hd) {
   MmaShape s;
-  s.mt = rows <= 16 || hd == 256 || dtype == DSM_DT_F32 ? 1 : 2;
   const int most = hd == 256 ? 64 : 128;
   s.mg = 1;
-  while (16 * s.mt * s.mg < std::min(rows, most)) s.mg *= 2;
-  s.cta_rows = 16 * s.mt * s.mg;
+  while (16 * s.mg < std::min(rows, most)) s.mg *= 2;
+  s.cta_rows = 16 * s.mg;
   s.row_blocks = int(ceil_div(rows, s.cta_rows));
   return s;
 }
 
-template <typename T, int HD, int MT>
+template <int HD>
 int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cudaStream_t s) {
-  constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
   int depth = std::max(kMaxDepth, sh.mg);
-  while (depth > 1 && mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes > kMmaSmemMax) --depth;
-  const int smem = mma_smem(HD, MT, sh.mg, TERMS, depth, a.batch).bytes;
+  while (depth > 1 && mma_smem(HD, sh.mg, depth, a.batch).bytes > kMmaSmemMax) --depth;
+  const int smem = mma_smem(HD, sh.mg, depth, a.batch).bytes;
   if (smem > kMmaSmemMax) return DSM_ERR_UNSUPPORTED;
   pl.depth = depth;
-  auto k = kv8_attn_mma_kernel<T, HD, MT>;
+  auto k = kv8_attn_mma_kernel<HD>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("gqa_attn_kv8 smem attribute");
   k<<<unsigned(ctas), mma_warps(HD) * 32, size_t(smem), s>>>(a, pl);
   const int st = check_launch("gqa_attn_kv8");
-  return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, std::is_same<T, float>::value ? DSM_DT_F32 : DSM_DT_BF16, s);
+  return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, DSM_DT_F32, s);
 }
 
 size_t mma_ws_bytes(int cta_rows, int hd) { return split_ws_bytes(num_sms(), cta_rows, hd); }
 
-template <typename T>
 int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
-  const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd, sizeof(T) == 4 ? DSM_DT_F32 : DSM_DT_BF16);
+  const MmaShape sh = mma_shape(a.n_heads / a.n_kv * a.block, hd);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * sh.row_blocks;
   const int ctas = int(std::min<int64_t>(num_sms(), most));
   MmaPlan pl;
@@ -1006,15 +941,14 @@ int run_mma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   pl.sp.ctas = ctas;
   if (!split_fits(a, pl.sp)) return DSM_ERR_UNSUPPORTED;
   pl.depth = 0;
-  pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 4 * sizeof(T));
-  pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 4 * sizeof(T)) &&
-               vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 4 * sizeof(T));
+  pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 16);
+  pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 16) &&
+               vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 16);
   split_ws(pl.sp, ws, hd);
-  constexpr int kWide = sizeof(T) == 4 ? 1 : 2;
   switch (hd) {
-    case 64: return sh.mt == 1 ? launch_mma<T, 64, 1>(a, sh, pl, ctas, s) : launch_mma<T, 64, kWide>(a, sh, pl, ctas, s);
-    case 128: return sh.mt == 1 ? launch_mma<T, 128, 1>(a, sh, pl, ctas, s) : launch_mma<T, 128, kWide>(a, sh, pl, ctas, s);
-    default: return launch_mma<T, 256, 1>(a, sh, pl, ctas, s);
+    case 64: return launch_mma<64>(a, sh, pl, ctas, s);
+    case 128: return launch_mma<128>(a, sh, pl, ctas, s);
+    default: return launch_mma<256>(a, sh, pl, ctas, s);
   }
 }
 
@@ -1052,7 +986,7 @@ extern "C" size_t dsm_gqa_attn_kv8_workspace_bytes(int batch, int block, int n_h
       !kv8_head_dim_ok(head_dim))
     return 0;
   const int rows = n_heads / n_kv * block;
-  return std::max(mma_ws_bytes(mma_shape(rows, head_dim, DSM_DT_F32).cta_rows, head_dim), kv8_umma_ws_bytes(rows, head_dim));
+  return std::max(mma_ws_bytes(mma_shape(rows, head_dim).cta_rows, head_dim), kv8_umma_ws_bytes(rows, head_dim));
 }
 
 extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const int32_t* block_table,
@@ -1111,7 +1045,7 @@ extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const
   if (attn_kernel() == 0) {
     int st = DSM_ERR_UNSUPPORTED;
     if (d->dtype == DSM_DT_F32)
-      st = run_mma<float>(a, d->head_dim, ws, s);
+      st = run_mma(a, d->head_dim, ws, s);
     else if (d->block <= kUmmaMaxBlock)
       st = kv8_umma(a, d->head_dim, ws, s);
     if (st != DSM_ERR_UNSUPPORTED) return st;

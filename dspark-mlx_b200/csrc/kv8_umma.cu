@@ -655,7 +655,8 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         float ks = 0.f;
         bool live;
         if (own) {
-          for (int j = 0; j < p.block; ++j) ev = max(ev, int(keys[j].y));
+          // a page's exponent is that of many more values than a row's: mostly a step or two above
+          for (int j = 0; j < p.block; ++j) ev = max(ev, int(keys[j].y) + 1);
           low = ev;
           live = gtid < p.block;
           if (live) {
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           top = fmaxf(top, fmaxf(fmaxf(y[r], y[r + 1]), fmaxf(y[r + 2], y[r + 3])));
         }
         if (any_of_group(grp, (live && top > kPMax) || i == 0 || want_rv != rv)) {
-          // new references: every row whose maximum lies above its own (all of them at first)
+          // new references: every row whose maximum has risen since its own was set (all of them at first)
 #pragma unroll
           for (int r = 0; r < RW; ++r) {
             const float x = redux_max(live ? y[r] : kLowest);
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           group_sync(grp);
           if (gtid < RW) {
             const float x = fmaxf(fmaxf(red[gtid], red[16 + gtid]), fmaxf(red[32 + gtid], red[48 + gtid]));
-            const float up = x == kLowest ? 0.f : i == 0 || x > kPExp ? x + (kPHead - kPExp) : 0.f;
+            const float up = x == kLowest ? 0.f : i == 0 || x > kPExp - kPHead ? x + (kPHead - kPExp) : 0.f;
             row_m[g0 + gtid] -= up;
             red[gtid] = up;
             row_a[g0 + gtid] = ex2(-up);
@@ -958,9 +959,9 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   if (groups * std::max(hd, kTile) > 0x7fffffff) return DSM_ERR_UNSUPPORTED;  // rows of the TMA maps
   const int most_ctas = ctas_per_sm(nr, hd) * num_sms();
   pl.sp.ctas = int(std::min<int64_t>(most_ctas, most));
-  pl.sp.cost = 6;
-  pl.sp.snap = 4;
-  pl.sp.least = 12;
+  pl.sp.cost = 10;
+  pl.sp.snap = 2;
+  pl.sp.least = 8;
   if (!split_fits(a, pl.sp)) return DSM_ERR_UNSUPPORTED;
   split_ws(pl.sp, ws, hd);
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 8);
