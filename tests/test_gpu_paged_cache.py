@@ -131,6 +131,30 @@ def test_extend_leaves_out_what_does_not_fit(short):
         _lib.raise_device_error()
 
 
+@pytest.mark.parametrize("short,page", [("pages", 64), ("pages", 192), ("rows", 1024), ("negative length", 128)])
+def test_a_long_step_leaves_out_what_does_not_fit(short, page):
+    """As above with more rows than one CTA writes; sequences without new rows lie between the others."""
+    b = 90
+    lengths, new, table, free, n_free, tg = _tables_case(7, b, page, 5 * page, 6 * page, 4 * b, most=14)
+    new[3] = 5 * page
+    max_rows = sum(new) + 11
+    assert max_rows > 3000
+    if short == "pages":
+        n_free = 60
+    elif short == "rows":
+        max_rows = max_rows * 2 // 3
+    else:
+        lengths[3] = -1
+    want = po.paged_extend(lengths, new, table, free, n_free, page, max_rows)
+    assert want[6]
+    L, F, N, rows = _run_extend(lengths, new, tg, free, n_free, page, max_rows)
+    assert L.tolist() == want[0] and tg.tolist() == want[1] and N.tolist() == [want[2]]
+    assert rows.cu_rows.tolist() == want[3] and rows.slot_map.tolist() == want[4]
+    assert rows.positions.tolist() == want[5]
+    with pytest.raises(_lib.DsmError, match="ran out"):
+        _lib.raise_device_error()
+
+
 def test_trim_refuses_more_pages_than_the_pool_holds():
     lengths, new, table, free, n_free, tg = _tables_case(2, 5, 64, 300, 1, 10)
     lengths = [64 * 3] * 5
@@ -222,6 +246,43 @@ def test_append_matches_the_oracle(dtype, hd, page, n_kv, n_runs, most):
     # the same rows again: nothing moves but pages that start afresh with the same rows
     _check_append(layer, (pool[0], pool[1], pool[2], pool[3]), rk, rv, slots)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,hd,page,n_kv,longest", [
+    (torch.bfloat16, 64, 64, 16, 1), (torch.bfloat16, 128, 64, 8, 40), (torch.float32, 64, 1024, 8, 1024),
+    (torch.bfloat16, 64, 1024, 8, 1024), (torch.bfloat16, 256, 192, 8, 192),
+])
+def test_append_of_many_rows(dtype, hd, page, n_kv, longest):
+    """Rows enough for windows of 64: runs of a row each, of a warp's size and longer ones side by side, and
+    runs that pass the window and the 256 rows behind its start, in order and not."""
+    r = random.Random(page + longest)
+    rows = 64 * (4 * 148 // n_kv + 9)
+    slots, n_pages = [], 0
+    while len(slots) < rows:
+        n = r.choice([1, 2, r.randint(1, longest), r.randint(1, longest), longest])
+        first = r.randint(0, page - n)
+        run = [n_pages * page + first + j for j in range(n)]
+        if r.random() < 0.2:
+            r.shuffle(run)
+        slots += run + [-1] * (r.random() < 0.1)
+        n_pages += 1
+    k, ks, v, vs, layer = _pool(hd, n_pages, n_kv, page, hd)
+    g = torch.Generator().manual_seed(page)
+    mag = torch.exp2(torch.randint(-14, 14, (len(slots), 1, 1), generator=g).float())
+    rk, rv = ((torch.randn(len(slots), n_kv, hd, generator=g) * mag).to(dtype) for _ in range(2))
+    _check_append(layer, (k, ks, v, vs), rk, rv, slots)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("where", [0, 5, 8, 15, 16, 17, 63])
+def test_append_infinities_anywhere_in_a_run(where):
+    """An infinity or NaN takes no part in the scale, wherever its row and column fall in a run."""
+    k, ks, v, vs, layer = _pool(2, 3, 2, 64, 128)
+    g = torch.Generator().manual_seed(where)
+    rk, rv = (torch.randn(70, 2, 128, generator=g).bfloat16() for _ in range(2))
+    rk[where, 1, 127 - where], rk[where, 0, where] = float("inf"), float("nan")
+    rv[where, 0, where], rv[where + 1, 1, 7] = float("-inf"), float("nan")
+    _check_append(layer, (k, ks, v, vs), rk, rv, list(range(64)) + list(range(150, 156)))
 
 
 @pytest.mark.parametrize("order", ["head first", "interleaved", "offset", "broadcast rows"])
@@ -455,6 +516,80 @@ def test_attention_is_the_same_twice_and_on_another_stream():
                 outs.append(pc.gqa_attention_kv8(q, c["layer"], c["tg"], n, *blk))
     torch.cuda.synchronize()
     assert all(torch.equal(o, a) for o in outs)
+
+
+@pytest.mark.parametrize("dtype,s,group,hd", [
+    (BF, 1, 7, 128), (BF, 3, 4, 64), (BF, 5, 4, 128), (BF, 3, 8, 128), (BF, 5, 8, 256), (BF, 6, 8, 64), (BF, 17, 2, 128),
+    (BF, 16, 4, 128), (BF, 13, 6, 256), (BF, 31, 4, 64), (BF, 64, 1, 128), (BF, 64, 3, 64), (BF, 65, 1, 128), (BF, 130, 2, 64),
+    (F32, 1, 7, 128), (F32, 9, 4, 64), (F32, 16, 8, 128), (F32, 43, 3, 64), (F32, 23, 3, 256), (F32, 70, 2, 128),
+])
+def test_attention_any_number_of_query_rows(dtype, s, group, hd):
+    """One row of a KV head to several blocks of them, blocks of own rows that fill a step and more, over a
+    sequence that many CTAs share, a short one, one of its own rows alone and one that ends at a page."""
+    c = _attn_case(s * group + hd, [2500, 70, 0, 256], s, 2, group, hd, 64, dtype)
+    _check_attn(c, norm=2.0 ** -8 if dtype == BF else 2.0 ** -20)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,lengths,s,page,with_block", [
+    (BF, [700, 0, 64, 1], 3, 64, True), (F32, [700, 0, 64, 1], 3, 128, True), (BF, [333], 1, 64, False),
+])
+def test_attention_on_the_cuda_cores(dtype, lengths, s, page, with_block):
+    L = _lib.lib()
+    c = _attn_case(9, lengths, s, 2, 4, 128, page, dtype, with_block)
+    a = _check_attn(c)
+    _lib.check(L.dsm_set_attn_kernel(1))
+    try:
+        b = _check_attn(c)
+    finally:
+        _lib.check(L.dsm_set_attn_kernel(_lib.ATTN_KERNEL_DEFAULT))
+    assert not torch.equal(a, b)  # another kernel, other roundings
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 64), (BF, 256), (F32, 128), (F32, 256)])
+def test_attention_of_the_largest_batch(dtype, hd):
+    r = random.Random(hd)
+    lengths = [r.choice([0, 0, 1, 5, 64, 65, 130]) for _ in range(8192)]
+    c = _attn_case(5, lengths, 1, 1, 2, hd, 64, dtype)
+    _check_attn(c)
+    assert _lib.device_error() == 0
+
+
+def test_attention_pages_of_unlike_scales_within_a_step():
+    """A step takes two groups of 64 keys: pages with scales 2^25 apart, and pages that are none, in either half."""
+    c = _attn_case(4, [640, 600, 200], 5, 2, 4, 128, 64, BF, e_lo=-24, e_hi=2)
+    _check_attn(c, scale=2.0 ** -12)
+    for i, cols in ((0, (1, 4)), (1, (0, 9)), (2, (2,))):
+        for j in cols:
+            c["table"][i][j] = -1 if j % 2 else 10 ** 6
+    c["tg"].copy_(torch.tensor(c["table"], dtype=torch.int32))
+    _check_attn(c, scale=2.0 ** -12)
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
+
+
+def test_two_captured_attentions_replay_side_by_side():
+    """Two graphs, each with its own workspace, on two streams at once, over and over."""
+    cases = [_attn_case(i, n, s, 2, 4, 128, 64, BF) for i, (n, s) in enumerate((([3000, 9], 7), ([700, 0, 4000], 3)))]
+    want, graphs, outs = [], [], []
+    for c in cases:
+        want.append(_check_attn(c))
+        args = [c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), *[t.to(DEV) for t in c["blk"]]]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pc.gqa_attention_kv8(*args))
+        graphs.append((g, args))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 def test_attention_bad_tables_are_skipped_and_reported():
