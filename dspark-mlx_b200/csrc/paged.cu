@@ -11,12 +11,15 @@
 //   dsm_paged_trim    sequence i shrinks to keep_i tokens; its surplus pages go back on the stack in
 //                     the mirrored order, so a trim to the lengths before an extend restores the stack.
 //
-// Bound by latency: a decode step moves a few KB, a prefill step 12 bytes per row. One kernel of
-// one cluster does the whole step. Every CTA scans all sequences itself (their lengths come from
-// L2), then the CTAs share out the rows and pages by flat index, each finding its sequence by
+// Bound by latency: a decode step moves a few KB, a prefill step 12 bytes per row. A decode step is one
+// CTA's. A prefill step goes to a cluster: every CTA scans all sequences itself (their lengths come
+// from L2), then the CTAs share out the pages by flat index, each finding its sequence by
 // bisection in shared memory, so that one long sequence among short ones costs no more than an
 // even batch. The cluster barrier between the reads of lengths / n_free and their updates is
-// what lets the update be in place: a captured step replays on the buffers it leaves behind.
+// what lets the update be in place: a captured step replays on the buffers it leaves behind. The rows of
+// such a step are written by a second kernel on the whole GPU: 130,000 rows of 253 sequences took
+// a cluster of 8 alone 21 us, of 47 with a bisection per row; extend and trim together now take 15 us (a decode
+// step of 64 sequences 8.3 us, two launches).
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
