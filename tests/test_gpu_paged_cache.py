@@ -731,6 +731,41 @@ def test_a_captured_step_replays_as_the_lengths_change():
     del graphs, gr
 
 
+def test_a_captured_prefill_replays():
+    """A step of more rows than one CTA writes, captured: extend's two kernels, append and attend, then a trim."""
+    b, n_kv, hd, page, most = 40, 2, 64, 64, 4000
+    caches = [pc.PagedKVCache(1, 400, n_kv, hd, b, 40, page_size=page) for _ in range(2)]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    mk = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    new, keep = i32([0] * b), i32([0] * b)
+    x, q = [mk(most, n_kv, hd) for _ in range(2)], mk(b, 2, n_kv * 4, hd)
+
+    def step(cache):
+        rows = cache.extend(new, most)
+        cache.append(0, *x, rows)
+        out = cache.attend(0, q)
+        cache.trim(keep)
+        return out, rows
+
+    step(caches[0])
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, rows = step(caches[0])
+    r = random.Random(8)
+    for i in range(6):
+        new.copy_(i32([r.choice([0, 1, r.randint(0, 130)]) for _ in range(b)]))
+        keep.copy_(i32([r.choice([0, 70, 10 ** 6]) for _ in range(b)]))
+        gr.replay()
+        want, want_rows = step(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        assert all(torch.equal(a, c) for a, c in zip(rows, want_rows))
+        assert torch.equal(caches[0].lengths, caches[1].lengths) and torch.equal(caches[0].n_free, caches[1].n_free)
+        assert torch.equal(caches[0].free_pages, caches[1].free_pages)
+    assert _lib.device_error() == 0
+    del gr
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_qwen3_layer_over_the_paged_cache(dtype):
     """``append_paged`` + ``forward_paged`` of a Qwen3 draft layer for sequences of different lengths against the
