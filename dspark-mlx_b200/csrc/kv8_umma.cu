@@ -8,7 +8,7 @@
 // 448, is the sum of two e4m3 terms (hi = e4m3(x), lo = e4m3(x - hi): exact for bf16's 8 bits wherever
 // the residual reaches e4m3's normals, 2^-10 of a unit off elsewhere, of a row maximum of 224 to 448).
 // The weights are p = 2^(s - m + 8), an e4m3 term and an e5m2 residual: 2^-7 of a weight off at most where it
-// is above 2^-15 of the largest, and nothing above 2^-22 of it is lost. m is the row's reference: its maximum
+// is above 2^-14 of the largest, and nothing above 2^-21 of it is lost. m is the row's reference: its maximum
 // when it was last set, plus three; it is set again, for every row that has risen, when a weight would pass
 // 2^8.75, and the sums in tensor memory are then rescaled (2,200 to 3,000 cycles, waiting for the products that
 // make them: with a reference just above the maximum, or moved for one row alone, most of a unit's first
