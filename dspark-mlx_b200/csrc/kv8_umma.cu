@@ -74,7 +74,7 @@ struct Cfg {
 struct UmmaPlan {
   KvSplit sp;
   int k_slots, v_slots;  // steps' keys and values in shared memory: keys are done with earlier
-  bool vec_q, vec_blk;
+  bool vec_q, vec_blk;   // q's rows / both the block's keys and values can be read 4 values at a time
 };
 
 struct UmmaSmem {
@@ -975,7 +975,8 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   if (!split_fits(a, pl.sp)) return DSM_ERR_UNSUPPORTED;
   split_ws(pl.sp, ws, hd);
   pl.vec_q = vec_ok(a.q, a.q_batch, a.q_row, a.q_head, 8);
-  pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 8);
+  pl.vec_blk = a.blk_k && vec_ok(a.blk_k, a.bk_batch, a.bk_head, a.bk_row, 8) &&
+               vec_ok(a.blk_v, a.bv_batch, a.bv_head, a.bv_row, 8);
   switch (hd) {
     case 64: return launch_rows<64>(nr, a, pl, s);
     case 128: return launch_rows<128>(nr, a, pl, s);

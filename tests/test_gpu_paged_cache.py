@@ -847,3 +847,33 @@ def test_modules_refuse_caches_that_do_not_fit():
                 lambda: cache.extend(i32([1, 1]), -1), lambda: cache.trim(i32([1, 1])[::2])):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------------------------------- alignment
+def _placed(t, kind):
+    """``t`` in memory that starts one element late, or whose rows are of odd length, or as it is."""
+    if kind == "aligned":
+        return t.contiguous()
+    if kind == "late":
+        return torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 1, dtype=t.dtype, device=t.device)
+    return wide[..., :-1].copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("q,bk,bv", [
+    ("aligned", "aligned", "late"), ("aligned", "aligned", "odd"), ("aligned", "late", "aligned"),
+    ("aligned", "odd", "aligned"), ("late", "aligned", "aligned"), ("odd", "aligned", "aligned"), ("odd", "late", "odd"),
+])
+def test_attention_inputs_aligned_apart(dtype, q, bk, bv):
+    """q, the block's keys and its values each have an alignment of their own: whichever is off, the
+    result is that of contiguous rows, bit for bit."""
+    c = _attn_case(21, [300, 64, 0], 5, 2, 4, 128, 64, dtype)
+    want = _check_attn(c)
+    at = [_placed(t.to(DEV), kind) for t, kind in ((c["q"], q), (c["blk"][0], bk), (c["blk"][1], bv))]
+    assert torch.equal(pc.gqa_attention_kv8(at[0], c["layer"], c["tg"], i32(c["lengths"]), at[1], at[2]), want)
+    one = [t[:1].expand_as(t) for t in at]  # strides of zero: the same rows for every sequence
+    want = pc.gqa_attention_kv8(*(one[0].contiguous(), c["layer"], c["tg"], i32(c["lengths"])),
+                                *(t.contiguous() for t in one[1:]))
+    assert torch.equal(pc.gqa_attention_kv8(one[0], c["layer"], c["tg"], i32(c["lengths"]), *one[1:]), want)
+    assert _lib.device_error() == 0
