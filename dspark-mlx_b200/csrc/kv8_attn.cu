@@ -1011,6 +1011,9 @@ extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const
               "dsm_gqa_attn_kv8: NULL pointer");
   DSM_REQUIRE(kv8_aligned16(d->k_codes) && kv8_aligned16(d->v_codes), "dsm_gqa_attn_kv8: codes must be 16-byte aligned");
   DSM_REQUIRE(kv8_aligned16(ws), "dsm_gqa_attn_kv8: workspace must be 16-byte aligned");
+  // fp32 results are stored two at a time
+  DSM_REQUIRE(d->dtype != DSM_DT_F32 || reinterpret_cast<uintptr_t>(out) % 8 == 0,
+              "dsm_gqa_attn_kv8: an fp32 out must be 8-byte aligned");
   if (ws_bytes < dsm_gqa_attn_kv8_workspace_bytes(d->batch, d->block, d->n_heads, d->n_kv, d->head_dim))
     return fail(DSM_ERR_WORKSPACE, "dsm_gqa_attn_kv8: workspace too small");
   const AttnArgs a = {q,

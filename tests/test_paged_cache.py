@@ -150,3 +150,11 @@ def test_python_functions_refuse_cpu_tensors_and_bad_settings():
         args.update(kw)
         with pytest.raises(ValueError):
             pc.PagedKVCache(**args)
+
+
+def test_attention_refuses_an_fp32_result_off_eight_bytes():
+    L = _lib.lib()
+    f = dict(q_row_stride=128, q_head_stride=128, table_stride=8, k_codes=16, v_codes=16, dtype=_lib.DT_F32, batch=2,
+             block=3, n_heads=8, n_kv=2, head_dim=128, page_size=64, n_pages=4, max_pages=8, k_scale=4, v_scale=4)
+    assert L.dsm_gqa_attn_kv8(ctypes.byref(_lib.KV8AttnDesc(**f)), 4, 4, 4, None, None, 4, 16, 1 << 30, None) != 0
+    assert "out must be 8-byte aligned" in L.dsm_last_error_message().decode()
