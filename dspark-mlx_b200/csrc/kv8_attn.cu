@@ -6,8 +6,8 @@
 //   kv8_attn_mma_kernel   fp32 rows: f16 products in two terms each, split over the keys
 //   kv8_attn_combine_kernel  joins what either has cut
 //   kv8_attn_core_kernel  fp32 products on the CUDA cores: what the others do not take (a longer block, a
-//                         batch whose prefix does not fit shared memory), and dsm_set_attn_kernel's other
-//                         choice (per host thread)
+//                         batch whose prefix does not fit shared memory, a sequence's result past 2^31
+//                         values), and dsm_set_attn_kernel's other choice (per host thread)
 #include <algorithm>
 
 #include "kv8_attn.cuh"
@@ -983,7 +983,7 @@ using namespace dsm;
 
 extern "C" size_t dsm_gqa_attn_kv8_workspace_bytes(int batch, int block, int n_heads, int n_kv, int head_dim) {
   if (batch <= 0 || batch > kKv8MaxBatch || block <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0 ||
-      !kv8_head_dim_ok(head_dim))
+      int64_t(block) * n_heads > 0x7fffffff || !kv8_head_dim_ok(head_dim))
     return 0;
   const int rows = n_heads / n_kv * block;
   return std::max(mma_ws_bytes(mma_shape(rows, head_dim).cta_rows, head_dim), kv8_umma_ws_bytes(rows, head_dim));
@@ -996,6 +996,7 @@ extern "C" int dsm_gqa_attn_kv8(const dsm_kv8_attn_desc* d, const void* q, const
   DSM_REQUIRE(d->batch >= 0 && d->batch <= kKv8MaxBatch, "dsm_gqa_attn_kv8: batch must be 0..8192");
   DSM_REQUIRE(d->block > 0 && d->n_kv > 0 && d->n_heads > 0 && d->n_heads % d->n_kv == 0,
               "dsm_gqa_attn_kv8: bad shape (n_heads must be a multiple of n_kv)");
+  DSM_REQUIRE(int64_t(d->block) * d->n_heads <= 0x7fffffff, "dsm_gqa_attn_kv8: too many rows");
   DSM_REQUIRE(kv8_head_dim_ok(d->head_dim), "dsm_gqa_attn_kv8: head_dim must be 64, 128 or 256");
   DSM_REQUIRE(kv8_page_ok(d->page_size), "dsm_gqa_attn_kv8: page_size must be a multiple of 64, at most 1024");
   DSM_REQUIRE(d->n_pages > 0 && d->max_pages > 0 && d->max_pages <= kKv8MaxPages && d->table_stride >= d->max_pages,

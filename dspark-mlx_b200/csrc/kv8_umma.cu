@@ -963,6 +963,8 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   const int64_t groups = int64_t(a.n_pages) * a.n_kv * (a.page / kTile);
   const int64_t most = int64_t(a.batch) * a.max_pages * (a.page / kTile) * a.n_kv * pl.sp.row_blocks;
   if (groups * std::max(hd, kTile) > 0x7fffffff) return DSM_ERR_UNSUPPORTED;  // rows of the TMA maps
+  // a row's place in its sequence's result is kept in 32 bits
+  if (int64_t(a.block) * a.n_heads * hd > 0x7fffffff) return DSM_ERR_UNSUPPORTED;
   const int most_ctas = ctas_per_sm(nr, hd) * num_sms();
   pl.sp.ctas = int(std::min<int64_t>(most_ctas, most));
   // A unit's staging, first step and result take as long as ten tiles (cost 6: 61 ragged sequences 107 us

@@ -877,3 +877,21 @@ def test_attention_inputs_aligned_apart(dtype, q, bk, bv):
                                 *(t.contiguous() for t in one[1:]))
     assert torch.equal(pc.gqa_attention_kv8(one[0], c["layer"], c["tg"], i32(c["lengths"]), *one[1:]), want)
     assert _lib.device_error() == 0
+
+
+def test_attention_results_past_32_bits():
+    """A sequence's result of more than 2^31 values: one query row, read for every head and block row."""
+    block, nh, hd = 64, 262150, 128
+    k, ks, v, vs, layer = _pool(6, 2, 1, 64, hd, -9, -4)
+    row = torch.randn(1, 1, 1, hd, generator=torch.Generator().manual_seed(6)).bfloat16().to(DEV)
+    table, n = i32([[1, 0]]), i32([100])
+    try:
+        out = pc.gqa_attention_kv8(row.expand(1, block, nh, hd), layer, table, n)
+    except torch.OutOfMemoryError:
+        pytest.skip("no room for the result")
+    c = dict(q=row.cpu(), layer=layer, table=[[1, 0]], tg=table, lengths=[100], blk=[None, None],
+             k=k * ks[..., None, None], v=v * vs[..., None, None], hd=hd)
+    want = out[:, :1, :hd].clone()
+    _check_attn(c, out=want)
+    assert all(bool((part == want[0]).all()) for part in out.view(block, nh, hd))
+    assert _lib.device_error() == 0

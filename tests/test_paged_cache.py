@@ -158,3 +158,11 @@ def test_attention_refuses_an_fp32_result_off_eight_bytes():
              block=3, n_heads=8, n_kv=2, head_dim=128, page_size=64, n_pages=4, max_pages=8, k_scale=4, v_scale=4)
     assert L.dsm_gqa_attn_kv8(ctypes.byref(_lib.KV8AttnDesc(**f)), 4, 4, 4, None, None, 4, 16, 1 << 30, None) != 0
     assert "out must be 8-byte aligned" in L.dsm_last_error_message().decode()
+
+
+def test_attention_refuses_more_rows_than_32_bits_count():
+    L = _lib.lib()
+    assert L.dsm_gqa_attn_kv8_workspace_bytes(1, 1 << 16, 1 << 15, 1, 64) == 0
+    assert L.dsm_gqa_attn_kv8_workspace_bytes(1, 1 << 16, (1 << 15) - 1, 1, 64) > 0
+    assert _attn(L, block=1 << 16, n_heads=1 << 15, n_kv=1) != 0
+    assert "too many rows" in L.dsm_last_error_message().decode()
