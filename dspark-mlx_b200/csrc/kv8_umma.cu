@@ -706,7 +706,9 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           y[r + 3] = b.y;
           top = fmaxf(top, fmaxf(fmaxf(y[r], y[r + 1]), fmaxf(y[r + 2], y[r + 3])));
         }
-        if (any_of_group(grp, (live && top > kPMax) || i == 0 || want_rv != rv)) {
+        // no step with a key yet (rv is -200 till then): the references are still to be set, the sums are zero
+        const bool first = rv <= -200;
+        if (any_of_group(grp, (live && top > kPMax) || first || want_rv != rv)) {
           // new references: every row whose maximum has risen since its own was set (all of them at first)
 #pragma unroll
           for (int r = 0; r < RW; ++r) {
@@ -716,13 +718,13 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           group_sync(grp);
           if (gtid < RW) {
             const float x = fmaxf(fmaxf(red[gtid], red[16 + gtid]), fmaxf(red[32 + gtid], red[48 + gtid]));
-            const float up = x == kLowest ? 0.f : i == 0 || x > kPExp - kPHead ? x + (kPHead - kPExp) : 0.f;
+            const float up = x == kLowest ? 0.f : first || x > kPExp - kPHead ? x + (kPHead - kPExp) : 0.f;
             row_m[g0 + gtid] -= up;
             red[gtid] = up;
-            row_a[g0 + gtid] = ex2(-up);
+            row_a[g0 + gtid] = first ? 1.f : ex2(-up);  // a first one may lie far below zero: 0 * 2^200 is no 0
           }
           group_sync(grp);
-          const float fv = rv <= -200 ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
+          const float fv = first ? 1.f : kv8_exp2i(min(max(rv - want_rv, -126), 126));
           rv = want_rv;
           if (i > 0) {  // the sums so far, after the products that make them
             const int j = k - 1;

@@ -895,3 +895,32 @@ def test_attention_results_past_32_bits():
     _check_attn(c, out=want)
     assert all(bool((part == want[0]).all()) for part in out.view(block, nh, hd))
     assert _lib.device_error() == 0
+
+
+# ------------------------------------------------------------------------------- references and weights
+def _all_negative(c):
+    """Every score negative: q below zero, the keys above."""
+    c["q"], c["k"] = -c["q"].abs(), c["k"].abs()
+    c["layer"].k_codes.bitwise_and_(0x7F)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths,page,absent,scale", [
+    ([640, 300], 64, (0, 1), 0.18), ([640, 300], 64, (0, 1, 2, 3), 1.8), ([640, 130], 128, (0,), 0.18),
+    ([5000], 64, tuple(range(3, 70)), 0.18), ([5000, 900], 256, (0, 1, 2), 1.8),
+])
+def test_attention_where_the_first_pages_are_absent(dtype, lengths, page, absent, scale):
+    """A unit, or a CTA's part of one, whose first keys lie on pages that are none: the rows' references
+    come from the first keys that there are. Scores lie some 30 or 300 octaves below zero, so that
+    weights relative to zero are nothing at all. Norm: bf16's rounding is at most 2^-8 and 2^-8.8 on the
+    average, twice the scores' error at 300 octaves less than as much again (fp32: 2 * 2^-17 * 330)."""
+    c = _attn_case(len(absent), lengths, 5, 2, 4, 128, page, dtype, with_block=False, e_lo=-6, e_hi=-5)
+    _all_negative(c)
+    for row in c["table"]:
+        for j in absent:
+            if j < len(row):
+                row[j] = -1 if j % 2 else 10 ** 6
+    c["tg"] = i32(c["table"])
+    _check_attn(c, scale=scale, norm=2.0 ** -8)
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
