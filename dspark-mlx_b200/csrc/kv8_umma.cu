@@ -7,18 +7,24 @@
 // kind::f8f6f4 multiplies the e4m3 codes themselves. q, scaled per row by a power of two to at most
 // 448, is the sum of two e4m3 terms (hi = e4m3(x), lo = e4m3(x - hi): exact for bf16's 8 bits wherever
 // the residual reaches e4m3's normals, 2^-10 of a unit off elsewhere, of a row maximum of 224 to 448).
-// The weights are p = 2^(s - m + 8), an e4m3 term and an e5m2 residual: 2^-7 of a weight off at most where it
-// is above 2^-14 of the largest, and nothing above 2^-21 of it is lost. m is the row's reference: its maximum
-// when it was last set, plus three; it is set again, for every row that has risen, when a weight would pass
-// 2^8.75, and the sums in tensor memory are then rescaled (2,200 to 3,000 cycles, waiting for the products that
-// make them: with a reference just above the maximum, or moved for one row alone, most of a unit's first
-// steps paid that). The page's value exponent is folded into the weights relative to a reference rv that moves
-// when an exponent leaves [rv - 10, rv]; the scores' page factor is one per thread. Scores, sums and weights'
+// The weights are p = 2^(s - m + 15), rounded to f16 (2^-11 of a weight) and held by three e5m2 terms down to half of
+// e5m2's smallest step, 2^-17. m is the row's reference: its maximum when it was last set, plus three, so that the
+// largest weight is 2^12 or more, and 2^-29 of it is the most that is lost of any beside its 2^-11. (An e4m3 and
+// an e5m2 term, relative to 2^8, left 2^-7 of a weight down to 2^-12 of the largest, an eighth at 2^-16 and nothing
+// below 2^-22: a tail behind a heavy key that gives nothing was off by 2 to 10 percent.) m is set again, for every
+// row that has risen, when a weight would pass 2^15.75, and the sums in tensor memory are then rescaled (2,200 to
+// 3,000 cycles, waiting for the products that make them: with a reference just above the maximum, or moved for
+// one row alone, most of a unit's first steps paid that). The page's value exponent is folded into the weights
+// relative to a reference rv that moves when an exponent leaves [rv - 10, rv]: the 2^-29 are of the largest weight
+// times the largest value that 2^rv stands for, and a page whose values are 2^29 times smaller than its
+// neighbour's gives nothing. The scores' page factor is one per thread. Scores, sums and weights'
 // sums are fp32. The block's own rows are a unit's first step, in two e4m3 terms per row like q.
 //
 // What bounds it: reading 2 * head_dim bytes per key and KV head. At the copy peak an SM gets 128 keys of
-// head_dim 128 per ~1400 cycles; their products take ~300 cycles of the tensor cores for 32 rows, the
-// shared-memory traffic ~1000, the softmax ~420 instructions of each of four warps. mma.sync runs e4m3
+// head_dim 128 per ~1400 cycles. Of shared memory that takes 256 cycles for the copies and 32 for each product's
+// 4 KB of codes, so a weight's terms are columns of one product (N = 3 x rows, a sum each, added at the end): as
+// products of their own, 20 a step instead of 12, they cost 210 us instead of 176 for 128 sequences of 4096 keys.
+// The softmax is ~420 instructions of each of four warps. mma.sync runs e4m3
 // operands as f16 products with the conversions around every one, and f16 fragments converted once per warp
 // need 1,700 unrolled instructions per 64 keys and 32 rows, which the instruction cache does not hold
 // (measured: 116 us for 131,071 keys x 8 heads x 20 rows, against 41 us for the bytes).
@@ -33,10 +39,10 @@
 //   product warp    one thread issues the products: scores of step i + 1 before the sums of step i
 // Code that runs once per unit is kept short: a CTA meets it with a cold instruction cache.
 //
-// Measured (32 query heads on 8 KV heads of 128): 128 sequences of 4096 keys, one row each, 192 us (5.6 TB/s);
-// one of 131,071 keys, 5 rows, 75 us (3.6 TB/s); 16 of 2048 keys, 7 rows, 39 us. Where rows are few the copies
-// bound it. At 20 to 32 rows a step takes 3,100 cycles of a CTA, two at a time: 1,400 of instructions, the
-// rest waits for scores and slots; a unit costs 12,000 (a CTA's first) to 8,000 cycles beside its steps.
+// Measured (32 query heads on 8 KV heads of 128): 128 sequences of 4096 keys, one row each, 177 us (6.1 TB/s);
+// one of 131,071 keys, 5 rows, 70 us (3.8 TB/s); 16 of 2048 keys, 7 rows, 38 us. Where rows are few the copies
+// bound it. At 20 to 32 rows a step's instructions and its waits for scores and slots do, and what a unit costs
+// beside its steps (ten tiles' time, kv8_umma below).
 #include <algorithm>
 #include <mutex>
 
@@ -50,9 +56,13 @@ using B16 = __nv_bfloat16;
 
 constexpr int kStepKeys = 128;
 constexpr int kGroupRows = 16;  // query rows of a softmax group
-constexpr float kPExp = 8.f;    // weights at the reference: 2^8
-constexpr float kPMax = 8.75f;  // 2^8.75 = 431 still fits e4m3
-constexpr float kPHead = 3.f;   // a new reference lies this much above the maximum: the maximum's own weight is 2^5
+constexpr float kPExp = 15.f;    // weights at the reference: 2^15
+constexpr float kPMax = 15.75f;  // 2^15.75 = 55,109 still fits e5m2 and f16
+constexpr float kPHead = 3.f;    // a new reference lies this much above the maximum: the maximum's own weight is 2^12
+constexpr int kPTerms = 3;       // e5m2 terms of a weight
+
+// steps whose weights are held: one where a second would cost a copy's slot (attn_long 74.7 us with one, 76 with two)
+__host__ __device__ constexpr int p_buffers(int hd, int nm) { return hd == 128 && nm <= 32 ? 1 : 2; }
 
 template <int HD, int NR>  // NR query rows per CTA: 4, 8, 16, 32 or 64
 struct Cfg {
@@ -66,9 +76,12 @@ struct Cfg {
   static constexpr int kHalf = kTile * HD;       // bytes of 64 keys, or of their values
   static constexpr int kSlot = 2 * kHalf;        // a step's keys, or its values
   static constexpr int kQTerm = NM * HD;         // bytes of one term of q
-  static constexpr int kPTerm = NM * kStepKeys;  // bytes of one term of the weights; two buffers of two
-  static constexpr int kCols = 2 * NM + NH * NM; // tensor memory: two score buffers, the sums
-  static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
+  static constexpr int kPTerm = NM * kStepKeys;  // bytes of one term of the weights
+  static constexpr int PB = p_buffers(HD, NM);   // steps' weights in shared memory
+  static constexpr int ON = kPTerms * NM;        // columns of the sums: each term of the weights has its own
+  static constexpr int kCols = 2 * NM + NH * ON; // tensor memory: two score buffers, the sums
+  static constexpr int kAlloc = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kCols <= 512 && CTAS * kAlloc <= 512);
 };
 
 struct UmmaPlan {
@@ -89,7 +102,7 @@ __host__ __device__ inline UmmaSmem umma_smem(int hd, int nm, int slots, int bat
   UmmaSmem s;
   s.q = slots * 2 * kTile * hd;
   s.p = s.q + 2 * nm * hd;
-  s.rows = s.p + 4 * nm * kStepKeys;
+  s.rows = s.p + p_buffers(hd, nm) * kPTerms * nm * kStepKeys;
   s.keys = s.rows + kRowFloats * nm * 4;  // the block's rows: key scale and value exponent
   s.info = s.keys + kUmmaMaxBlock * 8;
   s.bars = s.info + kInfos * 16;
@@ -111,19 +124,20 @@ __device__ __forceinline__ uint64_t desc_sw64(uint32_t saddr) {
   return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(512 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(4) << 61);
 }
-// the weights, rows of 16, 32 or 64 bytes per key (the operand's N dimension contiguous): 16-byte rows
-// unswizzled with groups of 8 keys at 128 B (the leading offset), 32- and 64-byte rows in the swizzle of their
-// width with groups of 8 keys at 256 and 512 B (the stride)
+// the weights, rows of 16, 32 or 64 bytes per key and term (the operand's N dimension contiguous), the terms one
+// after another: 16-byte rows unswizzled with groups of 8 keys at 128 B (the leading offset) and terms at the
+// stride, 32- and 64-byte rows in the swizzle of their width with groups of 8 keys at 256 and 512 B (the
+// stride) and terms at the leading offset
 template <int NM>
 __device__ __forceinline__ uint64_t desc_weights(uint32_t saddr) {
-  constexpr uint64_t lead = NM == 16 ? 128 >> 4 : 1, stride = NM == 16 ? 128 >> 4 : 8 * NM >> 4;
+  constexpr uint64_t keys8 = 8 * NM >> 4, term = NM * kStepKeys >> 4;
+  constexpr uint64_t lead = NM == 16 ? keys8 : term, stride = NM == 16 ? term : keys8;
   constexpr uint64_t swizzle = NM == 16 ? 0 : NM == 32 ? 6 : 4;
   return uint64_t((saddr >> 4) & 0x3FFFu) | (lead << 16) | (stride << 32) | (uint64_t(1) << 46) | (swizzle << 61);
 }
-// kind::f8f6f4: D f32, A e4m3 K-major, B e4m3 or e5m2, K-major or (b_rows) N-major
-__device__ __forceinline__ uint32_t idesc_f8(int n, bool b_e5m2, bool b_rows) {
-  return (1u << 4) | (b_e5m2 ? 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) |
-         (uint32_t(128 >> 4) << 24);
+// kind::f8f6f4: D f32, A e4m3 K-major, B e4m3 K-major (q), or e5m2 N-major (the weights)
+__device__ __forceinline__ uint32_t idesc_f8(int n, bool weights) {
+  return (1u << 4) | (weights ? 1u << 10 | 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   const uint32_t no_mask = 0u, acc = accumulate ? 1u : 0u;
@@ -212,24 +226,26 @@ __device__ __forceinline__ float redux_max(float x) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
 }
-// four weights -> an e4m3 term and an e5m2 residual, four bytes each, x0 lowest. They pass through f16,
-// whose 11 bits are more than the two terms keep.
-__device__ __forceinline__ void weight_terms(float x0, float x1, float x2, float x3, uint32_t& hi, uint32_t& lo) {
-  asm("{\n .reg .b32 x, y, g, h;\n .reg .b16 a, b, c, d;\n"
-      " cvt.rn.f16x2.f32 x, %3, %2;\n"
-      " cvt.rn.f16x2.f32 y, %5, %4;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 a, x;\n"
-      " cvt.rn.satfinite.e4m3x2.f16x2 b, y;\n"
+// Weights of up to 2^15.75 enter in three e5m2 terms. They pass through f16, whose 11 bits the terms hold: a residual
+// of 8 bits after the first (3 bits) is at most 8 units after the second, and fits the third.
+__device__ __forceinline__ uint32_t to_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// the next term of four weights, a byte each, taken off them. An e5m2 value is the upper byte of its f16.
+__device__ __forceinline__ uint32_t weight_term(uint32_t& x, uint32_t& y) {
+  uint32_t t;
+  asm("{\n .reg .b32 g, h;\n .reg .b16 a, b;\n"
+      " cvt.rn.satfinite.e5m2x2.f16x2 a, %1;\n"
+      " cvt.rn.satfinite.e5m2x2.f16x2 b, %2;\n"
       " mov.b32 %0, {a, b};\n"
-      " cvt.rn.f16x2.e4m3x2 g, a;\n"
-      " cvt.rn.f16x2.e4m3x2 h, b;\n"
-      " sub.rn.f16x2 x, x, g;\n"
-      " sub.rn.f16x2 y, y, h;\n"
-      " cvt.rn.satfinite.e5m2x2.f16x2 c, x;\n"
-      " cvt.rn.satfinite.e5m2x2.f16x2 d, y;\n"
-      " mov.b32 %1, {c, d};\n}"
-      : "=&r"(hi), "=&r"(lo)
-      : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+      " prmt.b32 g, %0, 0, 0x1404;\n"
+      " prmt.b32 h, %0, 0, 0x3424;\n"
+      " sub.rn.f16x2 %1, %1, g;\n"
+      " sub.rn.f16x2 %2, %2, h;\n}"
+      : "=&r"(t), "+r"(x), "+r"(y));
+  return t;
 }
 __device__ __forceinline__ void store_words(uint32_t at, const uint32_t (&w)[4], int n) {  // n is a constant
   if (n == 4)
@@ -444,7 +460,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
   } else if (warp == kProduct) {
     // ---------------------------------------------------------------- products
     if (lane == 0) {
-      const uint32_t id_s = idesc_f8(NM, false, false), id_hi = idesc_f8(NM, false, true), id_lo = idesc_f8(NM, true, true);
+      const uint32_t id_s = idesc_f8(NM, false), id_o = idesc_f8(C::ON, true);
       const uint32_t base = smem_u32(smem), qa = base + L.q, pa = base + L.p;
       int k = 0, seg = 0;  // steps, and units with steps, so far
       for (int a0 = 0; a0 < n_tiles;) {
@@ -454,29 +470,27 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         if (ok) ok = wait(q_full, seg++ & 1);
         tc::tc_fence_after();
         auto sums = [&](int j, bool first, bool blk) {  // step j's
-          const int pb = j & 1;
+          const int pb = j % C::PB;
           if (ok) ok = wait(v_full + j % VN, (j / VN) & 1);
           tc::tc_fence_after();
           if (!ok) return;
-          const uint32_t v = base + KN * C::kSlot + (j % VN) * C::kSlot, w = pa + pb * 2 * C::kPTerm;
+          const uint32_t v = base + KN * C::kSlot + (j % VN) * C::kSlot, w = pa + pb * kPTerms * C::kPTerm;
           // 32 keys a product
           const uint64_t av = desc_sw64(v), bw = desc_weights<NM>(w);
           if (!blk) {
 #pragma unroll
             for (int nh = 0; nh < C::NH; ++nh)
 #pragma unroll
-              for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                  umma_f8(t_o + nh * NM, av + (((ks >> 1) * C::kHalf + nh * 128 * 64 + (ks & 1) * 32) >> 4),
-                          bw + ((x * C::kPTerm + ks * 32 * NM) >> 4), x ? id_lo : id_hi, !first || x > 0 || ks > 0);
+              for (int ks = 0; ks < 4; ++ks)
+                umma_f8(t_o + nh * C::ON, av + (((ks >> 1) * C::kHalf + nh * 128 * 64 + (ks & 1) * 32) >> 4),
+                        bw + (ks * 32 * NM >> 4), id_o, !first || ks > 0);
           } else {  // its values' two terms lie where others have keys 0-63 and 64-127
             const int n = (p.block + 31) / 32;
 #pragma unroll 1
-            for (int i = 0; i < 4 * C::NH * n; ++i) {
-              const int ks = i % n, term = i / n & 1, x = i / n >> 1 & 1, nh = i / n >> 2;
-              umma_f8(t_o + nh * NM, av + ((term * C::kHalf + nh * 128 * 64 + ks * 32) >> 4),
-                      bw + ((x * C::kPTerm + ks * 32 * NM) >> 4), x ? id_lo : id_hi, !first || i % (4 * n) > 0);
+            for (int i = 0; i < 2 * C::NH * n; ++i) {
+              const int ks = i % n, term = i / n & 1, nh = i / n >> 1;
+              umma_f8(t_o + nh * C::ON, av + ((term * C::kHalf + nh * 128 * 64 + ks * 32) >> 4),
+                      bw + (ks * 32 * NM >> 4), id_o, !first || i % (2 * n) > 0);
             }
           }
           tc::umma_commit(v_empty + j % VN);
@@ -508,7 +522,7 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
             tc::umma_commit(k_empty + kk % KN);
             ++i;
             idle = 0;
-          } else if (j < i && done(p_full + (jj & 1), (jj >> 1) & 1)) {
+          } else if (j < i && done(p_full + jj % C::PB, (jj / C::PB) & 1)) {
             sums(jj, j == 0, sg.blk && j == 0);
             ++j;
             idle = 0;
@@ -531,6 +545,9 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
     const int row_r = tid / TPR, row_d = tid % TPR * VB;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const int group = p.n_heads / p.n_kv;
+    // rows of the sums at a time: 8 keep the 96 registers of two CTAs per SM from spilling (attn_long 74.7 -> 70.0 us),
+    // at head_dim 64 their second round costs more (attn_narrow_heads 27.4 us, with 8 rows 29.3)
+    constexpr int RP = HD == 64 || RW < 8 ? RW : 8;
     float* const red = reds + grp * 4 * kGroupRows;
     const float* const my_c = row_c + g0;
     const float* const my_m = row_m + g0;
@@ -728,19 +745,20 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
           rv = want_rv;
           if (i > 0) {  // the sums so far, after the products that make them
             const int j = k - 1;
-            if (ok) ok = wait(p_empty + (j & 1), (j >> 1) & 1);
+            if (ok) ok = wait(p_empty + j % C::PB, (j / C::PB) & 1);
             tc::tc_fence_after();
 #pragma unroll
             for (int r = 0; r < RW; ++r) l[r] *= my_a[r];
 #pragma unroll 1
-            for (int nh = 0; nh < C::NH; ++nh) {
-              float o[RW];
-              uint32_t u[RW];
-              const uint32_t at = t_o + t_lane + nh * NM + g0;
-              tmem_ld<RW>(at, o);
+            for (int x = 0; x < C::NH * kPTerms * (RW / RP); ++x) {
+              float o[RP];
+              uint32_t u[RP];
+              const int r0 = x % (RW / RP) * RP;
+              const uint32_t at = t_o + t_lane + x / (RW / RP) * NM + g0 + r0;
+              tmem_ld<RP>(at, o);
               tc::tmem_ld_wait();
 #pragma unroll
-              for (int r = 0; r < RW; ++r) u[r] = __float_as_uint(o[r] * (my_a[r] * fv));
+              for (int r = 0; r < RP; ++r) u[r] = __float_as_uint(o[r] * (my_a[r0 + r] * fv));
               tmem_st(at, u);
             }
             tc::tmem_st_wait();
@@ -766,15 +784,17 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
 #pragma unroll
           for (int r = 0; r < RW; ++r) y[r] *= fv;
         }
-        const int pb = k & 1;
-        if (ok && k >= 2) ok = wait(p_empty + pb, ((k >> 1) - 1) & 1);
-        {
-          uint32_t hi[4], lo[4];
+        uint32_t w[RW / 2];
 #pragma unroll
-          for (int w = 0; w < RW / 4; ++w) weight_terms(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3], hi[w], lo[w]);
-          const uint32_t at = p_at + pb * 2 * C::kPTerm;
-          store_words(at, hi, RW / 4);
-          store_words(at + C::kPTerm, lo, RW / 4);
+        for (int r = 0; r < RW; r += 2) w[r / 2] = to_f16x2(y[r], y[r + 1]);
+        const int pb = k % C::PB;
+        if (ok && k >= C::PB) ok = wait(p_empty + pb, (k / C::PB - 1) & 1);
+#pragma unroll
+        for (int x = 0; x < kPTerms; ++x) {
+          uint32_t t[4];
+#pragma unroll
+          for (int i = 0; i < RW / 4; ++i) t[i] = weight_term(w[2 * i], w[2 * i + 1]);
+          store_words(p_at + (pb * kPTerms + x) * C::kPTerm, t, RW / 4);
         }
         // value codes without a key (behind the length, or of a page that is none) are cleared: a weight of
         // zero would not take a NaN there out
@@ -833,10 +853,10 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
       group_sync(grp);
       const int part = 2 * blockIdx.x + (a0 == 0 && sg.t0 > 0 ? 0 : 1);
       if (gtid < RW) {
-        // o and l are relative to row_m, o in units of 2^rv
+        // o and l are relative to row_m, o in units of 2^rv (not in row_a: 2^rv / l may fall below fp32's normals)
         const int r = g0 + gtid;
         const float den = red[gtid] + red[16 + gtid] + red[32 + gtid] + red[48 + gtid];
-        row_a[r] = den == 0.f ? 0.f : kv8_exp2i(min(max(rv, -126), 126)) / den;
+        row_a[r] = den == 0.f ? 0.f : 1.f / den;
         if (!sg.whole && r < sg.n_rows)
           pl.sp.ml[int64_t(part) * NR + r] = make_float4(den == 0.f ? -INFINITY : -row_m[r], den, float(rv), 0.f);
       }
@@ -847,28 +867,42 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
         tc::tc_fence_after();
       }
 #pragma unroll 1
-      for (int nh = 0; nh < C::NH; ++nh) {
+      for (int i = 0; i < C::NH * (RW / RP); ++i) {
+        const int nh = i / (RW / RP), r0 = g0 + i % (RW / RP) * RP;
         const int d = nh * 128 + gtid;
-        float o[RW];
-        if (sg.steps > 0) {
-          tmem_ld<RW>(t_o + t_lane + nh * NM + g0, o);
-          tc::tmem_ld_wait();
-        } else {
+        float o[RP];
 #pragma unroll
-          for (int r = 0; r < RW; ++r) o[r] = 0.f;
+        for (int r = 0; r < RP; ++r) o[r] = 0.f;
+        if (sg.steps > 0) {
+          const uint32_t at = t_o + t_lane + nh * C::ON + r0;  // the terms' sums, small ones first
+          constexpr int kAtOnce = RP <= 8 ? kPTerms : 1;
+#pragma unroll 1
+          for (int x = kPTerms; x > 0; x -= kAtOnce) {
+            float t[kAtOnce][RP];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) tmem_ld<RP>(at + (x - 1 - j) * NM, t[j]);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+              for (int r = 0; r < RP; ++r) o[r] += t[j][r];
+          }
         }
         if (d >= HD) continue;  // head_dim 64: the other lanes multiplied whatever followed
         if (sg.whole) {
           B16* out = static_cast<B16*>(p.out) + int64_t(sg.b) * p.block * p.n_heads * HD + d;
+          const float unit = kv8_exp2i(min(max(rv, -126), 126));
 #pragma unroll
-          for (int r = 0; r < RW; ++r)
-            if (g0 + r < sg.n_rows)
-              out[row_out[g0 + r]] = __float2bfloat16_rn(my_a[r] == 0.f ? 0.f : o[r] * my_a[r]);
+          for (int r = 0; r < RP; ++r)
+            if (r0 + r < sg.n_rows) {
+              const float inv = row_a[r0 + r];
+              out[row_out[r0 + r]] = __float2bfloat16_rn(inv == 0.f ? 0.f : o[r] * inv * unit);
+            }
         } else {
-          float* out = pl.sp.part + (int64_t(part) * NR + g0) * HD + d;
+          float* out = pl.sp.part + (int64_t(part) * NR + r0) * HD + d;
 #pragma unroll
-          for (int r = 0; r < RW; ++r)
-            if (g0 + r < sg.n_rows) out[r * HD] = o[r];
+          for (int r = 0; r < RP; ++r)
+            if (r0 + r < sg.n_rows) out[r * HD] = o[r];
         }
       }
       tc::tc_fence_before();

@@ -924,3 +924,113 @@ def test_attention_where_the_first_pages_are_absent(dtype, lengths, page, absent
     _check_attn(c, scale=scale, norm=2.0 ** -8)
     with pytest.raises(_lib.DsmError, match="outside the pool"):
         _lib.raise_device_error()
+
+
+def _close(c, out, scale):
+    """Every value within the sum of its roundings, per query row, in the order of its own weights. With A the
+    mean of |v| under a row's weights, W the largest of these, n the keys, and Vs no less than 448 times any value
+    scale that the row's unit meets (its own rows: 4 max |v|):
+
+    * 2^-8 of the result, rounded once;
+    * own keys and values as two e4m3 terms like q, exact but for 2^-10, half of e4m3's smallest step, of a row scaled
+      to 224 or more: 2^-17 of the row's largest;
+    * scores off by ds move the weights by 2 ds, hence 2 ds A. ds is q's second term below e4m3's normals,
+      2^-17 max |q| sum |k| scale, and 2^-18 of S = sum |q k| scale for fp32 sums and the exponential's argument;
+    * a weight is rounded to f16, 2^-11 of it, whose 11 bits three e5m2 terms hold, down to half of e5m2's
+      smallest step, 2^-17 where the largest weight is 2^12 or more: 2^-11 A + n 2^-29 W Vs."""
+    hd = c["hd"]
+    b, s, nh, _ = c["q"].shape
+    n_pages, n_kv, page, _ = c["k"].shape
+    group = nh // n_kv
+    got = out.double().cpu().view(b, s, nh, hd)
+    assert torch.isfinite(got).all()
+    sq, sr = 0.0, 0.0
+    for i, n in enumerate(c["lengths"]):
+        ids = c["table"][i][:-(-n // page)]
+        for h in range(n_kv):
+            k = torch.cat([c["k"][p, h] for p in ids])[:n]
+            v = torch.cat([c["v"][p, h] for p in ids])[:n]
+            vs = 448 * float(c["layer"].v_scale[ids, h].max())
+            if c["blk"][0] is not None:
+                k, v = (torch.cat([t, u[i, h].double()]) for t, u in ((k, c["blk"][0]), (v, c["blk"][1])))
+                vs = max(vs, 4 * float(c["blk"][1][i, h].abs().max()))
+            q = c["q"][i, :, h * group:(h + 1) * group].double()  # [s, group, hd]
+            w = torch.softmax(q @ k.T * scale, -1)
+            ref = w @ v
+            a, top, m = w @ v.abs(), w.amax(-1, keepdim=True), len(k)
+            big = (q.abs() @ k.abs().T).amax(-1, keepdim=True) * abs(scale)
+            ds = 2.0 ** -17 * q.abs().amax(-1, keepdim=True) * k.abs().sum(-1).max() * abs(scale) + 2.0 ** -18 * big
+            own = 0.0
+            if c["blk"][0] is not None:
+                ds += 2.0 ** -17 * float(c["blk"][0][i, h].abs().max()) * q.abs().sum(-1, keepdim=True) * abs(scale)
+                own = 2.0 ** -17 * float(c["blk"][1][i, h].abs().max())
+            tol = 2.0 ** -8 * ref.abs() + (2 * ds + 2.0 ** -11) * a + own + m * 2.0 ** -29 * top * vs
+            err = got[i, :, h * group:(h + 1) * group] - ref
+            assert bool((err.abs() <= tol).all()), float((err.abs() / tol).max())
+            sq, sr = sq + float(err.square().sum()), sr + float(ref.square().sum())
+    return (sq / sr) ** 0.5
+
+
+def _sinks(seed, dtype, n, s, n_kv, group, hd, page, q0, with_block=False):
+    """Every 64th key draws q0 * 7 nats more than the others, whose scores are normal, and has a value of zero."""
+    c = _attn_case(seed, [n], s, n_kv, group, hd, page, dtype, with_block=with_block, e_lo=-6, e_hi=-5,
+                   q_mag=hd ** -0.5 / 1.5)
+    k, v = c["k"] * 2.0 ** 6, c["v"] * 2.0 ** 6
+    k[..., 0] = 0
+    k[:, :, ::64], v[:, :, ::64] = 0, 0
+    k[:, :, ::64, 0] = 448
+    c["k"], c["v"] = torch.nan_to_num(k) * 2.0 ** -6, torch.nan_to_num(v) * 2.0 ** -6
+    c["layer"] = pc.KV8Layer(_codes(po.store_keys(k)), _codes(po.store_values(v)),
+                             torch.full_like(c["layer"].k_scale, 2.0 ** -6), torch.full_like(c["layer"].v_scale, 2.0 ** -6))
+    c["q"][..., 0] = q0
+    return c
+
+
+SINKS = [(1.5, 700, 1, 1, 1, 64, 64), (1.5, 2048, 5, 2, 4, 128, 64), (2.0, 2048, 1, 2, 4, 128, 128),
+         (2.0, 1500, 7, 1, 8, 64, 64), (2.0, 1000, 2, 1, 4, 256, 256)]
+
+
+@pytest.mark.parametrize("q0,n,s,n_kv,group,hd,page", SINKS)
+def test_attention_under_sinks(q0, n, s, n_kv, group, hd, page):
+    """Keys 2^15 or 2^20 times heavier than the others that give nothing: the result is the others' alone. Norm: as far
+    off as bf16's own rounding at most (2^-8; 2^-8.8 on the average), the weights' 2^-11 and 2^-29 of the
+    largest, 2^-9 of one that is 2^-20 of it, taking the rest."""
+    c = _sinks(4, BF, n, s, n_kv, group, hd, page, q0)
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), scale=1.0)
+    assert _close(c, out, 1.0) <= 2.0 ** -8
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("lower,s,hd", [(6, 1, 128), (12, 5, 128), (12, 2, 64), (14, 7, 256)])
+def test_attention_to_pages_of_a_small_scale(lower, s, hd):
+    """Every second page has values 2^lower times smaller, and all of the weight: 2^-40 is left for its neighbour. What
+    the result owes to the small page is as exact as its distance leaves it: 2^-29 of the largest weight, in
+    units of the large scale."""
+    c = _attn_case(lower, [1024], s, 2, 4, hd, 64, BF, with_block=False, e_lo=-6, e_hi=-5, q_mag=hd ** -0.5 / 1.5,
+                   poison=False)
+    k = c["k"] * 2.0 ** 6
+    for j, p in enumerate(c["table"][0][:16]):
+        k[p, :, :, 0] = 448 if j % 2 else -448
+        f = 2.0 ** -lower if j % 2 else 1.0
+        c["v"][p] *= f
+        c["layer"].v_scale[p] *= f
+    c["k"] = k * 2.0 ** -6
+    c["layer"].k_codes.copy_(_codes(po.store_keys(k)))
+    c["q"][..., 0] = 2.0
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), scale=1.0)
+    assert _close(c, out, 1.0) <= 2.0 ** -8
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,lengths,s,n_kv,group,hd,page", [
+    (BF, [150, 0, 1], 1, 8, 4, 128, 64), (BF, [700, 3, 1999], 7, 2, 4, 128, 64), (BF, [1000, 77], 7, 2, 8, 64, 64),
+    (BF, [513, 300], 5, 1, 3, 256, 128),
+])
+def test_attention_row_by_row(dtype, lengths, s, n_kv, group, hd, page):
+    """The bound of each row by its own weights, own rows included. Norm: bf16's rounding alone is 2^-8.8 on the average
+    (its half step's third root); 1.1 times it leaves half as much for all else."""
+    c = _attn_case(sum(lengths) + 1, [n or 1 for n in lengths], s, n_kv, group, hd, page, dtype)
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), *(t.to(DEV) for t in c["blk"]))
+    norm = _close(c, out, hd ** -0.5)
+    assert norm <= 1.1 * 2.0 ** -8 / 3 ** 0.5
+    assert _lib.device_error() == 0
