@@ -1034,3 +1034,62 @@ def test_attention_row_by_row(dtype, lengths, s, n_kv, group, hd, page):
     norm = _close(c, out, hd ** -0.5)
     assert norm <= 1.1 * 2.0 ** -8 / 3 ** 0.5
     assert _lib.device_error() == 0
+
+
+def _close_f32(c, out, scale):
+    """The same for fp32 calls, whose factors are two f16 terms each; returns the norm of the error over what it may be.
+    2^-24 of the result; scores off by ds <= (2^-21 + (hd + 8) 2^-24) S; a weight's second term is held times 2^11, so
+    that both leave 2^-22 of a weight and 2^-36 where the largest is 2^6 or more, own values 2^-22, sums of n keys
+    (n / 32 + 64) 2^-24: (2 ds + 2^-21 + (n / 32 + 64) 2^-24) A + n 2^-42 W Vs. Norm: 2^-20 for the terms, and
+    2^-23 S, for the tensor cores cut off 2^-23 of a sum at each of the four steps that are added in them, a
+    quarter of a row's products each, hence S 2^-23 for all of a row's at most."""
+    hd = c["hd"]
+    b, s, nh, _ = c["q"].shape
+    n_pages, n_kv, page, _ = c["k"].shape
+    group = nh // n_kv
+    got = out.double().cpu().view(b, s, nh, hd)
+    sq, sr, most = 0.0, 0.0, 0.0
+    for i, n in enumerate(c["lengths"]):
+        ids = c["table"][i][:-(-n // page)]
+        for h in range(n_kv):
+            k = torch.cat([c["k"][p, h] for p in ids])[:n]
+            v = torch.cat([c["v"][p, h] for p in ids])[:n]
+            vs = 448 * float(c["layer"].v_scale[ids, h].max())
+            if c["blk"][0] is not None:
+                k, v = (torch.cat([t, u[i, h].double()]) for t, u in ((k, c["blk"][0]), (v, c["blk"][1])))
+                vs = max(vs, 4 * float(c["blk"][1][i, h].abs().max()))
+            q = c["q"][i, :, h * group:(h + 1) * group].double()
+            w = torch.softmax(q @ k.T * scale, -1)
+            ref, a, top, m = w @ v, w @ v.abs(), w.amax(-1, keepdim=True), len(k)
+            big = (q.abs() @ k.abs().T).amax(-1, keepdim=True) * abs(scale)
+            ds = (2.0 ** -21 + (hd + 8) * 2.0 ** -24) * big
+            tol = 2.0 ** -24 * ref.abs() + (2 * ds + 2.0 ** -21 + (m / 32 + 64) * 2.0 ** -24) * a + m * 2.0 ** -42 * top * vs
+            err = got[i, :, h * group:(h + 1) * group] - ref
+            assert bool((err.abs() <= tol).all()), float((err.abs() / tol).max())
+            sq, sr, most = sq + float(err.square().sum()), sr + float(ref.square().sum()), max(most, float(big.max()))
+    return (sq / sr) ** 0.5 / (2.0 ** -20 + 2.0 ** -23 * most)
+
+
+@pytest.mark.parametrize("with_block", [False, True])
+@pytest.mark.parametrize("q0,n,s,n_kv,group,hd,page", SINKS)
+def test_fp32_attention_under_sinks(q0, n, s, n_kv, group, hd, page, with_block):
+    c = _sinks(4, F32, n, s, n_kv, group, hd, page, q0, with_block)
+    if with_block:  # own rows: the first draws as the sinks do and gives nothing
+        c["blk"][0][..., 0] = 0
+        c["blk"][0][:, :, 0] = 0
+        c["blk"][0][:, :, 0, 0] = 7
+        c["blk"][1][:, :, 0] = 0
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]),
+                               *(None if t is None else t.to(DEV) for t in c["blk"]), scale=1.0)
+    assert _close_f32(c, out, 1.0) <= 1
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("lengths,s,n_kv,group,hd,page", [
+    ([150, 700], 5, 2, 4, 128, 64), ([500, 40], 5, 1, 4, 256, 64), ([1, 333], 1, 2, 8, 64, 128),
+])
+def test_fp32_attention_row_by_row(lengths, s, n_kv, group, hd, page):
+    c = _attn_case(sum(lengths) + 1, lengths, s, n_kv, group, hd, page, F32)
+    out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), *(t.to(DEV) for t in c["blk"]))
+    assert _close_f32(c, out, hd ** -0.5) <= 1
+    assert _lib.device_error() == 0
