@@ -16,8 +16,8 @@ namespace dsm {
 namespace {
 
 // The CUDA-core kernel: one warp per query row, 32 keys at a time with an online softmax, all in
-// fp32. Lanes take a key each for the scores, then head_dim / 32 columns each for the sum. Runs
-// for every type; the time goes into the fp32 products (two per code and query row).
+// fp32. Lanes take a key each for the scores, then head_dim / 32 columns each for the sum. What is not
+// finite counts as NaN, as in the other kernels, whose scaled terms have no infinity. Runs for every type; the time goes into the fp32 products (two per code and query row).
 constexpr int kCoreWarps = 4;
 
 template <typename T, int HD>
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kCoreWarps * 32) kv8_attn_core_kernel(const At
   float* q = q_sm[warp];
   float* ps = p_sm[warp];
   const T* qg = static_cast<const T*>(p.q) + b * p.q_batch + s * p.q_row + h * p.q_head;
-  for (int d = lane; d < HD; d += 32) q[d] = ld_f(qg, d) * p.scale;
+  for (int d = lane; d < HD; d += 32) q[d] = scaled(ld_f(qg, d), p.scale);
   __syncwarp();
   const int64_t cap = int64_t(p.max_pages) * p.page;
   const int asked = p.lengths[b];
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kCoreWarps * 32) kv8_attn_core_kernel(const At
       float x = -INFINITY;
       if (lane < n) {
         x = 0.f;
-        for (int d = 0; d < HD; ++d) x = fmaf(q[d], ld_f(bk, (base + lane) * p.bk_row + d), x);
+        for (int d = 0; d < HD; ++d) x = fmaf(q[d], scaled(ld_f(bk, (base + lane) * p.bk_row + d), 1.f), x);
       }
       const float m_new = fmaxf(m, kv8_warp_max(x));
       const float ref = m_new == -INFINITY ? 0.f : m_new;
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kCoreWarps * 32) kv8_attn_core_kernel(const At
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
         float o = acc[i] * alpha;
-        for (int j = 0; j < n; ++j) o = fmaf(ps[j], ld_f(bv, (base + j) * p.bv_row + lane + 32 * i), o);
+        for (int j = 0; j < n; ++j) o = fmaf(ps[j], scaled(ld_f(bv, (base + j) * p.bv_row + lane + 32 * i), 1.f), o);
         acc[i] = o;
       }
       __syncwarp();

@@ -212,7 +212,8 @@ def gqa_attention_kv8(q: torch.Tensor, layer: KV8Layer, block_table: torch.Tenso
     cached rows and then, unless ``blk_k`` is None, the block's own rows ``blk_k`` / ``blk_v``
     ``[batch, n_kv, block, head_dim]``, with no mask; ``scale`` defaults to ``head_dim ** -0.5``.
     Returns ``[batch, block, n_heads * head_dim]`` in q's dtype; a sequence without any row gives
-    zeros. q and the block's rows may have any strides with contiguous rows."""
+    zeros, and what is not finite in q or the block's rows counts as NaN. q and the block's rows may
+    have any strides with contiguous rows."""
     n_pages, n_kv, page, hd, dev = _layer(layer)
     dt = _ROW_DTYPES.get(q.dtype)
     if not (dt is not None and q.dim() == 4 and q.shape[3] == hd and q.get_device() == dev):

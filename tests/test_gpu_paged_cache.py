@@ -1093,3 +1093,30 @@ def test_fp32_attention_row_by_row(lengths, s, n_kv, group, hd, page):
     out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]), *(t.to(DEV) for t in c["blk"]))
     assert _close_f32(c, out, hd ** -0.5) <= 1
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("kernel", ["default", "cuda cores"])
+@pytest.mark.parametrize("dtype,s", [(BF, 5), (BF, 65), (F32, 5), (F32, 65)])
+@pytest.mark.parametrize("what", ["q", "keys", "values"])
+@pytest.mark.parametrize("x", [float("inf"), float("-inf"), float("nan")])
+def test_attention_counts_what_is_not_finite_as_nan(kernel, dtype, s, what, x):
+    """As the append stores it: an infinity or NaN in q, the block's keys or its values gives NaN wherever it counts
+    and nowhere else, whichever kernel takes the call."""
+    c = _attn_case(13, [100, 70], s, 2, 2, 64, 64, dtype)
+    t = {"q": c["q"], "keys": c["blk"][0], "values": c["blk"][1]}[what]
+    t[(1, 3, 2, 9) if what == "q" else (1, 1, 3, 9)] = x  # sequence 1, row 3; query head 2 is of KV head 1
+    want = torch.zeros(2, s, 4, 64, dtype=torch.bool)
+    if what == "q":
+        want[1, 3, 2] = True
+    elif what == "keys":
+        want[1, :, 2:] = True
+    else:
+        want[1, :, 2:, 9] = True
+    L = _lib.lib()
+    _lib.check(L.dsm_set_attn_kernel(1 if kernel == "cuda cores" else _lib.ATTN_KERNEL_DEFAULT))
+    try:
+        out = pc.gqa_attention_kv8(c["q"].to(DEV), c["layer"], c["tg"], i32(c["lengths"]),
+                                   *(b.to(DEV) for b in c["blk"])).view(2, s, 4, 64).cpu()
+    finally:
+        _lib.check(L.dsm_set_attn_kernel(_lib.ATTN_KERNEL_DEFAULT))
+    assert torch.equal(out.isnan(), want) and bool(torch.isfinite(out[~want]).all())
