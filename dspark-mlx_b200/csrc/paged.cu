@@ -265,16 +265,14 @@ struct TrimArgs {
   int n_pages;
 };
 
-// shared memory: off [batch], left [batch]
+// one CTA; shared memory: off [batch], left [batch]
 __global__ void __launch_bounds__(kPagedThreads) paged_trim_kernel(const TrimArgs p) {
   extern __shared__ int sm[];
   __shared__ int64_t sa[kPagedWarps];
   __shared__ int sb[kPagedWarps];
-  cg::cluster_group cluster = cg::this_cluster();
   int* off = sm;
   int* left = off + p.batch;
   const int tid = threadIdx.x;
-  const int rank = int(cluster.block_rank()), ctas = int(cluster.num_blocks());
   const int free0 = min(max(*p.n_free, 0), p.n_pages);
   const int64_t most = int64_t(p.max_pages) * p.page;
   int64_t total = 0;
@@ -298,24 +296,47 @@ __global__ void __launch_bounds__(kPagedThreads) paged_trim_kernel(const TrimArg
     }
     total += t;
   }
-  cluster.sync();  // every CTA has read lengths and n_free (and its own off / left are complete)
+  __syncthreads();  // lengths and n_free have been read, off and left are complete
   if (free0 + total > p.n_pages) {  // more pages than the pool holds come back: leave everything as it is
-    if (rank == 0 && tid == 0) raise_device_error(DSM_DEV_ERR_PAGES_SHORT);
+    if (tid == 0) raise_device_error(DSM_DEV_ERR_PAGES_SHORT);
     return;
   }
   const int back = int(total);
-  if (rank == 0) {
-    for (int i = tid; i < p.batch; i += kPagedThreads) {
-      const int n = int(min(int64_t(max(p.lengths[i], 0)), most));
-      p.lengths[i] = min(max(p.keep_len[i], 0), n);
+  // an entry that is no page must not reach the stack: all are looked at before anything moves, eight per thread at a
+  // time, the first of them last, which stay
+  constexpr int kKept = 8, kRound = kKept * kPagedThreads;
+  int kept[kKept], bad = 0;
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) {
+      const int k = base + j * kPagedThreads + tid;
+      kept[j] = 0;
+      if (k >= back) continue;
+      const int i = last_not_above(off, p.batch, k);
+      kept[j] = p.table[int64_t(i) * p.table_stride + left[i] + (k - off[i])];
     }
-    if (tid == 0) *p.n_free = free0 + back;
+  };
+  for (int base = (back - 1) / kRound * kRound; base >= 0; base -= kRound) {
+    load(base);
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) bad |= kept[j] < 0 || kept[j] >= p.n_pages;
   }
-  for (int k = rank * kPagedThreads + tid; k < back; k += ctas * kPagedThreads) {
-    const int i = last_not_above(off, p.batch, k);
-    const int pg = p.table[int64_t(i) * p.table_stride + left[i] + (k - off[i])];
-    if (pg < 0 || pg >= p.n_pages) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
-    p.free_pages[free0 + back - 1 - k] = pg;
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
+    return;
+  }
+  for (int i = tid; i < p.batch; i += kPagedThreads) {
+    const int n = int(min(int64_t(max(p.lengths[i], 0)), most));
+    p.lengths[i] = min(max(p.keep_len[i], 0), n);
+  }
+  if (tid == 0) *p.n_free = free0 + back;
+  for (int base = 0; base < back; base += kRound) {
+    if (base > 0) load(base);
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) {
+      const int k = base + j * kPagedThreads + tid;
+      if (k < back) p.free_pages[free0 + back - 1 - k] = kept[j];
+    }
   }
 }
 

@@ -161,7 +161,8 @@ def _extend(dev, lengths, new_len, block_table, free_pages, n_free, page_size, m
 def paged_trim(lengths: torch.Tensor, keep_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                n_free: torch.Tensor, page_size: int) -> None:
     """Every sequence shrinks to ``min(lengths[i], keep_len[i])`` tokens (0 releases it): its surplus
-    pages go back on the stack, ``lengths`` and ``n_free`` are updated in place."""
+    pages go back on the stack, ``lengths`` and ``n_free`` are updated in place. Where a table entry is
+    outside the pool, nothing is changed and the device error word is set."""
     b, dev = _lengths(lengths)
     _tensor(keep_len, "keep_len", torch.int32, (b,), dev)
     stride, cols = _table(block_table, b, dev)

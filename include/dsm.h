@@ -390,7 +390,8 @@ int dsm_add_rms_norm(const void* x, const void* delta, int dtype, int64_t n_rows
  * paged_trim: sequence i shrinks to min(lengths[i], max(keep_len[i], 0)) tokens. Surplus pages go
  *   back on the stack in the mirrored order, so that a trim to the lengths before an extend
  *   restores the stack. Table entries behind a sequence's pages are left as they are. If more
- *   pages came back than the pool holds, nothing is changed and the error word is set.
+ *   pages came back than the pool holds (DSM_DEV_ERR_PAGES_SHORT), or one that is outside the pool
+ *   (DSM_DEV_ERR_PAGE_RANGE), nothing is changed and the error word is set.
  *   Both: all buffers int32 but slot_map; the buffers of one call must not overlap.
  *
  * kv8_append: rows k, v (element r * row_stride + h * head_stride + d; F32 or BF16) into the slots

@@ -60,7 +60,7 @@ def paged_trim(lengths: List[int], keep: List[int], table: List[List[int]], free
         k = min(max(k, 0), n)
         back += [table[i][j] for j in range(-(-k // page), -(-n // page))]
         out[i] = k
-    if n_free + len(back) > len(free):
+    if n_free + len(back) > len(free) or any(not 0 <= p < len(free) for p in back):
         return list(lengths), free, n_free, True
     for j, p in enumerate(reversed(back)):
         free[n_free + j] = p

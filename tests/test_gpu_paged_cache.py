@@ -1120,3 +1120,28 @@ def test_attention_counts_what_is_not_finite_as_nan(kernel, dtype, s, what, x):
     finally:
         _lib.check(L.dsm_set_attn_kernel(_lib.ATTN_KERNEL_DEFAULT))
     assert torch.equal(out.isnan(), want) and bool(torch.isfinite(out[~want]).all())
+
+
+# ------------------------------------------------------------------------------- ids outside the pool
+@pytest.mark.parametrize("b,longest,bad", [(5, 300, -1), (61, 700, 10 ** 6), (900, 300, -64), (8192, 500, -1)])
+def test_trim_refuses_pages_outside_the_pool(b, longest, bad):
+    """A table entry that is no page: nothing moves, and the error word says so. Entries that stay are not looked at."""
+    page = 64
+    lengths, new, table, free, n_free, tg = _tables_case(b, b, page, longest, 1, 3 * b)
+    at = max(range(b), key=lambda i: lengths[i])
+    last = -(-lengths[at] // page) - 1
+    keep = [n // 2 for n in lengths]
+    keep[at] = 0
+    tg[at, last] = bad
+    table[at][last] = bad
+    assert po.paged_trim(lengths, keep, table, free, n_free, page) == (lengths, free, n_free, True)
+    L, F, N = i32(lengths), i32(free), i32([n_free])
+    pc.paged_trim(L, i32(keep), tg, F, N, page)
+    assert L.tolist() == lengths and F.tolist() == free and N.tolist() == [n_free] and tg.tolist() == table
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
+    keep[at] = lengths[at]  # the entry stays where it is
+    want = po.paged_trim(lengths, keep, table, free, n_free, page)
+    pc.paged_trim(L, i32(keep), tg, F, N, page)
+    assert not want[3] and L.tolist() == want[0] and F.tolist() == want[1] and N.tolist() == [want[2]]
+    assert _lib.device_error() == 0
