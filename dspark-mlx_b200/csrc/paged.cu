@@ -18,8 +18,8 @@
 // even batch. The cluster barrier between the reads of lengths / n_free and their updates is
 // what lets the update be in place: a captured step replays on the buffers it leaves behind. The rows of
 // such a step are written by a second kernel on the whole GPU: 130,000 rows of 253 sequences took
-// a cluster of 8 alone 21 us, of 47 with a bisection per row; extend and trim together now take 15 us (a decode
-// step of 64 sequences 8.3 us, two launches).
+// a cluster of 8 alone 21 us, of 47 with a bisection per row; extend and trim together now take 15.8 us (a decode
+// step of 64 sequences 8.7 us, two launches), 0.4 us of it the look at the pages before they are handed out.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_extend_kernel(const Exten
   extern __shared__ int sm[];
   __shared__ int64_t sa[kPagedWarps];
   __shared__ int sb[kPagedWarps];
-  __shared__ int used_sm;
+  __shared__ int used_sm, bad_sm;
   cg::cluster_group cluster = cg::this_cluster();
   int* cu = sm;
   int* off = cu + p.batch + 1;
@@ -119,46 +119,69 @@ __global__ void __launch_bounds__(kPagedThreads) paged_extend_kernel(const Exten
   const int tid = threadIdx.x;
   const int rank = int(cluster.block_rank()), ctas = int(cluster.num_blocks());
   const int free0 = min(max(*p.n_free, 0), p.n_pages);
-  if (tid == 0) used_sm = 0;
-  __syncthreads();
-  int64_t rows_before = 0;
-  int pages_before = 0;
+  // The stack ends at a page outside the pool: should one be among those that are handed out, the sequences are gone
+  // through once more with the pages above it.
+  int avail = free0;
   bool failed = false;
-  for (int base = 0; base < p.batch; base += kPagedThreads) {
-    const int i = base + tid;
-    int n0 = -1, n1 = 0, have = 0, need = 0;
-    if (i < p.batch) {
-      n0 = p.lengths[i];
-      n1 = p.new_len[i];
-      const int64_t end = int64_t(n0) + n1;
-      if (n0 < 0 || n1 < 0 || end > int64_t(p.max_pages) * p.page || end > 0x7fffffff) {
-        failed |= n1 != 0;
-        n0 = -1;
-        n1 = max(n1, 0);
-      } else {
-        have = int((int64_t(n0) + p.page - 1) / p.page);
-        need = int((end + p.page - 1) / p.page) - have;
+  int64_t rows_before = 0;
+  for (bool again = true; again;) {
+    if (tid == 0) {
+      used_sm = 0;
+      bad_sm = 0x7fffffff;
+    }
+    __syncthreads();
+    rows_before = 0;
+    int pages_before = 0;
+    failed = false;
+    for (int base = 0; base < p.batch; base += kPagedThreads) {
+      const int i = base + tid;
+      int n0 = -1, n1 = 0, have = 0, need = 0;
+      if (i < p.batch) {
+        n0 = p.lengths[i];
+        n1 = p.new_len[i];
+        const int64_t end = int64_t(n0) + n1;
+        if (n0 < 0 || n1 < 0 || end > int64_t(p.max_pages) * p.page || end > 0x7fffffff) {
+          failed |= n1 != 0;
+          n0 = -1;
+          n1 = max(n1, 0);
+        } else {
+          have = int((int64_t(n0) + p.page - 1) / p.page);
+          need = int((end + p.page - 1) / p.page) - have;
+        }
       }
+      int64_t r0 = n1;
+      int p0 = need;
+      int64_t rt;
+      int pt;
+      cta_scan(r0, p0, rt, pt, sa, sb);
+      r0 += rows_before;
+      p0 += pages_before;
+      if (i < p.batch) {
+        // once a sequence finds too few pages or rows, so does every later one that needs any: the
+        // pages that are handed out stay one run from the top of the stack
+        const bool fits = n0 >= 0 && r0 + n1 <= p.max_rows && (need == 0 || int64_t(p0) + need <= avail);
+        failed |= !fits && n1 > 0;
+        cu[i] = int(min(r0, int64_t(0x7fffffff)));
+        off[i] = min(p0, avail);
+        len[i] = fits ? n0 : -1;
+        if (fits && need) atomicMax(&used_sm, p0 + need);
+      }
+      rows_before += rt;
+      pages_before = int(min(int64_t(pages_before) + pt, int64_t(0x3fffffff)));
     }
-    int64_t r0 = n1;
-    int p0 = need;
-    int64_t rt;
-    int pt;
-    cta_scan(r0, p0, rt, pt, sa, sb);
-    r0 += rows_before;
-    p0 += pages_before;
-    if (i < p.batch) {
-      // once a sequence finds too few pages or rows, so does every later one that needs any: the
-      // pages that are handed out stay one run from the top of the stack
-      const bool fits = n0 >= 0 && r0 + n1 <= p.max_rows && (need == 0 || int64_t(p0) + need <= free0);
-      failed |= !fits && n1 > 0;
-      cu[i] = int(min(r0, int64_t(0x7fffffff)));
-      off[i] = min(p0, free0);
-      len[i] = fits ? n0 : -1;
-      if (fits && need) atomicMax(&used_sm, p0 + need);
+    __syncthreads();
+    const int taken = used_sm;
+    for (int k = tid; k < taken; k += kPagedThreads) {
+      const int pg = p.free_pages[free0 - 1 - k];
+      if (pg < 0 || pg >= p.n_pages) atomicMin(&bad_sm, k);
     }
-    rows_before += rt;
-    pages_before = int(min(int64_t(pages_before) + pt, int64_t(0x3fffffff)));
+    __syncthreads();
+    again = bad_sm < taken;
+    if (again) {
+      avail = bad_sm;
+      if (rank == 0 && tid == 0) raise_device_error(DSM_DEV_ERR_PAGE_RANGE);
+      __syncthreads();  // bad_sm has been read
+    }
   }
   if (tid == 0) cu[p.batch] = int(min(rows_before, int64_t(0x7fffffff)));
   if (failed && rank == 0) raise_device_error(DSM_DEV_ERR_PAGES_SHORT);

@@ -131,7 +131,8 @@ def paged_extend(lengths: torch.Tensor, new_len: torch.Tensor, block_table: torc
     """Every sequence grows by ``new_len[i]`` tokens: pages off the stack ``free_pages[:n_free]`` go
     into ``block_table``, ``lengths`` and ``n_free`` are updated in place. Returns the step's rows;
     ``max_rows`` (known on the host) bounds them, rows behind the last sequence get slot -1. A
-    sequence that finds no pages, table or rows keeps its length and sets the device error word."""
+    sequence that finds no pages, table or rows keeps its length and sets the device error word; a page
+    outside the pool ends the stack."""
     b, dev = _lengths(lengths)
     _tensor(new_len, "new_len", torch.int32, (b,), dev)
     stride, cols = _table(block_table, b, dev)

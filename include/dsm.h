@@ -386,7 +386,8 @@ int dsm_add_rms_norm(const void* x, const void* delta, int dtype, int64_t n_rows
  *   rows behind the last sequence get slot -1, position 0. A sequence that cannot be served (a
  *   negative length, more tokens than its table or int32 holds, no pages or rows left, or a
  *   sequence before it ran out of either) keeps its length; its rows get slot -1, position 0, and
- *   the error word is set (DSM_DEV_ERR_PAGES_SHORT).
+ *   the error word is set (DSM_DEV_ERR_PAGES_SHORT). The stack ends at a page outside the pool: what
+ *   lies below it is not handed out (DSM_DEV_ERR_PAGE_RANGE).
  * paged_trim: sequence i shrinks to min(lengths[i], max(keep_len[i], 0)) tokens. Surplus pages go
  *   back on the stack in the mirrored order, so that a trim to the lengths before an extend
  *   restores the stack. Table entries behind a sequence's pages are left as they are. If more

@@ -26,6 +26,9 @@ def paged_extend(lengths: List[int], new: List[int], table: List[List[int]], fre
     n_free = min(max(n_free, 0), len(free))
     slots, pos = [-1] * max_rows, [0] * max_rows
     cu, wanted, failed, top = [0], 0, False, n_free
+    usable = 0  # the stack ends at a page outside the pool
+    while usable < n_free and 0 <= free[n_free - 1 - usable] < len(free):
+        usable += 1
     for i, (n, add) in enumerate(zip(list(lengths), new)):
         rows = max(add, 0)
         first = cu[-1]
@@ -36,7 +39,7 @@ def paged_extend(lengths: List[int], new: List[int], table: List[List[int]], fre
         have, want = -(-n // page), -(-(n + add) // page)
         need = want - have
         wanted += need
-        if first + rows > max_rows or (need and wanted > n_free):
+        if first + rows > max_rows or (need and wanted > usable):
             failed |= rows > 0
             continue
         for j in range(have, want):

@@ -1145,3 +1145,26 @@ def test_trim_refuses_pages_outside_the_pool(b, longest, bad):
     pc.paged_trim(L, i32(keep), tg, F, N, page)
     assert not want[3] and L.tolist() == want[0] and F.tolist() == want[1] and N.tolist() == [want[2]]
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("b,new_most,where,bad", [
+    (1, 5, 0, -1), (30, 150, 0, -2), (30, 150, 7, 10 ** 6), (30, 150, 40, -64), (90, 384, 100, -1), (700, 3, 60, 10 ** 9),
+])
+def test_extend_stops_at_a_page_outside_the_pool(b, new_most, where, bad):
+    """A free page that is none ends the stack there: who would need it, or one below, is not served."""
+    page = 64
+    lengths, new, table, free, n_free, tg = _tables_case(b + where, b, page, 300, new_most, 60 + b * (new_most // page + 2))
+    new = [max(1, n) for n in new]
+    new[0] += page
+    need = sum(-(-(n + a) // page) - -(-n // page) for n, a in zip(lengths, new))
+    where = min(where, need - 1)
+    free[n_free - 1 - where] = bad
+    max_rows = sum(new) + 3
+    want = po.paged_extend(lengths, new, table, free, n_free, page, max_rows)
+    assert want[6] and want[2] >= n_free - where
+    L, F, N, rows = _run_extend(lengths, new, tg, free, n_free, page, max_rows)
+    assert L.tolist() == want[0] and tg.tolist() == want[1] and N.tolist() == [want[2]] and F.tolist() == free
+    assert rows.cu_rows.tolist() == want[3] and rows.slot_map.tolist() == want[4]
+    assert rows.positions.tolist() == want[5]
+    with pytest.raises(_lib.DsmError, match="outside the pool"):
+        _lib.raise_device_error()
