@@ -958,15 +958,16 @@ int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
   if (smem > 227 * 1024) return DSM_ERR_UNSUPPORTED;
   pl.k_slots = slots / 2;
   pl.v_slots = slots - pl.k_slots;
+  // before the maps: cuTensorMapEncodeTiled wants a current context, which a host thread's first runtime call makes
+  auto kern = kv8_umma_kernel<HD, NR>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return check_launch("gqa_attn_kv8 smem attribute");
   CUtensorMap kmap{}, vmap{};
   const int64_t groups = int64_t(a.n_pages) * a.n_kv * (a.page / kTile);
   int st = byte_map(&vmap, a.v_codes, groups * HD, kTile, kTile, HD, true);
   if (st == DSM_OK && HD == 64) st = byte_map(&kmap, a.k_codes, groups * kTile, 64, 64, kTile, true);
   if (st == DSM_OK && HD == 256) st = byte_map(&kmap, a.k_codes, groups * kTile, 256, 128, kTile, false);
   if (st != DSM_OK) return st;
-  auto kern = kv8_umma_kernel<HD, NR>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return check_launch("gqa_attn_kv8 smem attribute");
   kern<<<unsigned(pl.sp.ctas), C::kThreads, size_t(smem), s>>>(a, pl, kmap, vmap);
   st = check_launch("gqa_attn_kv8");
   return st != DSM_OK ? st : kv8_combine(a, pl.sp, HD, DSM_DT_BF16, s);

@@ -1168,3 +1168,36 @@ def test_extend_stops_at_a_page_outside_the_pool(b, new_most, where, bad):
     assert rows.positions.tolist() == want[5]
     with pytest.raises(_lib.DsmError, match="outside the pool"):
         _lib.raise_device_error()
+
+
+# ------------------------------------------------------------------------------- host threads
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_host_thread_whose_first_cuda_call_is_the_attention(dtype):
+    """The C entry point on a thread that has no context yet."""
+    import ctypes
+    import threading
+
+    c = _attn_case(17, [100, 65], 1, 2, 2, 128, 64, dtype, with_block=False)
+    L, q, n = _lib.lib(), c["q"].to(DEV), i32(c["lengths"])
+    size = L.dsm_gqa_attn_kv8_workspace_bytes(2, 1, 4, 2, 128)
+    ws, out = torch.empty(size, dtype=torch.uint8, device=DEV), torch.empty(2, 1, 512, dtype=dtype, device=DEV)
+    layer = [t.data_ptr() for t in c["layer"]]
+    desc = _lib.KV8AttnDesc(q_batch_stride=512, q_row_stride=512, q_head_stride=128, table_stride=c["tg"].stride(0),
+                            k_codes=layer[0], v_codes=layer[1], k_scale=layer[2], v_scale=layer[3],
+                            dtype=_lib.DT_BF16 if dtype == BF else _lib.DT_F32, batch=2, block=1, n_heads=4, n_kv=2,
+                            head_dim=128, page_size=64, n_pages=c["layer"].k_codes.shape[0], max_pages=c["tg"].shape[1],
+                            scale=128 ** -0.5)
+    args = [t.data_ptr() for t in (q, c["tg"], n)] + [None, None, out.data_ptr(), ws.data_ptr(), size,
+                                                      torch.cuda.current_stream().cuda_stream]
+    torch.cuda.synchronize()
+    rc = []
+
+    def run():
+        rc.append((L.dsm_gqa_attn_kv8(ctypes.addressof(desc), *args), L.dsm_last_error_message().decode()))
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    assert rc[0][0] == 0, rc[0][1]
+    torch.cuda.synchronize()
+    _check_attn(c, out=out)
