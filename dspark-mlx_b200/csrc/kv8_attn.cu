@@ -933,7 +933,8 @@ int launch_mma(const AttnArgs& a, const MmaShape& sh, MmaPlan pl, int ctas, cuda
   if (smem > kMmaSmemMax) return DSM_ERR_UNSUPPORTED;
   pl.depth = depth;
   auto k = kv8_attn_mma_kernel<HD>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  // all that a CTA may have, whatever this call takes: the kernel's limit is every host thread's
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmaSmemMax) != cudaSuccess)
     return check_launch("gqa_attn_kv8 smem attribute");
   k<<<unsigned(ctas), mma_warps(HD) * 32, size_t(smem), s>>>(a, pl);
   const int st = check_launch("gqa_attn_kv8");

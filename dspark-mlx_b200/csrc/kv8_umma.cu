@@ -945,6 +945,8 @@ int byte_map(CUtensorMap* map, const void* base, int64_t rows, int width, int bo
 int rows_of(int rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 int ctas_per_sm(int nr, int hd) { return hd == 256 || nr == 64 ? 1 : 2; }
 
+constexpr int kSmemMax = 227 * 1024;
+
 template <int HD, int NR>
 int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
   using C = Cfg<HD, NR>;
@@ -955,12 +957,13 @@ int launch(const AttnArgs& a, UmmaPlan pl, cudaStream_t s) {
   int slots = 2 * kMaxSlots;
   while (slots > 4 && umma_smem(HD, C::NM, slots, a.batch).bytes > room) --slots;
   const int smem = umma_smem(HD, C::NM, slots, a.batch).bytes;
-  if (smem > 227 * 1024) return DSM_ERR_UNSUPPORTED;
+  if (smem > kSmemMax) return DSM_ERR_UNSUPPORTED;
   pl.k_slots = slots / 2;
   pl.v_slots = slots - pl.k_slots;
-  // before the maps: cuTensorMapEncodeTiled wants a current context, which a host thread's first runtime call makes
+  // All that a CTA may have, whatever this call takes: the kernel's limit is every host thread's. Before the maps:
+  // cuTensorMapEncodeTiled wants a current context, which a host thread's first runtime call makes
   auto kern = kv8_umma_kernel<HD, NR>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax) != cudaSuccess)
     return check_launch("gqa_attn_kv8 smem attribute");
   CUtensorMap kmap{}, vmap{};
   const int64_t groups = int64_t(a.n_pages) * a.n_kv * (a.page / kTile);

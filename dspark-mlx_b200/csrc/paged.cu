@@ -363,10 +363,16 @@ __global__ void __launch_bounds__(kPagedThreads) paged_trim_kernel(const TrimArg
   }
 }
 
+// words of shared memory
+constexpr size_t extend_words(int batch) { return size_t(3 * batch + 1); }
+constexpr size_t trim_words(int batch) { return size_t(2 * batch); }
+
 template <typename A>
-int launch_cluster(void (*kernel)(const A), const A& args, int ctas, size_t smem, void* stream, const char* what) {
+int launch_cluster(void (*kernel)(const A), const A& args, int ctas, size_t smem, size_t smem_most, void* stream,
+                   const char* what) {
+  // what the largest batch takes, whatever this one does: the kernel's limit is every host thread's
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_most)) != cudaSuccess)
     return check_launch(what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas));
@@ -408,8 +414,8 @@ extern "C" int dsm_paged_extend(int32_t* lengths, const int32_t* new_len, int ba
   const bool many = max_rows > 4 * kPagedThreads;
   const ExtendArgs a = {lengths,  new_len, batch,   page_size, block_table, table_stride, max_pages, free_pages,
                         n_free,   n_pages, cu_rows, slot_map,  positions,   max_rows, per_page,    many};
-  const int st = launch_cluster(paged_extend_kernel, a, many ? kPagedCluster : 1, size_t(3 * batch + 1) * 4, stream,
-                                "dsm_paged_extend");
+  const int st = launch_cluster(paged_extend_kernel, a, many ? kPagedCluster : 1, extend_words(batch) * 4,
+                                extend_words(kKv8MaxBatch) * 4, stream, "dsm_paged_extend");
   if (st != DSM_OK || !many) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ceil_div(max_rows, int64_t(kRowThreads * kRowsPerLane))));
@@ -436,5 +442,6 @@ extern "C" int dsm_paged_trim(int32_t* lengths, const int32_t* keep_len, int bat
   if (batch == 0) return DSM_OK;
   DSM_REQUIRE(lengths && keep_len && block_table && free_pages && n_free, "dsm_paged_trim: NULL pointer");
   const TrimArgs a = {lengths, keep_len, batch, page_size, block_table, table_stride, max_pages, free_pages, n_free, n_pages};
-  return launch_cluster(paged_trim_kernel, a, 1, size_t(2 * batch) * 4, stream, "dsm_paged_trim");
+  return launch_cluster(paged_trim_kernel, a, 1, trim_words(batch) * 4, trim_words(kKv8MaxBatch) * 4, stream,
+                        "dsm_paged_trim");
 }

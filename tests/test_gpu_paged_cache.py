@@ -1201,3 +1201,60 @@ def test_a_host_thread_whose_first_cuda_call_is_the_attention(dtype):
     assert rc[0][0] == 0, rc[0][1]
     torch.cuda.synchronize()
     _check_attn(c, out=out)
+
+
+@pytest.mark.parametrize("what", ["extend", "trim", "bf16 attention", "fp32 attention"])
+def test_calls_of_unlike_sizes_from_two_threads(what):
+    """Two host threads, each with a stream of its own, call the C entry points with batches that need unlike amounts of
+    shared memory: what one sets must not take the other's launch."""
+    import ctypes
+    import threading
+
+    L, kept = _lib.lib(), []
+
+    def ptr(t):
+        kept.append(t)
+        return t.data_ptr()
+
+    def setup(b, stream):
+        zeros, table, pool, n = (ptr(torch.zeros(k, dtype=torch.int32, device=DEV)) for k in (b, 2 * b, 2, 1))
+        lengths = ptr(torch.zeros(b, dtype=torch.int32, device=DEV))
+        if what == "extend":
+            cu, slots, pos = (ptr(torch.zeros(k, dtype=t, device=DEV)) for k, t in
+                              ((b + 1, torch.int32), (1, torch.int64), (1, torch.int32)))
+            return lambda: L.dsm_paged_extend(lengths, zeros, b, 64, table, 2, 2, pool, n, 2, cu, slots, pos, 1, stream)
+        if what == "trim":
+            return lambda: L.dsm_paged_trim(lengths, zeros, b, 64, table, 2, 2, pool, n, 2, stream)
+        layer = [ptr(t) for t in _pool(0, 2, 1, 64, 128)[4]]
+        dt, dtype = (_lib.DT_BF16, BF) if what[0] == "b" else (_lib.DT_F32, F32)
+        q, out = (ptr(torch.zeros(b * 128, dtype=dtype, device=DEV)) for _ in range(2))
+        size = L.dsm_gqa_attn_kv8_workspace_bytes(b, 1, 1, 1, 128)
+        ws = ptr(torch.zeros(size, dtype=torch.uint8, device=DEV))
+        desc = _lib.KV8AttnDesc(q_batch_stride=128, q_row_stride=128, q_head_stride=128, table_stride=2, k_codes=layer[0],
+                                v_codes=layer[1], k_scale=layer[2], v_scale=layer[3], dtype=dt, batch=b, block=1,
+                                n_heads=1, n_kv=1, head_dim=128, page_size=64, n_pages=2, max_pages=2, scale=1.0)
+        kept.append(desc)
+        d = ctypes.addressof(desc)
+        return lambda: L.dsm_gqa_attn_kv8(d, q, table, lengths, None, None, out, ws, size, stream)
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sizes = (8192, 6500) if what in ("extend", "trim") else (8192, 2)
+    calls = [setup(b, s.cuda_stream) for b, s in zip(sizes, streams)]
+    torch.cuda.synchronize()
+    errors, start = [], threading.Barrier(2)
+
+    def run(call):
+        start.wait()
+        for _ in range(10000):
+            if call():
+                errors.append(L.dsm_last_error_message().decode())
+                return
+
+    threads = [threading.Thread(target=run, args=(call,)) for call in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
+    assert _lib.device_error() == 0
