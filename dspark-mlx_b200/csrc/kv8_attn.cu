@@ -154,10 +154,13 @@ int launch_core(const AttnArgs& a, cudaStream_t s) {
 // sequences of 4096 keys, 8 KV heads of 4 rows). Sums, weights and maxima are fp32. The tensor cores' own additions cut off what they round, too
 // coarse for fp32 calls over long sums: products go into the fp32 sums a few steps at a time, by CUDA cores.
 //
-// What bounds it: the products, two terms of q (and of the weights) for each code at 0.46 mma.sync per clock
-// and SM: 64 keys of head_dim 128 and 16 rows take 512 of them, 1,100 cycles against the ~700 that their bytes
-// take at the copy peak. The tcgen05 kernel multiplies the codes without conversion, but e4m3 terms of an
-// fp32 row would be four. 23 us for 8 sequences of up to 1000 rows, 4 KV heads of 20 rows.
+// What bounds it: for long sequences the products, two terms of q (and of the weights) for each code at 0.46
+// mma.sync per clock and SM: 64 keys of head_dim 128 and 16 rows take 512 of them, 1,100 cycles against the ~700
+// that their bytes take at the copy peak (32 sequences of 4096 keys, 8 KV heads of 4 rows: 93 us, 3 TB/s). The
+// tcgen05 kernel multiplies the codes without conversion, but e4m3 terms of an fp32 row would be four. Short
+// sequences are bound by what a unit costs: 8 sequences, 4 KV heads of 20 rows, take 12.3 us at one tile each, 13.2
+// at four (launch, scan, staging, the lanes' join), 2 more with own rows, 7 more as soon as units are cut (a second
+// unit's staging and the join: 20.3 us at eight tiles, 24.5 at 32). Hence 23 us for such sequences of up to 1000 keys.
 //
 // Layout of the work. A unit is one sequence's KV head (and block of up to 128 query rows); its
 // tiles of 64 keys follow one another, and all units' tiles form one line that is cut into ranges of
@@ -169,7 +172,10 @@ int launch_core(const AttnArgs& a, cudaStream_t s) {
 // values' half after the sums, and waits for no other lane in the main loop. The block's own rows are
 // 16-key tiles of whichever CTA holds the unit's last tile, read straight from the caller's tensors.
 constexpr int kMaxDepth = 2;  // stages per lane, where they fit
-constexpr int kUnitCost = 6;  // a unit's q, join and output, in tiles
+// a unit's q, join and output, in tiles, and the least that a range should cost. 20 ragged sequences of up to 3000, 4 KV
+// heads of 20 rows of 64, 128 and 256: 20.5, 26.8 and 43.1 us; with cost 3 23.0, 29.5, 44.8; with 10 23.8, 31.3, 48.8.
+// Ranges of 12 are slower still (24.5, 32.1, 58.8); of 3 as fast there, and up to 25% faster for equal short sequences.
+constexpr int kUnitCost = 6;
 // warps per CTA: a stage of head_dim 256 holds 32 KB, so four lanes fill shared memory
 constexpr int mma_warps(int hd) { return hd == 256 ? 4 : 8; }
 constexpr float kPScale = 6.f;  // weights at the reference enter f16 as 2^6,

@@ -11,7 +11,7 @@
 // e5m2's smallest step, 2^-17. m is the row's reference: its maximum when it was last set, plus three, so that the
 // largest weight is 2^12 or more, and 2^-29 of it is the most that is lost of any beside its 2^-11. (An e4m3 and
 // an e5m2 term, relative to 2^8, left 2^-7 of a weight down to 2^-12 of the largest, an eighth at 2^-16 and nothing
-// below 2^-22: a tail behind a heavy key that gives nothing was off by 2 to 10 percent.) m is set again, for every
+// below 2^-22: a tail behind a heavy key that gives nothing was off by 1 to 7 percent.) m is set again, for every
 // row that has risen, when a weight would pass 2^15.75, and the sums in tensor memory are then rescaled (2,200 to
 // 3,000 cycles, waiting for the products that make them: with a reference just above the maximum, or moved for
 // one row alone, most of a unit's first steps paid that). The page's value exponent is folded into the weights
@@ -61,7 +61,7 @@ constexpr float kPMax = 15.75f;  // 2^15.75 = 55,109 still fits e5m2 and f16
 constexpr float kPHead = 3.f;    // a new reference lies this much above the maximum: the maximum's own weight is 2^12
 constexpr int kPTerms = 3;       // e5m2 terms of a weight
 
-// steps whose weights are held: one where a second would cost a copy's slot (attn_long 74.7 us with one, 76 with two)
+// steps whose weights are held: one where a second would cost a copy's slot (one sequence of 131,071 keys 70.0 us with one, 71.1 with two)
 __host__ __device__ constexpr int p_buffers(int hd, int nm) { return hd == 128 && nm <= 32 ? 1 : 2; }
 
 template <int HD, int NR>  // NR query rows per CTA: 4, 8, 16, 32 or 64
@@ -545,8 +545,9 @@ __global__ void __launch_bounds__(Cfg<HD, NR>::kThreads, Cfg<HD, NR>::CTAS)
     const int row_r = tid / TPR, row_d = tid % TPR * VB;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const int group = p.n_heads / p.n_kv;
-    // rows of the sums at a time: 8 keep the 96 registers of two CTAs per SM from spilling (attn_long 74.7 -> 70.0 us),
-    // at head_dim 64 their second round costs more (attn_narrow_heads 27.4 us, with 8 rows 29.3)
+    // rows of the sums at a time: 8 keep the 96 registers of two CTAs per SM from spilling (one sequence of 131,071 keys
+    // 70.0 us, with all 16 74.7), at head_dim 64 their second round costs more (33 sequences of up to 5001, 56 rows:
+    // 27.4 us, with 8 rows 29.3)
     constexpr int RP = HD == 64 || RW < 8 ? RW : 8;
     float* const red = reds + grp * 4 * kGroupRows;
     const float* const my_c = row_c + g0;
@@ -1007,10 +1008,12 @@ int kv8_umma(const AttnArgs& a, int hd, void* ws, cudaStream_t s) {
   if (int64_t(a.block) * a.n_heads * hd > 0x7fffffff) return DSM_ERR_UNSUPPORTED;
   const int most_ctas = ctas_per_sm(nr, hd) * num_sms();
   pl.sp.ctas = int(std::min<int64_t>(most_ctas, most));
-  // A unit's staging, first step and result take as long as ten tiles (cost 6: 61 ragged sequences 107 us
-  // instead of 95, 16 equal ones 42 both; 14: 90 and 44). Cuts that move further leave uneven ranges (snap 4: 91 us
-  // instead of 90; 8: 93, and 16 sequences 51 instead of 42), none at all more parts to join. Ranges of eight
-  // tiles' cost give each unit of a short request a CTA (8 units of 3 tiles 10.8 us, at 12 two to a CTA 18.6).
+  // A unit's staging, first step and result take as long as ten tiles. Measured at 28 rows of head_dim 128 for 61 ragged
+  // sequences and for 16 equal ones: cost 6 / 10 / 14 92, 81, 74 us and 37, 38, 39; at head_dim 64 and 256 and 4, 16, 28
+  // and 56 rows, ragged, cost 6 is up to 22% slower than 10, and 14 from 4% faster to 8% slower (4 rows of 256).
+  // Cuts that move further leave uneven ranges (snap 0 / 2 / 4 / 8: 81, 81, 79, 78 us and 39, 38, 40, 47; 4 instead of
+  // 2 is 1% faster to 9% slower at the other widths), none at all leave one short request's units in pieces (11.4 us ->
+  // 13.3). Ranges of at least 4, 8 or 12 tiles' cost differ by 2%, but at 16 rows, where 12 is 9 to 13% slower.
   pl.sp.cost = 10;
   pl.sp.snap = 2;
   pl.sp.least = 8;

@@ -6,14 +6,15 @@ and V = max |v| of a sequence:
 
 * the result is rounded once: u |o|;
 * a score that is off by ds moves each weight by a factor of e^ds, numerator and denominator alike:
-  at most 2 ds V. bf16 calls split q and the weights into two e4m3 terms each. q: a term's half step
+  at most 2 ds V. bf16 calls split q into two e4m3 terms. A term's half step
   is 2^-4 of its value, so two leave 2^-8 |q_d|, and 2^-10 of e4m3's unit (its smallest step 2^-9,
   halved) of a row scaled to at least 224: 2^-17 max |q|; the products are exact and their fp32 sums
   add less than 2^-18 S. So ds <= (2^-8 + 2^-18) S in the worst case; but bf16's q has 8
   significant bits, a first term takes 4, the residual at most 4 with its sign, and is exact where it
   reaches e4m3's normals: 2^-17 max|q| sum|k| scale is what is left, held below 2^-17 * head_dim * S;
-* the weights' two terms leave 2^-8 of each, and 2^-18 of the largest of 64: at most
-  (2^-8 + 2^-12) V, and their sum is taken before the rounding;
+* the weights' terms leave less than 2^-8 of each, and 2^-18 of the largest of 64: at most
+  (2^-8 + 2^-12) V, and their sum is taken before the rounding (three e5m2 terms of an f16 leave 2^-11 and 2^-29 of
+  the largest: ``_close`` below holds each row to that);
 * fp32 calls split into two f16 terms (2^-22 each), or use fp32 products: ds <= (2^-21 + (hd + 8)
   2^-24) S, weights 2^-21 + (n / 32 + 64) 2^-24 for n summed rows.
 """
