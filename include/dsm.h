@@ -413,7 +413,9 @@ int dsm_add_rms_norm(const void* x, const void* delta, int dtype, int64_t n_rows
  *   zeros. Lengths below 0 count as 0; a length past the table is cut to it, and a page outside
  *   the pool counts as absent, both with DSM_DEV_ERR_PAGE_RANGE. What the cache holds behind a
  *   sequence's length is never read as a number. What is not finite in q or the block's own rows
- *   counts as NaN, as the append stores it. Strides are in elements; head_dim values of a
+ *   counts as NaN, as the append stores it. Rounding beside the result's own: a BF16 call's weights
+ *   to 2^-11, and 2^-29 of the row's largest times the largest value scale; an F32 call's factors
+ *   to 2^-22, and weights 2^-42 of the largest. Strides are in elements; head_dim values of a
  *   row are contiguous. out in F32 is 8-byte aligned. workspace: dsm_gqa_attn_kv8_workspace_bytes,
  *   16-byte aligned. */
 typedef struct dsm_kv8_attn_desc {
